@@ -126,6 +126,23 @@ _SIGS = {
     "mi_bias_gelu_forward_to_half": (c_int, [P, P, P, c_int, c_int, P]),
     "mi_bias_gelu_forward_to_bf16": (c_int, [P, P, P, c_int, c_int, P]),
     "mi_relu_backward_with_bias_backward_half_mask": (c_int, [P, P, P, P, c_int, c_int, P]),
+    # mixture of experts
+    "mi_moe_gate_forward": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_moe_gate_backward": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_moe_sort": (c_int, [P, P, P, P, c_int, c_int, P]),
+    "mi_moe_sort_workspace": (c_size_t, [c_int, c_int]),
+    "mi_moe_dispatch_forward": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_moe_dispatch_backward": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_moe_combine_forward": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_moe_combine_backward": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    # 8-bit checkpoints
+    "mi_float_to_ckpt8": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
+    "mi_ckpt8_to_float": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
+    "mi_bias_gelu_forward_ckpt8":
+        (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_gelu_backward_with_bias_backward_ckpt8":
+        (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_gelu_backward_ckpt8_workspace": (c_size_t, [c_int, c_int, c_int]),
 }
 
 for _name, (_res, _args) in _SIGS.items():
@@ -477,3 +494,191 @@ def relu_backward_with_bias_backward_half_mask(mask16, grad_out, grad_in, dbias,
     _check(lib.mi_relu_backward_with_bias_backward_half_mask(_h(mask16), _f(grad_out),
                                                              _f(grad_in), _f(dbias), rows, cols,
                                                              _stream(stream)))
+
+
+# ----- typed rows: fp32, fp16 or bf16 tensors ------------------------------------
+
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+CKPT8_INT8, CKPT8_E4M3 = 0, 1
+CKPT8_BLOCK = 32
+
+
+def _type_of(rows, type):
+    """MI_TYPE_* of a tensor; of an int address, the `type` given."""
+    import torch
+    if isinstance(rows, torch.Tensor):
+        code = {torch.float32: TYPE_F32, torch.float16: TYPE_F16,
+                torch.bfloat16: TYPE_BF16}.get(rows.dtype)
+        if code is None:
+            raise ValueError(f"rows of dtype {rows.dtype}: float32, float16 or bfloat16 expected")
+        if type is not None and type != code:
+            raise ValueError(f"rows of dtype {rows.dtype} given as type {type}")
+        return code
+    if type is None:
+        raise ValueError("rows given by address need their type (TYPE_F32, TYPE_F16, TYPE_BF16)")
+    return type
+
+
+def _buf(x, count, *dtypes):
+    """Device address of a buffer that the call takes `count` elements of: a
+    contiguous tensor of one of the dtypes, on the current device, with at
+    least that many elements, or a raw int address."""
+    if x is None or isinstance(x, int):
+        return x
+    import torch
+    p = _ptr(x)
+    if x.dtype not in dtypes:
+        raise ValueError(f"tensor dtype {x.dtype}, expected {' or '.join(map(str, dtypes))}")
+    if x.numel() < count:
+        raise ValueError(f"tensor of {x.numel()} elements, at least {count} are needed")
+    if x.get_device() != torch.cuda.current_device():
+        raise ValueError(f"tensor on cuda:{x.get_device()}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return p
+
+
+def _row_dtype(type):
+    import torch
+    return {TYPE_F32: torch.float32, TYPE_F16: torch.float16, TYPE_BF16: torch.bfloat16}.get(type)
+
+
+def _codes_dtypes(fmt):
+    import torch
+    return (torch.uint8, torch.int8 if fmt == CKPT8_INT8 else torch.float8_e4m3fn)
+
+
+# ----- mixture of experts ----------------------------------------------------------
+
+def moe_gate_forward(logits, ids, weights, tokens, experts, k, renormalise=True, type=None,
+                     stream=None):
+    """The k largest of each token's logits [tokens, experts] into ids [tokens, k] (int32), and
+    their softmax weights [tokens, k] over the chosen experts (renormalise) or over all."""
+    import torch
+    t = _type_of(logits, type)
+    _check(lib.mi_moe_gate_forward(_buf(logits, tokens * experts, _row_dtype(t)),
+                                   _buf(ids, tokens * k, torch.int32),
+                                   _buf(weights, tokens * k, torch.float32), tokens, experts, k,
+                                   int(renormalise), t, _stream(stream)))
+
+
+def moe_gate_backward(logits, ids, weights, dweights, dlogits, tokens, experts, k,
+                      renormalise=True, type=None, stream=None):
+    """dlogits from dweights; logits may be None if renormalise."""
+    import torch
+    t = _type_of(dlogits, type)
+    _check(lib.mi_moe_gate_backward(_buf(logits, tokens * experts, _row_dtype(t)),
+                                    _buf(ids, tokens * k, torch.int32),
+                                    _buf(weights, tokens * k, torch.float32),
+                                    _buf(dweights, tokens * k, torch.float32),
+                                    _buf(dlogits, tokens * experts, _row_dtype(t)), tokens,
+                                    experts, k, int(renormalise), t, _stream(stream)))
+
+
+def moe_sort(ids, offsets, order, position, slots, experts, stream=None):
+    """Sorts the slots' expert ids stably: offsets [experts + 1], order [slots] (may be None) and
+    position [slots], all int32."""
+    import torch
+    _check(lib.mi_moe_sort(_buf(ids, slots, torch.int32), _buf(offsets, experts + 1, torch.int32),
+                           _buf(order, slots, torch.int32), _buf(position, slots, torch.int32),
+                           slots, experts, _stream(stream)))
+
+
+def moe_dispatch_forward(x, position, out, tokens, k, rows, cols, type=None, stream=None):
+    """out[position[t * k + j]] = x[t]."""
+    import torch
+    t = _type_of(x, type)
+    _check(lib.mi_moe_dispatch_forward(_buf(x, tokens * cols, _row_dtype(t)),
+                                       _buf(position, tokens * k, torch.int32),
+                                       _buf(out, rows * cols, _row_dtype(t)), tokens, k, rows,
+                                       cols, t, _stream(stream)))
+
+
+def moe_dispatch_backward(dout, position, dx, tokens, k, rows, cols, type=None, stream=None):
+    """dx[t] = sum over j of dout[position[t * k + j]]."""
+    import torch
+    t = _type_of(dx, type)
+    _check(lib.mi_moe_dispatch_backward(_buf(dout, rows * cols, _row_dtype(t)),
+                                        _buf(position, tokens * k, torch.int32),
+                                        _buf(dx, tokens * cols, _row_dtype(t)), tokens, k, rows,
+                                        cols, t, _stream(stream)))
+
+
+def moe_combine_forward(y, position, weights, out, tokens, k, rows, cols, type=None, stream=None):
+    """out[t] = sum over j of weights[t, j] * y[position[t * k + j]]."""
+    import torch
+    t = _type_of(out, type)
+    _check(lib.mi_moe_combine_forward(_buf(y, rows * cols, _row_dtype(t)),
+                                      _buf(position, tokens * k, torch.int32),
+                                      _buf(weights, tokens * k, torch.float32),
+                                      _buf(out, tokens * cols, _row_dtype(t)), tokens, k, rows,
+                                      cols, t, _stream(stream)))
+
+
+def moe_combine_backward(dout, y, position, weights, dy, dweights, tokens, k, rows, cols,
+                         type=None, stream=None):
+    """dy[position[t * k + j]] = weights[t, j] * dout[t]; dweights[t, j] = dout[t] . y[position
+    [t * k + j]].  dy may be y."""
+    import torch
+    t = _type_of(dout, type)
+    _check(lib.mi_moe_combine_backward(_buf(dout, tokens * cols, _row_dtype(t)),
+                                       _buf(y, rows * cols, _row_dtype(t)),
+                                       _buf(position, tokens * k, torch.int32),
+                                       _buf(weights, tokens * k, torch.float32),
+                                       _buf(dy, rows * cols, _row_dtype(t)),
+                                       _buf(dweights, tokens * k, torch.float32), tokens, k, rows,
+                                       cols, t, _stream(stream)))
+
+
+# ----- activations kept in 8 bits ---------------------------------------------------
+
+def ckpt8_scales(rows, cols) -> int:
+    """Bytes of a checkpoint's scales."""
+    return rows * -(-cols // CKPT8_BLOCK)
+
+
+def float_to_ckpt8(inp, q, scales, rows, cols, fmt=CKPT8_INT8, type=None, stream=None):
+    import torch
+    t = _type_of(inp, type)
+    _check(lib.mi_float_to_ckpt8(_buf(inp, rows * cols, _row_dtype(t)),
+                                 _buf(q, rows * cols, *_codes_dtypes(fmt)),
+                                 _buf(scales, ckpt8_scales(rows, cols), torch.uint8), rows, cols,
+                                 fmt, t, _stream(stream)))
+
+
+def ckpt8_to_float(q, scales, out, rows, cols, fmt=CKPT8_INT8, type=None, stream=None):
+    import torch
+    t = _type_of(out, type)
+    _check(lib.mi_ckpt8_to_float(_buf(q, rows * cols, *_codes_dtypes(fmt)),
+                                 _buf(scales, ckpt8_scales(rows, cols), torch.uint8),
+                                 _buf(out, rows * cols, _row_dtype(t)), rows, cols, fmt, t,
+                                 _stream(stream)))
+
+
+def bias_gelu_forward_ckpt8(inp, bias, offsets, out, q, scales, rows, cols, groups=1,
+                            fmt=CKPT8_INT8, type=None, stream=None):
+    """out = gelu(inp + bias[g]) and the checkpoint of inp; offsets (groups + 1 row numbers, None
+    for one group of all rows) say which rows are group g's."""
+    import torch
+    t = _type_of(inp, type)
+    _check(lib.mi_bias_gelu_forward_ckpt8(_buf(inp, rows * cols, _row_dtype(t)),
+                                          _buf(bias, groups * cols, torch.float32),
+                                          _buf(offsets, groups + 1, torch.int32),
+                                          _buf(out, rows * cols, _row_dtype(t)),
+                                          _buf(q, rows * cols, *_codes_dtypes(fmt)),
+                                          _buf(scales, ckpt8_scales(rows, cols), torch.uint8),
+                                          rows, cols, groups, fmt, t, _stream(stream)))
+
+
+def gelu_backward_with_bias_backward_ckpt8(q, scales, bias, offsets, grad_out, grad_in, act, dbias,
+                                           rows, cols, groups=1, fmt=CKPT8_INT8, type=None,
+                                           stream=None):
+    """grad_in, the activation again (act; None: not wanted) and dbias += from the checkpoint."""
+    import torch
+    t = _type_of(grad_out, type)
+    _check(lib.mi_gelu_backward_with_bias_backward_ckpt8(
+        _buf(q, rows * cols, *_codes_dtypes(fmt)),
+        _buf(scales, ckpt8_scales(rows, cols), torch.uint8),
+        _buf(bias, groups * cols, torch.float32), _buf(offsets, groups + 1, torch.int32),
+        _buf(grad_out, rows * cols, _row_dtype(t)), _buf(grad_in, rows * cols, _row_dtype(t)),
+        _buf(act, rows * cols, _row_dtype(t)), _buf(dbias, groups * cols, torch.float32), rows,
+        cols, groups, fmt, t, _stream(stream)))

@@ -1,0 +1,541 @@
+// Activations kept for the backward pass in 8 bits, for gfx950: rows to a
+// checkpoint and back, and bias + tanh-GELU of rows grouped by expert whose
+// backward pass reads the checkpoint of its input.  No counterpart in the
+// reference, which keeps the activation itself, in fp32 or half
+// (FINAL_CLEAN_CODE/src/kernels/activations.cu:199-217,285-323).
+//
+// Format: 32 consecutive columns of a row share a power of two (the last
+// block of a row may be shorter).  With e = max(floor(log2 max |x|), -118) the
+// scale byte is e + 127; 255 marks a block that holds a NaN or an infinity, and
+// all of it reads as NaN.  An element is
+//   int8:  q = rint(x 2^(6-e)), at most 127, of value q 2^(e-6);
+//   e4m3:  q = e4m3(x 2^(8-e)), at most 448 in magnitude, of value q 2^(e-8).
+// The scaling is exact and the rounding (to nearest even) the only one, so a
+// value has one code whatever computes it: off by at most 2^(e-7) for int8
+// (2^(e-6) where it is cut to 127, in the top 1/256 of the block's range), by
+// 2^-4 of itself for normal e4m3 codes (64 2^(e-8) where it is cut to 448).
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "mi_common.hpp"
+#include "mi_gelu.hpp"
+#include "mi_rowtype.hpp"
+
+namespace mi {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kUnit = 8;                 // consecutive columns of one lane
+constexpr int kTile = kUnit * kWave;     // columns of one wave
+constexpr int kBlock = MI_CKPT8_BLOCK;   // four lanes
+constexpr int kMaxGroups = 1024;
+constexpr int kMaxRows = 1 << 30;  // keep row and column numbers, one tile or band
+constexpr int kMaxCols = 1 << 24;  // further on, inside an int, and the grids legal
+static_assert(kBlock == 4 * kUnit, "a block's lanes are one DPP quad");
+
+// ---------------------------------------------------------------------------
+// A wave takes one tile of 512 columns and a band of consecutive rows: lane i
+// owns columns 8 i .. 8 i + 7 of the tile, so four adjacent lanes hold a block.
+// The lane's biases and column sums stay in registers over the band.
+// ---------------------------------------------------------------------------
+struct Unit {
+    int col;  // first column
+    int n;    // columns of it inside the row, 0 to 8
+};
+
+__device__ __forceinline__ Unit lane_unit(int tile, int cols) {
+    const int col = tile * kTile + (threadIdx.x & (kWave - 1)) * kUnit;
+    return {col, max(0, min(kUnit, cols - col))};
+}
+
+template <int T>
+struct RawUnit {
+    u32x4 a[kUnit / row_vec<T>()];
+};
+
+template <int T>
+__device__ __forceinline__ RawUnit<T> load_unit(const char* row, const Unit& un) {
+    RawUnit<T> r;
+    const char* p = row + static_cast<size_t>(un.col) * sizeof(row_elem<T>);
+    if (un.n == kUnit) {
+#pragma unroll
+        for (int i = 0; i < kUnit / row_vec<T>(); ++i) r.a[i] = load16b(p + 16 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kUnit / row_vec<T>(); ++i) {
+            float v[row_vec<T>()];
+#pragma unroll
+            for (int e = 0; e < row_vec<T>(); ++e) {
+                const int at = i * row_vec<T>() + e;
+                v[e] = at < un.n ? row_get<T>(p, at) : 0.0f;
+            }
+            r.a[i] = row_pack<T>(v);
+        }
+    }
+    return r;
+}
+
+template <int T>
+__device__ __forceinline__ void unpack_unit(const RawUnit<T>& r, float (&v)[kUnit]) {
+#pragma unroll
+    for (int i = 0; i < kUnit / row_vec<T>(); ++i) {
+        float part[row_vec<T>()];
+        row_unpack<T>(r.a[i], part);
+#pragma unroll
+        for (int e = 0; e < row_vec<T>(); ++e) v[i * row_vec<T>() + e] = part[e];
+    }
+}
+
+template <int T>
+__device__ __forceinline__ void store_unit(char* row, const Unit& un, const float (&v)[kUnit]) {
+    char* p = row + static_cast<size_t>(un.col) * sizeof(row_elem<T>);
+    if (un.n == kUnit) {
+#pragma unroll
+        for (int i = 0; i < kUnit / row_vec<T>(); ++i) {
+            float part[row_vec<T>()];
+#pragma unroll
+            for (int e = 0; e < row_vec<T>(); ++e) part[e] = v[i * row_vec<T>() + e];
+            store16b(p + 16 * i, row_pack<T>(part));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e)
+            if (e < un.n) row_put<T>(p, e, v[e]);
+    }
+}
+
+typedef uint32_t u32x2_at1 __attribute__((ext_vector_type(2), aligned(1)));
+
+__device__ __forceinline__ u32x2 load_codes(const uint8_t* row, const Unit& un) {
+    const uint8_t* p = row + un.col;
+    if (un.n == kUnit) return *reinterpret_cast<const u32x2_at1*>(p);
+    u32x2 r = {0, 0};
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e)
+        if (e < un.n) r[e / 4] |= static_cast<uint32_t>(p[e]) << (e % 4 * 8);
+    return r;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* row, const Unit& un, const u32x2& q) {
+    uint8_t* p = row + un.col;
+    if (un.n == kUnit) {
+        *reinterpret_cast<u32x2_at1*>(p) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e)
+            if (e < un.n) p[e] = static_cast<uint8_t>(q[e / 4] >> (e % 4 * 8));
+    }
+}
+
+// The scale byte of the block that the lane's quad holds.  Magnitudes compare
+// as integers, with NaN and infinity above every number, and the exponent
+// field of the largest is e + 127.
+__device__ __forceinline__ int block_scale(const float (&v)[kUnit]) {
+    int m = 0;
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) m = max(m, __float_as_int(v[e]) & 0x7fffffff);
+    m = max(m, dpp_move_i<0xB1>(m));
+    m = max(m, dpp_move_i<0x4E>(m));
+    return max(m >> 23, 9);
+}
+
+// The codes of a unit.  int8: adding 1.5 2^23 leaves rint(x 2^(6-e)) in the low
+// bits of the sum, two's complement; the product is exact inside the FMA.
+template <int FMT>
+__device__ __forceinline__ u32x2 encode(const float (&v)[kUnit], int scale) {
+    u32x2 q = {0, 0};
+    if (scale == 255) return q;
+    const float mul = __int_as_float(((FMT == MI_CKPT8_INT8 ? 260 : 262) - scale) << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (FMT == MI_CKPT8_INT8) {
+            uint32_t b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                b[e] = __float_as_uint(fminf(fmaf(v[4 * h + e], mul, 12582912.0f), 12583039.0f));
+            const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+            q[h] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+        } else {
+            float s[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                s[e] = __builtin_amdgcn_fmed3f(v[4 * h + e] * mul, -448.0f, 448.0f);
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], w, true);
+            q[h] = static_cast<uint32_t>(w);
+        }
+    }
+    return q;
+}
+
+template <int FMT>
+__device__ __forceinline__ void decode(const u32x2& q, int scale, float (&v)[kUnit]) {
+    const float step = scale == 255
+                           ? __int_as_float(0x7fc00000)
+                           : __builtin_ldexpf(1.0f, scale - (FMT == MI_CKPT8_INT8 ? 133 : 135));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int w = static_cast<int>(q[h]);
+        if constexpr (FMT == MI_CKPT8_INT8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[4 * h + e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e))) * step;
+        } else {
+            v[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8(w, 0) * step;
+            v[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(w, 1) * step;
+            v[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(w, 2) * step;
+            v[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3) * step;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Segments.  Group g's rows are offsets[g] .. offsets[g + 1] - 1; without
+// offsets there is one group of all rows.  Values outside [0, rows] are cut,
+// so that offsets which are not what they should be cannot lead out of the
+// tensors.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int group_end(const int* offsets, int g, int rows) {
+    return offsets == nullptr ? rows : max(0, min(offsets[g + 1], rows));
+}
+
+// The first row of any group.
+__device__ __forceinline__ int first_row(const int* offsets, int rows) {
+    return offsets == nullptr ? 0 : max(0, min(offsets[0], rows));
+}
+
+// The first group that ends behind row r; groups where there is none.
+__device__ __forceinline__ int group_of(const int* offsets, int groups, int rows, int r) {
+    int lo = 0, hi = groups;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (group_end(offsets, mid, rows) > r)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void load_bias(const float* bias, int g, int cols, const Unit& un,
+                                          float (&b)[kUnit]) {
+    const float* p = bias + static_cast<size_t>(g) * cols + un.col;
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) b[e] = e < un.n ? p[e] : 0.0f;
+}
+
+struct WaveTask {
+    int tile, band;
+};
+
+__device__ __forceinline__ WaveTask wave_task(int tiles) {
+    const unsigned w = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    return {static_cast<int>(w % tiles), static_cast<int>(w / tiles)};
+}
+
+// GELU: out = gelu(in + bias) and the checkpoint of in; else the checkpoint.
+// out may be in: a lane reads its unit of a row before it writes it.
+template <int T, int FMT, bool GELU>
+__global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
+    const char* in, const float* __restrict__ bias, const int* __restrict__ offsets, char* out,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ scales, int rows, int cols, int groups,
+    int band, int tiles, int bands) {
+    const WaveTask task = wave_task(tiles);
+    if (task.band >= bands) return;
+    const Unit un = lane_unit(task.tile, cols);
+    const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
+    const int blocks = (cols + kBlock - 1) / kBlock;
+    const int r1 = min((task.band + 1) * band, rows);
+    int r0 = task.band * band, g = 0, end = r1;
+    float b[kUnit];
+    if constexpr (GELU) {
+        r0 = max(r0, first_row(offsets, rows));
+        g = group_of(offsets, groups, rows, r0);
+        end = r0;  // the first row loads its group's bias
+    }
+    for (int r = r0; r < r1; ++r) {
+        if constexpr (GELU) {
+            if (r >= end) {
+                while (g < groups && group_end(offsets, g, rows) <= r) ++g;
+                if (g >= groups) break;
+                end = group_end(offsets, g, rows);
+                load_bias(bias, g, cols, un, b);
+            }
+        }
+        float v[kUnit];
+        unpack_unit<T>(load_unit<T>(in + r * row_bytes, un), v);
+        const int scale = block_scale(v);
+        store_codes(q + static_cast<size_t>(r) * cols, un, encode<FMT>(v, scale));
+        if (un.n > 0 && un.col % kBlock == 0)
+            scales[static_cast<size_t>(r) * blocks + un.col / kBlock] = static_cast<uint8_t>(scale);
+        if constexpr (GELU) {
+#pragma unroll
+            for (int e = 0; e < kUnit; ++e) v[e] = gelu_fwd(v[e] + b[e]);
+            store_unit<T>(out + r * row_bytes, un, v);
+        }
+    }
+}
+
+template <int T, int FMT>
+__global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
+    const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, char* __restrict__ out,
+    int rows, int cols, int band, int tiles, int bands) {
+    const WaveTask task = wave_task(tiles);
+    if (task.band >= bands) return;
+    const Unit un = lane_unit(task.tile, cols);
+    if (un.n == 0) return;
+    const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
+    const int blocks = (cols + kBlock - 1) / kBlock;
+    const int r0 = task.band * band, r1 = min(r0 + band, rows);
+    for (int r = r0; r < r1; ++r) {
+        float v[kUnit];
+        decode<FMT>(load_codes(q + static_cast<size_t>(r) * cols, un),
+                    scales[static_cast<size_t>(r) * blocks + un.col / kBlock], v);
+        store_unit<T>(out + r * row_bytes, un, v);
+    }
+}
+
+// u = value of the checkpoint + bias; grad_in = grad_out gelu'(u); act =
+// gelu(u); the column sums of grad_in over the band's rows of group g go to
+// partial row band + g.  Going down the rows, band and g only grow, and one of
+// them does with every new pair, so no two pairs share a partial row.
+// grad_in may be grad_out.
+template <int T, int FMT, bool ACT>
+__global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
+    const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales,
+    const float* __restrict__ bias, const int* __restrict__ offsets, const char* grad_out,
+    char* grad_in, char* __restrict__ act, float* __restrict__ part, int rows, int cols,
+    int groups, int band, int tiles, int bands) {
+    const WaveTask task = wave_task(tiles);
+    if (task.band >= bands) return;
+    const Unit un = lane_unit(task.tile, cols);
+    if (un.n == 0) return;
+    const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
+    const int blocks = (cols + kBlock - 1) / kBlock;
+    const int r0 = max(task.band * band, first_row(offsets, rows));
+    const int r1 = min((task.band + 1) * band, rows);
+    if (r0 >= r1) return;
+    int g = group_of(offsets, groups, rows, r0), end = r0;
+    float b[kUnit], acc[kUnit];
+    auto flush = [&]() {
+        float* p = part + static_cast<size_t>(task.band + g) * cols + un.col;
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e)
+            if (e < un.n) p[e] = acc[e];
+    };
+    for (int r = r0; r < r1; ++r) {
+        if (r >= end) {
+            if (r > r0) flush();
+            while (g < groups && group_end(offsets, g, rows) <= r) ++g;
+            if (g >= groups) return;
+            end = group_end(offsets, g, rows);
+            load_bias(bias, g, cols, un, b);
+#pragma unroll
+            for (int e = 0; e < kUnit; ++e) acc[e] = 0.0f;
+        }
+        float v[kUnit], d[kUnit];
+        unpack_unit<T>(load_unit<T>(grad_out + r * row_bytes, un), d);
+        decode<FMT>(load_codes(q + static_cast<size_t>(r) * cols, un),
+                    scales[static_cast<size_t>(r) * blocks + un.col / kBlock], v);
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e) {
+            const float u = v[e] + b[e];
+            d[e] *= gelu_grad(u);
+            acc[e] += d[e];
+            if constexpr (ACT) v[e] = gelu_fwd(u);
+        }
+        store_unit<T>(grad_in + r * row_bytes, un, d);
+        if constexpr (ACT) store_unit<T>(act + r * row_bytes, un, v);
+    }
+    if (g < groups) flush();
+}
+
+// dbias[g][c] += sum of group g's partial rows, in band order within 16 slices
+// and then over the slices.
+constexpr int kFinThreads = 512;
+constexpr int kFinCols = 32;
+constexpr int kFinSlices = kFinThreads / kFinCols;
+
+__global__ __launch_bounds__(kFinThreads) void group_sum_kernel(
+    const float* __restrict__ part, const int* __restrict__ offsets, float* __restrict__ dbias,
+    int rows, int cols, int band) {
+    __shared__ float tot[kFinSlices][kFinCols];
+    const int g = blockIdx.y;
+    const int start = g == 0 ? first_row(offsets, rows) : group_end(offsets, g - 1, rows);
+    const int end = group_end(offsets, g, rows);
+    if (start >= end) return;
+    const int c = blockIdx.x * kFinCols + threadIdx.x % kFinCols;
+    const int slice = threadIdx.x / kFinCols;
+    const int first = start / band, n = (end - 1) / band - first + 1;
+    const int p0 = static_cast<int>(static_cast<long long>(slice) * n / kFinSlices);
+    const int p1 = static_cast<int>(static_cast<long long>(slice + 1) * n / kFinSlices);
+    float s = 0.0f;
+    if (c < cols)
+        for (int p = p0; p < p1; ++p) s += part[static_cast<size_t>(first + p + g) * cols + c];
+    tot[slice][threadIdx.x % kFinCols] = s;
+    __syncthreads();
+    if (slice == 0 && c < cols) {
+        float t = tot[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < kFinSlices; ++w) t += tot[w][threadIdx.x];
+        dbias[static_cast<size_t>(g) * cols + c] += t;
+    }
+}
+
+struct Plan {
+    int band, bands, tiles;
+    unsigned grid;
+};
+
+// Rows per band: few enough that the waves fill the chip, and at most 64.
+Plan plan_ckpt8(int rows, int cols) {
+    const long long tiles = (static_cast<long long>(cols) + kTile - 1) / kTile;
+    long long band = static_cast<long long>(rows) * tiles / 8192;
+    band = std::min<long long>(std::max<long long>(band, 1), 64);
+    // the waves' number stays below 2^24
+    band = std::max(band, (static_cast<long long>(rows) * tiles >> 24) + 1);
+    const long long bands = (rows + band - 1) / band;
+    return {static_cast<int>(band), static_cast<int>(bands), static_cast<int>(tiles),
+            static_cast<unsigned>((bands * tiles + kWaves - 1) / kWaves)};
+}
+
+int check_args(const char* name, int rows, int cols, int groups, int format, int type) {
+    if (rows < 0 || rows > kMaxRows || cols < 1 || cols > kMaxCols || groups < 1 ||
+        groups > kMaxGroups)
+        return set_error(MI_ERR_INVALID_ARG,
+                         "%s: invalid shape rows=%d cols=%d groups=%d (rows is 0 to %d, cols 1 to "
+                         "%d, groups 1 to %d)",
+                         name, rows, cols, groups, kMaxRows, kMaxCols, kMaxGroups);
+    if (format != MI_CKPT8_INT8 && format != MI_CKPT8_E4M3)
+        return set_error(MI_ERR_INVALID_ARG, "%s: unknown format %d", name, format);
+    if (!row_type_ok(type))
+        return set_error(MI_ERR_INVALID_ARG, "%s: unknown type %d", name, type);
+    return MI_OK;
+}
+
+template <class F>
+void with_format(int format, F f) {
+    if (format == MI_CKPT8_INT8)
+        f(std::integral_constant<int, MI_CKPT8_INT8>());
+    else
+        f(std::integral_constant<int, MI_CKPT8_E4M3>());
+}
+
+template <bool GELU>
+int launch_to_ckpt8(const char* name, const void* in, const float* bias, const int* offsets,
+                    void* out, void* q, void* scales, int rows, int cols, int groups, int format,
+                    int type, hipStream_t st) {
+    const Plan p = plan_ckpt8(rows, cols);
+    with_row_type(type, [&](auto t) {
+        with_format(format, [&](auto f) {
+            hipLaunchKernelGGL((to_ckpt8_kernel<decltype(t)::value, decltype(f)::value, GELU>),
+                               dim3(p.grid), dim3(kThreads), 0, st, static_cast<const char*>(in),
+                               bias, offsets, static_cast<char*>(out), static_cast<uint8_t*>(q),
+                               static_cast<uint8_t*>(scales), rows, cols, groups, p.band, p.tiles,
+                               p.bands);
+        });
+    });
+    return check_launch(name);
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" {
+
+int mi_float_to_ckpt8(const void* in, void* q, void* scales, int rows, int cols, int format,
+                      int type, void* stream) {
+    const char* name = "mi_float_to_ckpt8";
+    if (int rc = check_args(name, rows, cols, 1, format, type)) return rc;
+    if (rows == 0) return MI_OK;
+    if (!in || !q || !scales) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    return launch_to_ckpt8<false>(name, in, nullptr, nullptr, nullptr, q, scales, rows, cols, 1,
+                                  format, type, to_stream(stream));
+}
+
+int mi_ckpt8_to_float(const void* q, const void* scales, void* out, int rows, int cols, int format,
+                      int type, void* stream) {
+    const char* name = "mi_ckpt8_to_float";
+    if (int rc = check_args(name, rows, cols, 1, format, type)) return rc;
+    if (rows == 0) return MI_OK;
+    if (!q || !scales || !out) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    const Plan p = plan_ckpt8(rows, cols);
+    with_row_type(type, [&](auto t) {
+        with_format(format, [&](auto f) {
+            hipLaunchKernelGGL((from_ckpt8_kernel<decltype(t)::value, decltype(f)::value>),
+                               dim3(p.grid), dim3(kThreads), 0, to_stream(stream),
+                               static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales),
+                               static_cast<char*>(out), rows, cols, p.band, p.tiles, p.bands);
+        });
+    });
+    return check_launch(name);
+}
+
+int mi_bias_gelu_forward_ckpt8(const void* in, const float* bias, const int* offsets, void* out,
+                               void* q, void* scales, int rows, int cols, int groups, int format,
+                               int type, void* stream) {
+    const char* name = "mi_bias_gelu_forward_ckpt8";
+    if (int rc = check_args(name, rows, cols, groups, format, type)) return rc;
+    if (rows == 0) return MI_OK;
+    if (!in || !bias || !out || !q || !scales)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    if (groups > 1 && !offsets)
+        return set_error(MI_ERR_INVALID_ARG, "%s: %d groups need offsets", name, groups);
+    return launch_to_ckpt8<true>(name, in, bias, offsets, out, q, scales, rows, cols, groups,
+                                 format, type, to_stream(stream));
+}
+
+size_t mi_gelu_backward_ckpt8_workspace(int rows, int cols, int groups) {
+    if (rows <= 0 || cols <= 0 || groups <= 0) return 0;
+    return colsum_bytes(plan_ckpt8(rows, cols).bands + groups - 1, cols);
+}
+
+int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales, const float* bias,
+                                              const int* offsets, const void* grad_out,
+                                              void* grad_in, void* act, float* dbias, int rows,
+                                              int cols, int groups, int format, int type,
+                                              void* stream) {
+    const char* name = "mi_gelu_backward_with_bias_backward_ckpt8";
+    if (int rc = check_args(name, rows, cols, groups, format, type)) return rc;
+    if (rows == 0) return MI_OK;
+    if (!q || !scales || !bias || !grad_out || !grad_in || !dbias)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    if (groups > 1 && !offsets)
+        return set_error(MI_ERR_INVALID_ARG, "%s: %d groups need offsets", name, groups);
+    hipStream_t st = to_stream(stream);
+    const Plan p = plan_ckpt8(rows, cols);
+    int err = MI_OK;
+    char* ws = static_cast<char*>(
+        workspace_get(mi_gelu_backward_ckpt8_workspace(rows, cols, groups), st, &err));
+    if (!ws) return err;
+    float* part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    with_row_type(type, [&](auto t) {
+        with_format(format, [&](auto f) {
+            constexpr int T = decltype(t)::value, F = decltype(f)::value;
+            auto launch = [&](auto a) {
+                hipLaunchKernelGGL((gelu_bwd_ckpt8_kernel<T, F, decltype(a)::value>), dim3(p.grid),
+                                   dim3(kThreads), 0, st, static_cast<const uint8_t*>(q),
+                                   static_cast<const uint8_t*>(scales), bias, offsets,
+                                   static_cast<const char*>(grad_out), static_cast<char*>(grad_in),
+                                   static_cast<char*>(act), part, rows, cols, groups, p.band,
+                                   p.tiles, p.bands);
+            };
+            if (act != nullptr)
+                launch(std::true_type());
+            else
+                launch(std::false_type());
+        });
+    });
+    if (int rc = check_launch(name)) return rc;
+    hipLaunchKernelGGL(group_sum_kernel, dim3((cols + kFinCols - 1) / kFinCols, groups),
+                       dim3(kFinThreads), 0, st, part, offsets, dbias, rows, cols, p.band);
+    return check_launch(name);
+}
+
+}  // extern "C"

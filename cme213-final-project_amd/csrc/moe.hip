@@ -1,0 +1,788 @@
+// What a mixture-of-experts feed-forward layer does around its matrix
+// products, for gfx950: the router's choice of experts and its gradient, the
+// slots sorted by expert, token rows copied to their experts' rows and back.
+// No counterpart in the reference, whose feed-forward layer is dense; the rows
+// move as in its embedding gather and scatter-add
+// (FINAL_CLEAN_CODE/src/kernels/embedding.cu:4-79), without atomics.
+//
+// Notation: N tokens, k choices each; slot t * k + j is choice j of token t.
+// The sorted buffer has `rows` rows; position[slot] is the slot's row, and any
+// value outside [0, rows) means the slot was dropped.
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "mi_common.hpp"
+#include "mi_rowtype.hpp"
+
+namespace mi {
+
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChoices = 16;
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kMaxGrid = 1 << 20;  // workgroups over the tokens, which are taken in strides
+constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's second dimension
+
+// ---------------------------------------------------------------------------
+// Router.  A row's E logits lie in the registers of L lanes, P consecutive
+// ones in each.  A logit becomes an integer key of the same order: the bits,
+// the lower 31 inverted for negative numbers, -0 made +0; NaN ranks above all
+// and -inf is the lowest key, which is never chosen.  Each of the k rounds
+// finds the largest key left (registers, then DPP over the lanes), the first
+// lane that holds it and its first element there: the lowest expert of that
+// logit.  The lane group's lane j keeps the key of round j.
+// ---------------------------------------------------------------------------
+constexpr int kNoKey = INT_MIN;
+
+__device__ __forceinline__ int order_key(float f) {
+    if (f != f) return INT_MAX;
+    if (f == -__builtin_inff()) return kNoKey;
+    const int b = __float_as_int(f + 0.0f);
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+
+// The logit of a key (NaN for NaN's key); undefined for kNoKey.
+__device__ __forceinline__ float key_value(int key) {
+    return __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
+}
+
+template <int T, int L, int P>
+__device__ __forceinline__ void load_logits(const void* logits, size_t row, int gl, int experts,
+                                            float (&v)[P]) {
+    const size_t base = row * experts;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int e = gl * P + p;
+        v[p] = e < experts ? row_get<T>(logits, base + e) : -__builtin_inff();
+    }
+}
+
+template <int T, int L, int P, bool RENORM>
+__global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restrict__ logits,
+                                                            int* __restrict__ ids,
+                                                            float* __restrict__ weights,
+                                                            int tokens, int experts, int k) {
+    constexpr int PER = kThreads / L;  // rows per workgroup
+    const int lane = threadIdx.x & (kWave - 1);
+    const int gl = lane & (L - 1);
+    for (long long first = static_cast<long long>(blockIdx.x) * PER; first < tokens;
+         first += static_cast<long long>(gridDim.x) * PER) {
+        const long long want = first + threadIdx.x / L;
+        const bool valid = want < tokens;  // the others repeat the last row and store nothing
+        const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
+        float v[P];
+        load_logits<T, L, P>(logits, row, gl, experts, v);
+        int key[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) key[p] = order_key(v[p]);
+
+        const size_t out = row * k;
+        float top = 0.0f, total = 0.0f;
+        int mine = kNoKey;
+        for (int j = 0; j < k; ++j) {
+            int local = key[0];
+#pragma unroll
+            for (int p = 1; p < P; ++p) local = max(local, key[p]);
+            const int m = group_max<L>(local);
+            if (j == 0) {
+                top = key_value(m);
+                if constexpr (!RENORM) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+                        s += key[p] == kNoKey ? 0.0f : expf(key_value(key[p]) - top);
+                    total = group_sum<L>(s);
+                }
+            }
+            const unsigned long long holds = __ballot(local == m) >> (lane & ~(L - 1));
+            const bool winner = __ffsll(holds) - 1 == gl;
+            int at = 0;
+#pragma unroll
+            for (int p = P - 1; p >= 0; --p) at = key[p] == m ? p : at;
+            if (winner && valid) ids[out + j] = m == kNoKey ? -1 : gl * P + at;
+#pragma unroll
+            for (int p = 0; p < P; ++p) key[p] = winner && p == at ? kNoKey : key[p];
+            mine = gl == j ? m : mine;
+        }
+        const float e = mine == kNoKey ? 0.0f : expf(key_value(mine) - top);
+        if constexpr (RENORM) total = group_sum<L>(e);
+        if (valid && gl < k) weights[out + gl] = mine == kNoKey ? 0.0f : e / total;
+    }
+}
+
+// dl_e = sum over the slots j with id_j = e of w_j (dw_j [- d]) - p_e d, with
+// d = sum_j w_j dw_j; the term in p_e only where the weights are not
+// renormalised, [- d] only where they are.
+template <int T, int L, int P, bool RENORM>
+__global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
+    const void* __restrict__ logits, const int* __restrict__ ids,
+    const float* __restrict__ weights, const float* __restrict__ dweights,
+    void* __restrict__ dlogits, int tokens, int experts, int k) {
+    constexpr int PER = kThreads / L;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int gl = lane & (L - 1);
+    for (long long first = static_cast<long long>(blockIdx.x) * PER; first < tokens;
+         first += static_cast<long long>(gridDim.x) * PER) {
+        const long long want = first + threadIdx.x / L;
+        const bool valid = want < tokens;
+        const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
+
+        int id = -1;
+        float w = 0.0f, dw = 0.0f;
+        if (gl < k) {
+            id = ids[row * k + gl];
+            w = weights[row * k + gl];
+            dw = dweights[row * k + gl];
+        }
+        const float wd = id >= 0 ? w * dw : 0.0f;
+        const float d = group_sum<L>(wd);
+        const float term = RENORM ? (id >= 0 ? w * (dw - d) : 0.0f) : wd;
+
+        float v[P];
+        if constexpr (RENORM) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) v[p] = 0.0f;
+        } else {
+            load_logits<T, L, P>(logits, row, gl, experts, v);
+            float top = v[0];
+#pragma unroll
+            for (int p = 1; p < P; ++p) top = fmaxf(top, v[p]);
+            top = group_max<L>(top);
+            if (top == -__builtin_inff()) top = 0.0f;  // every e below is 0, or NaN
+            float s = 0.0f;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                v[p] = v[p] == -__builtin_inff() ? 0.0f : expf(v[p] - top);
+                s += v[p];
+            }
+            s = group_sum<L>(s);
+            const float scale = -d / (s == 0.0f ? 1.0f : s);
+#pragma unroll
+            for (int p = 0; p < P; ++p) v[p] *= scale;
+        }
+        for (int j = 0; j < k; ++j) {
+            const int idj = __shfl(id, j, L);
+            const float tj = __shfl(term, j, L);
+#pragma unroll
+            for (int p = 0; p < P; ++p) v[p] += idj == gl * P + p ? tj : 0.0f;
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            if (gl * P + p < experts) row_put<T>(dlogits, row * experts + gl * P + p, v[p]);
+    }
+}
+
+// f(L, P): 16 lanes a row up to 256 experts, 64 lanes above.
+template <class F>
+void with_gate_shape(int experts, F f) {
+    using std::integral_constant;
+    if (experts <= 16)
+        f(integral_constant<int, 16>(), integral_constant<int, 1>());
+    else if (experts <= 32)
+        f(integral_constant<int, 16>(), integral_constant<int, 2>());
+    else if (experts <= 64)
+        f(integral_constant<int, 16>(), integral_constant<int, 4>());
+    else if (experts <= 128)
+        f(integral_constant<int, 16>(), integral_constant<int, 8>());
+    else if (experts <= 256)
+        f(integral_constant<int, 16>(), integral_constant<int, 16>());
+    else if (experts <= 512)
+        f(integral_constant<int, 64>(), integral_constant<int, 8>());
+    else
+        f(integral_constant<int, 64>(), integral_constant<int, 16>());
+}
+
+unsigned gate_grid(int tokens, int lanes) {
+    const int per = kThreads / lanes;
+    return static_cast<unsigned>(
+        std::min<long long>((static_cast<long long>(tokens) + per - 1) / per, kMaxGrid));
+}
+
+// ---------------------------------------------------------------------------
+// Stable sort of the slots by expert (a counting sort).  A workgroup takes a
+// chunk of consecutive slots, each of its 16 waves a consecutive part of it.
+// A wave takes 64 slots at a time: the lanes with the same expert are found by
+// one ballot per bit of the id, a slot's rank among them is the number of such
+// lanes before it, and the first of them advances the wave's count of that
+// expert.  Counts are whole numbers, so the result does not depend on timing.
+// ---------------------------------------------------------------------------
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / kWave;
+constexpr int kSortChunk = 4096;     // slots per workgroup, at least
+constexpr int kSortMaxChunks = 256;
+
+struct SortPlan {
+    int chunk;   // slots per workgroup, a multiple of kSortThreads
+    int chunks;
+};
+
+SortPlan plan_sort(int slots) {
+    long long chunk = (static_cast<long long>(slots) + kSortMaxChunks - 1) / kSortMaxChunks;
+    chunk = (chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
+    if (chunk < kSortChunk) chunk = kSortChunk;
+    return {static_cast<int>(chunk),
+            static_cast<int>((static_cast<long long>(slots) + chunk - 1) / chunk)};
+}
+
+// hist[c][e]: slots of expert e in chunk c.
+__global__ __launch_bounds__(kSortThreads) void sort_hist_kernel(const int* __restrict__ ids,
+                                                                 int* __restrict__ hist,
+                                                                 int slots, int experts,
+                                                                 int chunk) {
+    extern __shared__ int count[];
+    for (int e = threadIdx.x; e < experts; e += kSortThreads) count[e] = 0;
+    __syncthreads();
+    const long long begin = static_cast<long long>(blockIdx.x) * chunk;
+    for (int i = threadIdx.x; i < chunk; i += kSortThreads) {
+        const long long s = begin + i;
+        if (s < slots) {
+            const int id = ids[s];
+            if (id >= 0 && id < experts) atomicAdd(&count[id], 1);
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kSortThreads)
+        hist[static_cast<size_t>(blockIdx.x) * experts + e] = count[e];
+}
+
+// The lanes whose id equals this lane's, among the lanes with an id.
+__device__ __forceinline__ unsigned long long same_id(int id, bool has, int bits) {
+    unsigned long long m = __ballot(has);
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (id >> b) & 1;
+        const unsigned long long ones = __ballot(one);
+        m &= one ? ones : ~ones;
+    }
+    return m;
+}
+
+// hist == nullptr: there is one chunk.
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(
+    const int* __restrict__ ids, const int* __restrict__ hist, int* __restrict__ offsets,
+    int* __restrict__ order, int* __restrict__ position, int slots, int experts, int chunk,
+    int chunks, int bits) {
+    extern __shared__ int lds[];
+    int* count = lds;                          // [kSortWaves][experts]
+    __shared__ int wave_total[kSortWaves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+    for (int i = threadIdx.x; i < kSortWaves * experts; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+
+    const int part = chunk / kSortWaves;  // a multiple of 64
+    const long long begin = static_cast<long long>(blockIdx.x) * chunk +
+                            static_cast<long long>(wave) * part;
+    int* mine = count + wave * experts;
+    for (int i = 0; i < part; i += kWave) {
+        const long long s = begin + i + lane;
+        const int id = s < slots ? ids[s] : -1;
+        if (id >= 0 && id < experts) atomicAdd(&mine[id], 1);
+    }
+    __syncthreads();
+
+    // Thread e owns expert e (experts <= kSortThreads): its slots in this
+    // chunk by wave, in the chunks before and in all of them.
+    const int e = threadIdx.x;
+    int total = 0, before = 0;
+    if (e < experts) {
+        if (hist == nullptr) {
+            for (int w = 0; w < kSortWaves; ++w) total += count[w * experts + e];
+        } else {
+            for (int c = 0; c < chunks; ++c) {
+                const int h = hist[static_cast<size_t>(c) * experts + e];
+                before += c < static_cast<int>(blockIdx.x) ? h : 0;
+                total += h;
+            }
+        }
+    }
+    // exclusive sum of the totals over the experts
+    int incl = total;
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int up = __shfl_up(incl, d);
+        if (lane >= d) incl += up;
+    }
+    if (lane == kWave - 1) wave_total[wave] = incl;
+    __syncthreads();
+    int first = incl - total;
+    for (int w = 0; w < wave; ++w) first += wave_total[w];
+    if (e < experts) {
+        if (blockIdx.x == 0) {
+            offsets[e] = first;
+            if (e == experts - 1) offsets[experts] = first + total;
+        }
+        int at = first + before;
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int n = count[w * experts + e];
+            count[w * experts + e] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+
+    for (int i = 0; i < part; i += kWave) {
+        const long long s = begin + i + lane;
+        const int id = s < slots ? ids[s] : -1;
+        const bool has = id >= 0 && id < experts;
+        const unsigned long long same = same_id(id, has, bits);
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const int at = has ? mine[id] : 0;
+        wave_order();
+        if (has && rank == 0) mine[id] = at + __popcll(same);
+        wave_order();
+        if (s < slots) position[s] = has ? at + rank : -1;
+        if (has && order != nullptr) order[at + rank] = static_cast<int>(s);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows moved between token order and expert order.  A wave takes one token
+// and a segment of U * 64 16-byte chunks of its row, so the token's positions
+// are wave-uniform.  Where the row is no multiple of 16 bytes the last chunk
+// is moved back to end with the row: the elements that it shares with the one
+// before are computed twice, with the same result.
+// ---------------------------------------------------------------------------
+struct Chunk {
+    bool on;
+    size_t at;  // byte offset in the row
+};
+
+__device__ __forceinline__ Chunk row_chunk(int c, int chunks, size_t row_bytes) {
+    const size_t at = static_cast<size_t>(c) * 16;
+    return {c < chunks, at < row_bytes - 16 ? at : row_bytes - 16};
+}
+
+template <int U>
+__global__ __launch_bounds__(kThreads) void scatter_rows_kernel(
+    const char* __restrict__ x, const int* __restrict__ position, char* __restrict__ out,
+    int tokens, int k, int rows, int chunks, size_t row_bytes) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
+                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    for (long long token = wave; token < tokens;
+         token += static_cast<long long>(gridDim.x) * kWaves) {
+        const char* src = x + static_cast<size_t>(token) * row_bytes;
+        u32x4 v[U];
+        Chunk ch[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * kWave + u * kWave + lane, chunks,
+                              row_bytes);
+            if (ch[u].on) v[u] = load16b(src + ch[u].at);
+        }
+        const int* pos = position + static_cast<size_t>(token) * k;
+        for (int j = 0; j < k; ++j) {
+            const int p = pos[j];
+            if (p < 0 || p >= rows) continue;
+            char* dst = out + static_cast<size_t>(p) * row_bytes;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (ch[u].on) store16b(dst + ch[u].at, v[u]);
+        }
+    }
+}
+
+// out[t] = sum over j, in order, of [w[t, j]] rows[position[t, j]].
+template <int T, int U, bool WEIGHTED>
+__global__ __launch_bounds__(kThreads) void gather_sum_kernel(
+    const char* __restrict__ src, const int* __restrict__ position,
+    const float* __restrict__ weights, char* __restrict__ out, int tokens, int k, int rows,
+    int chunks, size_t row_bytes) {
+    constexpr int V = row_vec<T>();
+    const int lane = threadIdx.x & (kWave - 1);
+    const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
+                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    for (long long token = wave; token < tokens;
+         token += static_cast<long long>(gridDim.x) * kWaves) {
+        Chunk ch[U];
+        float acc[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * kWave + u * kWave + lane, chunks,
+                              row_bytes);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[u][e] = 0.0f;
+        }
+        const size_t slot = static_cast<size_t>(token) * k;
+        for (int j = 0; j < k; ++j) {
+            const int p = position[slot + j];
+            if (p < 0 || p >= rows) continue;
+            const float w = WEIGHTED ? weights[slot + j] : 1.0f;
+            const char* r = src + static_cast<size_t>(p) * row_bytes;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (ch[u].on) {
+                    float y[V];
+                    row_unpack<T>(load16b(r + ch[u].at), y);
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        acc[u][e] = WEIGHTED ? fmaf(w, y[e], acc[u][e]) : acc[u][e] + y[e];
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ch[u].on)
+                store16b(out + static_cast<size_t>(token) * row_bytes + ch[u].at,
+                         row_pack<T>(acc[u]));
+    }
+}
+
+// dy[position[t, j]] = w[t, j] dout[t]; dw[t, j] = dout[t] . y[position[t, j]].
+// One wave per token; KB is k rounded up, so that the k sums stay in registers.
+// A lane writes a chunk of dy after it has read the same chunk of y, and what
+// the moved-back last chunk shares with its neighbour is left out of the sums,
+// so dy may be y.
+template <int T, int KB>
+__global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
+    const char* __restrict__ dout, const char* y, const int* __restrict__ position,
+    const float* __restrict__ weights, char* dy, float* __restrict__ dweights, int tokens, int k,
+    int rows, int chunks, size_t row_bytes) {
+    constexpr int V = row_vec<T>();
+    constexpr int S = 16 / V;
+    const int lane = threadIdx.x & (kWave - 1);
+    const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
+                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    for (long long token = wave; token < tokens;
+         token += static_cast<long long>(gridDim.x) * kWaves) {
+        const size_t slot = static_cast<size_t>(token) * k;
+        const char* g_row = dout + static_cast<size_t>(token) * row_bytes;
+        int pos[KB];
+        float w[KB], dot[KB];
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+            pos[j] = j < k ? position[slot + j] : -1;
+            w[j] = j < k ? weights[slot + j] : 0.0f;
+            dot[j] = 0.0f;
+        }
+        for (int c = lane; c < chunks; c += kWave) {
+            const size_t at = row_chunk(c, chunks, row_bytes).at;
+            const int twice = static_cast<int>((static_cast<size_t>(c) * 16 - at) / S);
+            float g[V];
+            row_unpack<T>(load16b(g_row + at), g);
+#pragma unroll
+            for (int j = 0; j < KB; ++j) {
+                if (pos[j] < 0 || pos[j] >= rows) continue;
+                const size_t r = static_cast<size_t>(pos[j]) * row_bytes + at;
+                float v[V];
+                row_unpack<T>(load16b(y + r), v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float term = g[e] * v[e];
+                    dot[j] += e < twice ? 0.0f : term;
+                    v[e] = w[j] * g[e];
+                }
+                store16b(dy + r, row_pack<T>(v));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+            const float s = wave_sum(dot[j]);
+            if (lane == 0 && j < k) dweights[slot + j] = s;
+        }
+    }
+}
+
+// Rows of less than 16 bytes: one thread per token.
+enum class Narrow { Scatter, Sum, WeightedSum, Backward };
+
+template <int T, Narrow OP>
+__global__ __launch_bounds__(kThreads) void narrow_kernel(
+    const void* a, const void* y, const int* __restrict__ position,
+    const float* __restrict__ weights, void* out, float* __restrict__ dweights, int tokens, int k,
+    int rows, int cols) {
+    const long long t = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
+    if (t >= tokens) return;
+    const size_t slot = static_cast<size_t>(t) * k, row = static_cast<size_t>(t) * cols;
+    if constexpr (OP == Narrow::Sum || OP == Narrow::WeightedSum) {
+        for (int c = 0; c < cols; ++c) {
+            float s = 0.0f;
+            for (int j = 0; j < k; ++j) {
+                const int p = position[slot + j];
+                if (p < 0 || p >= rows) continue;
+                const float v = row_get<T>(a, static_cast<size_t>(p) * cols + c);
+                s = OP == Narrow::Sum ? s + v : fmaf(weights[slot + j], v, s);
+            }
+            row_put<T>(out, row + c, s);
+        }
+    } else {
+        for (int j = 0; j < k; ++j) {
+            const int p = position[slot + j];
+            const bool there = p >= 0 && p < rows;
+            float dot = 0.0f;
+            if (there)
+                for (int c = 0; c < cols; ++c) {
+                    const size_t r = static_cast<size_t>(p) * cols + c;
+                    const float v = row_get<T>(a, row + c);
+                    if constexpr (OP == Narrow::Backward) {
+                        dot += v * row_get<T>(y, r);
+                        row_put<T>(out, r, weights[slot + j] * v);
+                    } else {
+                        row_put<T>(out, r, v);
+                    }
+                }
+            if constexpr (OP == Narrow::Backward) dweights[slot + j] = dot;
+        }
+    }
+}
+
+template <Narrow OP>
+int launch_narrow(const char* name, const void* a, const void* y, const int* position,
+                  const float* weights, void* out, float* dweights, int tokens, int k, int rows,
+                  int cols, int type, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>((static_cast<long long>(tokens) + kThreads - 1) / kThreads));
+    with_row_type(type, [&](auto t) {
+        hipLaunchKernelGGL((narrow_kernel<decltype(t)::value, OP>), grid, dim3(kThreads), 0, st, a,
+                           y, position, weights, out, dweights, tokens, k, rows, cols);
+    });
+    return check_launch(name);
+}
+
+unsigned token_grid(int tokens) {
+    return static_cast<unsigned>(
+        std::min<long long>((static_cast<long long>(tokens) + kWaves - 1) / kWaves, kMaxGrid));
+}
+
+// Chunks per lane: as many as keep a few thousand waves in flight.
+int segment_chunks(int tokens, int chunks) {
+    const long long one = static_cast<long long>(tokens) * ((chunks + kWave - 1) / kWave);
+    if (one >= 8192 && chunks > 2 * kWave) return 4;
+    if (one >= 4096 && chunks > kWave) return 2;
+    return 1;
+}
+
+template <class F>
+void with_segment(int u, F f) {
+    if (u == 4)
+        f(std::integral_constant<int, 4>());
+    else if (u == 2)
+        f(std::integral_constant<int, 2>());
+    else
+        f(std::integral_constant<int, 1>());
+}
+
+int check_rows_args(const char* name, int tokens, int k, int rows, int cols, int type) {
+    if (tokens < 0 || k < 1 || k > kMaxChoices || rows < 0 || cols < 1 || cols > kMaxCols)
+        return set_error(MI_ERR_INVALID_ARG,
+                         "%s: invalid shape tokens=%d k=%d rows=%d cols=%d (k is 1 to %d, cols 1 "
+                         "to %d)",
+                         name, tokens, k, rows, cols, kMaxChoices, kMaxCols);
+    if (static_cast<long long>(tokens) * k > INT_MAX)
+        return set_error(MI_ERR_INVALID_ARG, "%s: tokens * k = %lld slots exceed an int", name,
+                         static_cast<long long>(tokens) * k);
+    if (!row_type_ok(type))
+        return set_error(MI_ERR_INVALID_ARG, "%s: unknown type %d", name, type);
+    return MI_OK;
+}
+
+template <bool WEIGHTED>
+int gather_sum(const char* name, const void* src, const int* position, const float* weights,
+               void* out, int tokens, int k, int rows, int cols, int type, hipStream_t st) {
+    const size_t row_bytes = static_cast<size_t>(cols) * row_type_size(type);
+    if (row_bytes < 16)
+        return launch_narrow<WEIGHTED ? Narrow::WeightedSum : Narrow::Sum>(
+            name, src, nullptr, position, weights, out, nullptr, tokens, k, rows, cols, type, st);
+    const int chunks = static_cast<int>((row_bytes + 15) / 16);
+    const int u = segment_chunks(tokens, chunks);
+    const dim3 grid(token_grid(tokens), (chunks + u * kWave - 1) / (u * kWave));
+    with_row_type(type, [&](auto t) {
+        with_segment(u, [&](auto uu) {
+            hipLaunchKernelGGL((gather_sum_kernel<decltype(t)::value, decltype(uu)::value, WEIGHTED>),
+                               grid, dim3(kThreads), 0, st, static_cast<const char*>(src), position,
+                               weights, static_cast<char*>(out), tokens, k, rows, chunks, row_bytes);
+        });
+    });
+    return check_launch(name);
+}
+
+int check_gate_args(const char* name, int tokens, int experts, int k, int type) {
+    if (tokens < 0 || experts < 1 || experts > kMaxExperts || k < 1 || k > kMaxChoices ||
+        k > experts)
+        return set_error(MI_ERR_INVALID_ARG,
+                         "%s: invalid shape tokens=%d experts=%d k=%d (experts is 1 to %d, k 1 to "
+                         "%d and at most experts)",
+                         name, tokens, experts, k, kMaxExperts, kMaxChoices);
+    if (static_cast<long long>(tokens) * k > INT_MAX)
+        return set_error(MI_ERR_INVALID_ARG, "%s: tokens * k = %lld slots exceed an int", name,
+                         static_cast<long long>(tokens) * k);
+    if (!row_type_ok(type))
+        return set_error(MI_ERR_INVALID_ARG, "%s: unknown type %d", name, type);
+    return MI_OK;
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" {
+
+int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens, int experts,
+                        int k, int renormalise, int type, void* stream) {
+    const char* name = "mi_moe_gate_forward";
+    if (int rc = check_gate_args(name, tokens, experts, k, type)) return rc;
+    if (tokens == 0) return MI_OK;
+    if (!logits || !ids || !weights)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    with_row_type(type, [&](auto t) {
+        with_gate_shape(experts, [&](auto l, auto p) {
+            constexpr int T = decltype(t)::value, L = decltype(l)::value, P = decltype(p)::value;
+            if (renormalise)
+                hipLaunchKernelGGL((gate_fwd_kernel<T, L, P, true>), dim3(gate_grid(tokens, L)),
+                                   dim3(kThreads), 0, to_stream(stream), logits, ids, weights,
+                                   tokens, experts, k);
+            else
+                hipLaunchKernelGGL((gate_fwd_kernel<T, L, P, false>), dim3(gate_grid(tokens, L)),
+                                   dim3(kThreads), 0, to_stream(stream), logits, ids, weights,
+                                   tokens, experts, k);
+        });
+    });
+    return check_launch(name);
+}
+
+int mi_moe_gate_backward(const void* logits, const int* ids, const float* weights,
+                         const float* dweights, void* dlogits, int tokens, int experts, int k,
+                         int renormalise, int type, void* stream) {
+    const char* name = "mi_moe_gate_backward";
+    if (int rc = check_gate_args(name, tokens, experts, k, type)) return rc;
+    if (tokens == 0) return MI_OK;
+    if ((!logits && !renormalise) || !ids || !weights || !dweights || !dlogits)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    with_row_type(type, [&](auto t) {
+        with_gate_shape(experts, [&](auto l, auto p) {
+            constexpr int T = decltype(t)::value, L = decltype(l)::value, P = decltype(p)::value;
+            if (renormalise)
+                hipLaunchKernelGGL((gate_bwd_kernel<T, L, P, true>), dim3(gate_grid(tokens, L)),
+                                   dim3(kThreads), 0, to_stream(stream), logits, ids, weights,
+                                   dweights, dlogits, tokens, experts, k);
+            else
+                hipLaunchKernelGGL((gate_bwd_kernel<T, L, P, false>), dim3(gate_grid(tokens, L)),
+                                   dim3(kThreads), 0, to_stream(stream), logits, ids, weights,
+                                   dweights, dlogits, tokens, experts, k);
+        });
+    });
+    return check_launch(name);
+}
+
+size_t mi_moe_sort_workspace(int slots, int experts) {
+    if (slots <= 0 || experts <= 0) return 0;
+    const SortPlan p = plan_sort(slots);
+    return p.chunks > 1
+               ? colsum_part_offset() + static_cast<size_t>(p.chunks) * experts * sizeof(int)
+               : 0;
+}
+
+int mi_moe_sort(const int* ids, int* offsets, int* order, int* position, int slots, int experts,
+                void* stream) {
+    const char* name = "mi_moe_sort";
+    if (slots < 0 || experts < 1 || experts > kMaxExperts)
+        return set_error(MI_ERR_INVALID_ARG,
+                         "%s: invalid shape slots=%d experts=%d (experts is 1 to %d)", name, slots,
+                         experts, kMaxExperts);
+    if (!offsets || (slots > 0 && (!ids || !position)))
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    hipStream_t st = to_stream(stream);
+    SortPlan p = plan_sort(slots);
+    if (p.chunks < 1) p.chunks = 1;  // no slots: the offsets are written all the same
+    int* hist = nullptr;
+    if (p.chunks > 1) {
+        int err = MI_OK;
+        char* ws = static_cast<char*>(workspace_get(mi_moe_sort_workspace(slots, experts), st, &err));
+        if (!ws) return err;
+        hist = reinterpret_cast<int*>(ws + colsum_part_offset());
+        hipLaunchKernelGGL(sort_hist_kernel, dim3(p.chunks), dim3(kSortThreads),
+                           experts * sizeof(int), st, ids, hist, slots, experts, p.chunk);
+        if (int rc = check_launch(name)) return rc;
+    }
+    int bits = 0;
+    while ((1 << bits) < experts) ++bits;
+    hipLaunchKernelGGL(sort_place_kernel, dim3(p.chunks), dim3(kSortThreads),
+                       kSortWaves * experts * sizeof(int), st, ids, hist, offsets, order, position,
+                       slots, experts, p.chunk, p.chunks, bits);
+    return check_launch(name);
+}
+
+int mi_moe_dispatch_forward(const void* x, const int* position, void* out, int tokens, int k,
+                            int rows, int cols, int type, void* stream) {
+    const char* name = "mi_moe_dispatch_forward";
+    if (int rc = check_rows_args(name, tokens, k, rows, cols, type)) return rc;
+    if (tokens == 0 || rows == 0) return MI_OK;
+    if (!x || !position || !out) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    hipStream_t st = to_stream(stream);
+    const size_t row_bytes = static_cast<size_t>(cols) * row_type_size(type);
+    if (row_bytes < 16)
+        return launch_narrow<Narrow::Scatter>(name, x, nullptr, position, nullptr, out, nullptr,
+                                              tokens, k, rows, cols, type, st);
+    const int chunks = static_cast<int>((row_bytes + 15) / 16);
+    const int u = segment_chunks(tokens, chunks);
+    const dim3 grid(token_grid(tokens), (chunks + u * kWave - 1) / (u * kWave));
+    with_segment(u, [&](auto uu) {
+        hipLaunchKernelGGL((scatter_rows_kernel<decltype(uu)::value>), grid, dim3(kThreads), 0, st,
+                           static_cast<const char*>(x), position, static_cast<char*>(out), tokens,
+                           k, rows, chunks, row_bytes);
+    });
+    return check_launch(name);
+}
+
+int mi_moe_dispatch_backward(const void* dout, const int* position, void* dx, int tokens, int k,
+                             int rows, int cols, int type, void* stream) {
+    const char* name = "mi_moe_dispatch_backward";
+    if (int rc = check_rows_args(name, tokens, k, rows, cols, type)) return rc;
+    if (tokens == 0) return MI_OK;
+    if ((!dout && rows > 0) || !position || !dx)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    return gather_sum<false>(name, dout, position, nullptr, dx, tokens, k, rows, cols, type,
+                             to_stream(stream));
+}
+
+int mi_moe_combine_forward(const void* y, const int* position, const float* weights, void* out,
+                           int tokens, int k, int rows, int cols, int type, void* stream) {
+    const char* name = "mi_moe_combine_forward";
+    if (int rc = check_rows_args(name, tokens, k, rows, cols, type)) return rc;
+    if (tokens == 0) return MI_OK;
+    if ((!y && rows > 0) || !position || !weights || !out)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    return gather_sum<true>(name, y, position, weights, out, tokens, k, rows, cols, type,
+                            to_stream(stream));
+}
+
+int mi_moe_combine_backward(const void* dout, const void* y, const int* position,
+                            const float* weights, void* dy, float* dweights, int tokens, int k,
+                            int rows, int cols, int type, void* stream) {
+    const char* name = "mi_moe_combine_backward";
+    if (int rc = check_rows_args(name, tokens, k, rows, cols, type)) return rc;
+    if (tokens == 0) return MI_OK;
+    if (!dout || (rows > 0 && (!y || !dy)) || !position || !weights || !dweights)
+        return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    hipStream_t st = to_stream(stream);
+    const size_t row_bytes = static_cast<size_t>(cols) * row_type_size(type);
+    if (row_bytes < 16)
+        return launch_narrow<Narrow::Backward>(name, dout, y, position, weights, dy, dweights,
+                                               tokens, k, rows, cols, type, st);
+    const int chunks = static_cast<int>((row_bytes + 15) / 16);
+    with_row_type(type, [&](auto t) {
+        constexpr int T = decltype(t)::value;
+        auto launch = [&](auto kb) {
+            hipLaunchKernelGGL((combine_bwd_kernel<T, decltype(kb)::value>),
+                               dim3(token_grid(tokens)), dim3(kThreads), 0, st,
+                               static_cast<const char*>(dout), static_cast<const char*>(y),
+                               position, weights, static_cast<char*>(dy), dweights, tokens, k,
+                               rows, chunks, row_bytes);
+        };
+        if (k <= 1)
+            launch(std::integral_constant<int, 1>());
+        else if (k <= 2)
+            launch(std::integral_constant<int, 2>());
+        else if (k <= 4)
+            launch(std::integral_constant<int, 4>());
+        else if (k <= 8)
+            launch(std::integral_constant<int, 8>());
+        else
+            launch(std::integral_constant<int, 16>());
+    });
+    return check_launch(name);
+}
+
+}  // extern "C"

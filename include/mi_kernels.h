@@ -340,6 +340,110 @@ int mi_relu_backward_with_bias_backward_half_mask(const void* mask16, const floa
                                                   float* grad_in, float* dbias, int rows,
                                                   int cols, void* stream);
 
+/* ----- mixture-of-experts layer: router, rows to their experts and back --- */
+/* No counterpart in the reference, whose feed-forward layer is dense.  Rows
+ * are fp32, fp16 or bf16 (MI_TYPE_*), passed as void*; weights and their
+ * gradients are fp32, sums are formed in fp32 and rounded once, to nearest
+ * even.  Slot t * k + j is choice j of token t; k is 1 to 16, experts 1 to
+ * 1024 (k <= experts), tokens * k at most INT_MAX, cols at most 2^22.  Every
+ * result is the same bits on every call.  No row needs an alignment beyond its
+ * element's.  Buffers must not overlap, except where it says so. */
+#define MI_TYPE_F32 0
+#define MI_TYPE_F16 1
+#define MI_TYPE_BF16 2
+
+/* The k experts of each token with the largest logits [tokens, experts], in
+ * falling order, equal logits by rising expert: ids [tokens, k].  weights
+ * [tokens, k] are their softmax over the chosen ones (renormalise != 0) or over
+ * all experts (0).  A logit of -inf is never chosen: where too few others are
+ * left, id -1 and weight 0.  NaN ranks above every number; a row with a NaN or
+ * +inf that takes part in its sum has NaN weights. */
+int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens, int experts,
+                        int k, int renormalise, int type, void* stream);
+
+/* dlogits (overwritten, all of [tokens, experts]) from dweights [tokens, k],
+ * with ids and weights as the forward call returned them.  Slots with id -1
+ * take no part.  logits may be NULL if renormalise != 0. */
+int mi_moe_gate_backward(const void* logits, const int* ids, const float* weights,
+                         const float* dweights, void* dlogits, int tokens, int experts, int k,
+                         int renormalise, int type, void* stream);
+
+/* Sorts `slots` expert ids, stably.  offsets [experts + 1]: expert e's rows are
+ * offsets[e] .. offsets[e + 1] - 1; position [slots]: the row of each slot, -1
+ * for an id outside [0, experts); order [slots] (NULL: not wanted): the slot of
+ * each row; entries from offsets[experts] on are left as they were.  Above 4096
+ * slots it uses the library workspace. */
+int mi_moe_sort(const int* ids, int* offsets, int* order, int* position, int slots, int experts,
+                void* stream);
+size_t mi_moe_sort_workspace(int slots, int experts);
+
+/* out[position[t * k + j], :] = x[t, :].  x is [tokens, cols], out [rows,
+ * cols]; a slot whose position is outside [0, rows) is dropped, and rows that no
+ * slot has are left as they were. */
+int mi_moe_dispatch_forward(const void* x, const int* position, void* out, int tokens, int k,
+                            int rows, int cols, int type, void* stream);
+
+/* dx[t, :] = sum over j, in order, of dout[position[t * k + j], :]; 0 for a
+ * token without rows. */
+int mi_moe_dispatch_backward(const void* dout, const int* position, void* dx, int tokens, int k,
+                             int rows, int cols, int type, void* stream);
+
+/* out[t, :] = sum over j, in order, of weights[t, j] y[position[t * k + j], :];
+ * 0 for a token without rows. */
+int mi_moe_combine_forward(const void* y, const int* position, const float* weights, void* out,
+                           int tokens, int k, int rows, int cols, int type, void* stream);
+
+/* dy[position[t * k + j], :] = weights[t, j] dout[t, :] (other rows are left as
+ * they were); dweights[t, j] = the product of dout[t, :] and y[position[t * k +
+ * j], :], 0 for a dropped slot.  dy may be y. */
+int mi_moe_combine_backward(const void* dout, const void* y, const int* position,
+                            const float* weights, void* dy, float* dweights, int tokens, int k,
+                            int rows, int cols, int type, void* stream);
+
+/* ----- activations kept in 8 bits for the backward pass ------------------- */
+/* A checkpoint of [rows, cols] is q [rows, cols] (bytes) and scales [rows,
+ * ceil(cols / 32)] (bytes): 32 consecutive columns of a row share a power of
+ * two.  With e = max(floor(log2 of the block's largest magnitude), -118) the
+ * scale byte is e + 127, and an element x is held as
+ *   MI_CKPT8_INT8: the integer rint(x 2^(6-e)), cut at 127, of value q 2^(e-6);
+ *   MI_CKPT8_E4M3: the OCP e4m3 number nearest to x 2^(8-e), cut at +-448, of
+ *                  value q 2^(e-8).
+ * A block with a NaN or an infinity has scale byte 255 and reads as NaN.  Half
+ * values round to even.  rows at most 2^30, cols at most 2^24; no alignment
+ * beyond the element's is needed. */
+#define MI_CKPT8_BLOCK 32
+#define MI_CKPT8_INT8 0
+#define MI_CKPT8_E4M3 1
+
+/* The checkpoint of `in`, and what it stands for, as MI_TYPE_* rows. */
+int mi_float_to_ckpt8(const void* in, void* q, void* scales, int rows, int cols, int format,
+                      int type, void* stream);
+int mi_ckpt8_to_float(const void* q, const void* scales, void* out, int rows, int cols, int format,
+                      int type, void* stream);
+
+/* out = gelu(in + bias[g]) and the checkpoint of in.  Rows belong to `groups`
+ * (1 to 1024) consecutive segments, g's being offsets[g] .. offsets[g + 1] - 1
+ * (as mi_moe_sort writes them; a rising list of groups + 1 device ints); bias is
+ * [groups, cols], fp32.  Rows outside the segments are left as they were, in
+ * out, q and scales.  offsets may be NULL for one group: all rows.  out may be
+ * in. */
+int mi_bias_gelu_forward_ckpt8(const void* in, const float* bias, const int* offsets, void* out,
+                               void* q, void* scales, int rows, int cols, int groups, int format,
+                               int type, void* stream);
+
+/* From the checkpoint of in: u = value + bias[g]; grad_in = grad_out *
+ * gelu_tanh'(u); act = gelu(u) (NULL: not wanted), the activation as the next
+ * product's weight gradient needs it; dbias [groups, cols] += column sums of
+ * the unrounded grad_in over each segment (fp32, deterministic, through the
+ * library workspace).  Rows outside the segments are left as they were.
+ * grad_in may be grad_out. */
+int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales, const float* bias,
+                                              const int* offsets, const void* grad_out,
+                                              void* grad_in, void* act, float* dbias, int rows,
+                                              int cols, int groups, int format, int type,
+                                              void* stream);
+size_t mi_gelu_backward_ckpt8_workspace(int rows, int cols, int groups);
+
 #ifdef __cplusplus
 }
 #endif
