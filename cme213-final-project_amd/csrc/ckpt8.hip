@@ -27,9 +27,8 @@ namespace mi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kUnit = 8;                 // consecutive columns of one lane
-constexpr int kTile = kUnit * kWave;     // columns of one wave
+constexpr int kTile = kUnit * kWave;     // columns of a full tile
 constexpr int kBlock = MI_CKPT8_BLOCK;   // four lanes
 constexpr int kMaxGroups = 1024;
 constexpr int kMaxRows = 1 << 30;  // keep row and column numbers, one tile or band
@@ -37,18 +36,34 @@ constexpr int kMaxCols = 1 << 24;  // further on, inside an int, and the grids l
 static_assert(kBlock == 4 * kUnit, "a block's lanes are one DPP quad");
 
 // ---------------------------------------------------------------------------
-// A wave takes one tile of 512 columns and a band of consecutive rows: lane i
-// owns columns 8 i .. 8 i + 7 of the tile, so four adjacent lanes hold a block.
-// The lane's biases and column sums stay in registers over the band.
+// A lane takes 8 consecutive columns of a row (a unit), so four adjacent lanes
+// hold a block.  A workgroup takes a tile of columns and a band of consecutive
+// rows; its threads are `lanes` units wide and `row_lanes` rows deep.  Tiles are
+// 64 units wide (512 columns, one wave a row); what is left of the width is a
+// narrower tile of its own, with more rows at a time, so that few lanes idle.
 // ---------------------------------------------------------------------------
 struct Unit {
     int col;  // first column
     int n;    // columns of it inside the row, 0 to 8
 };
 
-__device__ __forceinline__ Unit lane_unit(int tile, int cols) {
-    const int col = tile * kTile + (threadIdx.x & (kWave - 1)) * kUnit;
-    return {col, max(0, min(kUnit, cols - col))};
+struct Task {
+    int tile, band;
+    int lanes, row_lanes;
+    int row_lane;
+    Unit un;
+};
+
+__device__ __forceinline__ Task workgroup_task(int cols, int tiles, int last_lanes) {
+    Task t;
+    t.tile = static_cast<int>(blockIdx.x % static_cast<unsigned>(tiles));
+    t.band = static_cast<int>(blockIdx.x / static_cast<unsigned>(tiles));
+    t.lanes = t.tile == tiles - 1 ? last_lanes : kWave;
+    t.row_lanes = kThreads / t.lanes;
+    t.row_lane = static_cast<int>(threadIdx.x) / t.lanes;
+    t.un.col = t.tile * kTile + static_cast<int>(threadIdx.x & (t.lanes - 1)) * kUnit;
+    t.un.n = max(0, min(kUnit, cols - t.un.col));
+    return t;
 }
 
 template <int T>
@@ -132,13 +147,29 @@ __device__ __forceinline__ void store_codes(uint8_t* row, const Unit& un, const 
 
 // The scale byte of the block that the lane's quad holds.  Magnitudes compare
 // as integers, with NaN and infinity above every number, and the exponent
-// field of the largest is e + 127.
-__device__ __forceinline__ int block_scale(const float (&v)[kUnit]) {
+// field of the largest is e + 127.  Two 16-bit magnitudes compare at a time.
+template <int T>
+__device__ __forceinline__ int block_scale(const RawUnit<T>& r) {
     int m = 0;
+    if constexpr (T == MI_TYPE_F32) {
 #pragma unroll
-    for (int e = 0; e < kUnit; ++e) m = max(m, __float_as_int(v[e]) & 0x7fffffff);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = max(m, static_cast<int>(r.a[i][e] & 0x7fffffffu));
+    } else {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 p = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            p = __builtin_elementwise_max(p, __builtin_bit_cast(u16x2, r.a[0][e] & 0x7fff7fffu));
+        m = max(p.x, p.y);
+    }
     m = max(m, dpp_move_i<0xB1>(m));
     m = max(m, dpp_move_i<0x4E>(m));
+    if constexpr (T == MI_TYPE_BF16) m <<= 16;
+    if constexpr (T == MI_TYPE_F16)
+        m = __float_as_int(
+            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m))));
     return max(m >> 23, 9);
 }
 
@@ -172,24 +203,28 @@ __device__ __forceinline__ u32x2 encode(const float (&v)[kUnit], int scale) {
     return q;
 }
 
+// value + add: the product is exact, so this is one rounding, of the sum.
 template <int FMT>
-__device__ __forceinline__ void decode(const u32x2& q, int scale, float (&v)[kUnit]) {
+__device__ __forceinline__ void decode(const u32x2& q, int scale, const float (&add)[kUnit],
+                                       float (&v)[kUnit]) {
     const float step = scale == 255
                            ? __int_as_float(0x7fc00000)
                            : __builtin_ldexpf(1.0f, scale - (FMT == MI_CKPT8_INT8 ? 133 : 135));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int w = static_cast<int>(q[h]);
+        float x[4];
         if constexpr (FMT == MI_CKPT8_INT8) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[4 * h + e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e))) * step;
+            for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
         } else {
-            v[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8(w, 0) * step;
-            v[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(w, 1) * step;
-            v[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(w, 2) * step;
-            v[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3) * step;
+            x[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
+            x[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+            x[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
+            x[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = fmaf(x[e], step, add[4 * h + e]);
     }
 }
 
@@ -228,179 +263,244 @@ __device__ __forceinline__ void load_bias(const float* bias, int g, int cols, co
     for (int e = 0; e < kUnit; ++e) b[e] = e < un.n ? p[e] : 0.0f;
 }
 
-struct WaveTask {
-    int tile, band;
-};
-
-__device__ __forceinline__ WaveTask wave_task(int tiles) {
-    const unsigned w = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    return {static_cast<int>(w % tiles), static_cast<int>(w / tiles)};
+// f(g, a, b) for the rows a .. b - 1 of group g inside r0 .. r1 - 1.  Everything
+// here is the same for a whole workgroup.
+template <class F>
+__device__ __forceinline__ void for_segments(const int* offsets, int groups, int rows, int r0,
+                                             int r1, F f) {
+    if (offsets == nullptr) {
+        f(0, r0, r1);
+        return;
+    }
+    int a = max(r0, first_row(offsets, rows));
+    if (a >= r1) return;
+    for (int g = group_of(offsets, groups, rows, a); a < r1 && g < groups; ++g) {
+        const int b = min(group_end(offsets, g, rows), r1);
+        if (b > a) {
+            f(g, a, b);
+            a = b;
+        }
+    }
 }
 
+#ifndef MI_CKPT8_FWD_ROWS
+#define MI_CKPT8_FWD_ROWS 2
+#endif
+#ifndef MI_CKPT8_FWD_TRIPS
+#define MI_CKPT8_FWD_TRIPS 4
+#endif
+#ifndef MI_CKPT8_BWD_ROWS
+#define MI_CKPT8_BWD_ROWS 2
+#endif
+
 // GELU: out = gelu(in + bias) and the checkpoint of in; else the checkpoint.
-// out may be in: a lane reads its unit of a row before it writes it.
+// out may be in: a lane reads its units of the rows in hand before it writes
+// them.
 template <int T, int FMT, bool GELU>
 __global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
     const char* in, const float* __restrict__ bias, const int* __restrict__ offsets, char* out,
     uint8_t* __restrict__ q, uint8_t* __restrict__ scales, int rows, int cols, int groups,
-    int band, int tiles, int bands) {
-    const WaveTask task = wave_task(tiles);
-    if (task.band >= bands) return;
-    const Unit un = lane_unit(task.tile, cols);
+    int band, int tiles, int last_lanes) {
+    constexpr int U = MI_CKPT8_FWD_ROWS;
+    const Task t = workgroup_task(cols, tiles, last_lanes);
+    const Unit un = t.un;
     const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
     const int blocks = (cols + kBlock - 1) / kBlock;
-    const int r1 = min((task.band + 1) * band, rows);
-    int r0 = task.band * band, g = 0, end = r1;
-    float b[kUnit];
-    if constexpr (GELU) {
-        r0 = max(r0, first_row(offsets, rows));
-        g = group_of(offsets, groups, rows, r0);
-        end = r0;  // the first row loads its group's bias
-    }
-    for (int r = r0; r < r1; ++r) {
-        if constexpr (GELU) {
-            if (r >= end) {
-                while (g < groups && group_end(offsets, g, rows) <= r) ++g;
-                if (g >= groups) break;
-                end = group_end(offsets, g, rows);
-                load_bias(bias, g, cols, un, b);
+    const int r0 = t.band * band, r1 = min(r0 + band, rows);
+    for_segments(offsets, groups, rows, r0, r1, [&](int g, int a, int end) {
+        float b[kUnit];
+        if constexpr (GELU) load_bias(bias, g, cols, un, b);
+        for (int r = a + t.row_lane; r < end; r += U * t.row_lanes) {
+            RawUnit<T> raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int rr = r + u * t.row_lanes;
+                raw[u] = load_unit<T>(in + (rr < end ? rr : r) * row_bytes, un);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int rr = r + u * t.row_lanes;
+                if (rr >= end) break;
+                const int scale = block_scale<T>(raw[u]);
+                float v[kUnit];
+                unpack_unit<T>(raw[u], v);
+                store_codes(q + static_cast<size_t>(rr) * cols, un, encode<FMT>(v, scale));
+                if (un.n > 0 && un.col % kBlock == 0)
+                    scales[static_cast<size_t>(rr) * blocks + un.col / kBlock] =
+                        static_cast<uint8_t>(scale);
+                if constexpr (GELU) {
+#pragma unroll
+                    for (int e = 0; e < kUnit; ++e) v[e] = gelu_pair(v[e] + b[e]).y;
+                    store_unit<T>(out + rr * row_bytes, un, v);
+                }
             }
         }
-        float v[kUnit];
-        unpack_unit<T>(load_unit<T>(in + r * row_bytes, un), v);
-        const int scale = block_scale(v);
-        store_codes(q + static_cast<size_t>(r) * cols, un, encode<FMT>(v, scale));
-        if (un.n > 0 && un.col % kBlock == 0)
-            scales[static_cast<size_t>(r) * blocks + un.col / kBlock] = static_cast<uint8_t>(scale);
-        if constexpr (GELU) {
-#pragma unroll
-            for (int e = 0; e < kUnit; ++e) v[e] = gelu_fwd(v[e] + b[e]);
-            store_unit<T>(out + r * row_bytes, un, v);
-        }
-    }
+    });
 }
 
 template <int T, int FMT>
 __global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
     const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, char* __restrict__ out,
-    int rows, int cols, int band, int tiles, int bands) {
-    const WaveTask task = wave_task(tiles);
-    if (task.band >= bands) return;
-    const Unit un = lane_unit(task.tile, cols);
+    int rows, int cols, int band, int tiles, int last_lanes) {
+    const Task t = workgroup_task(cols, tiles, last_lanes);
+    const Unit un = t.un;
     if (un.n == 0) return;
     const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
     const int blocks = (cols + kBlock - 1) / kBlock;
-    const int r0 = task.band * band, r1 = min(r0 + band, rows);
-    for (int r = r0; r < r1; ++r) {
+    const int r0 = t.band * band, r1 = min(r0 + band, rows);
+    const float none[kUnit] = {};
+    for (int r = r0 + t.row_lane; r < r1; r += t.row_lanes) {
         float v[kUnit];
         decode<FMT>(load_codes(q + static_cast<size_t>(r) * cols, un),
-                    scales[static_cast<size_t>(r) * blocks + un.col / kBlock], v);
+                    scales[static_cast<size_t>(r) * blocks + un.col / kBlock], none, v);
         store_unit<T>(out + r * row_bytes, un, v);
     }
 }
 
 // u = value of the checkpoint + bias; grad_in = grad_out gelu'(u); act =
-// gelu(u); the column sums of grad_in over the band's rows of group g go to
-// partial row band + g.  Going down the rows, band and g only grow, and one of
-// them does with every new pair, so no two pairs share a partial row.
-// grad_in may be grad_out.
+// gelu(u); the column sums of grad_in over the band's rows of group g, added
+// over the row lanes in order, go to partial row band + g.  Going down the
+// rows, band and g only grow, and one of them does with every new pair, so no
+// two pairs share a partial row.  grad_in may be grad_out.
 template <int T, int FMT, bool ACT>
 __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
     const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales,
     const float* __restrict__ bias, const int* __restrict__ offsets, const char* grad_out,
     char* grad_in, char* __restrict__ act, float* __restrict__ part, int rows, int cols,
-    int groups, int band, int tiles, int bands) {
-    const WaveTask task = wave_task(tiles);
-    if (task.band >= bands) return;
-    const Unit un = lane_unit(task.tile, cols);
-    if (un.n == 0) return;
+    int groups, int band, int tiles, int last_lanes) {
+    constexpr int U = MI_CKPT8_BWD_ROWS;
+    __shared__ float red[kThreads * kUnit];
+    const Task t = workgroup_task(cols, tiles, last_lanes);
+    const Unit un = t.un;
     const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
     const int blocks = (cols + kBlock - 1) / kBlock;
-    const int r0 = max(task.band * band, first_row(offsets, rows));
-    const int r1 = min((task.band + 1) * band, rows);
-    if (r0 >= r1) return;
-    int g = group_of(offsets, groups, rows, r0), end = r0;
-    float b[kUnit], acc[kUnit];
-    auto flush = [&]() {
-        float* p = part + static_cast<size_t>(task.band + g) * cols + un.col;
+    const int scale_at = min(un.col / kBlock, blocks - 1);
+    const int r0 = t.band * band, r1 = min(r0 + band, rows);
+    for_segments(offsets, groups, rows, r0, r1, [&](int g, int a, int end) {
+        float b[kUnit], acc[kUnit];
+        load_bias(bias, g, cols, un, b);
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e)
-            if (e < un.n) p[e] = acc[e];
-    };
-    for (int r = r0; r < r1; ++r) {
-        if (r >= end) {
-            if (r > r0) flush();
-            while (g < groups && group_end(offsets, g, rows) <= r) ++g;
-            if (g >= groups) return;
-            end = group_end(offsets, g, rows);
-            load_bias(bias, g, cols, un, b);
+        for (int e = 0; e < kUnit; ++e) acc[e] = 0.0f;
+        for (int r = a + t.row_lane; r < end; r += U * t.row_lanes) {
+            RawUnit<T> raw[U];
+            u32x2 code[U];
+            int scale[U];
 #pragma unroll
-            for (int e = 0; e < kUnit; ++e) acc[e] = 0.0f;
+            for (int u = 0; u < U; ++u) {
+                const int want = r + u * t.row_lanes;
+                const size_t rr = want < end ? want : r;
+                code[u] = load_codes(q + rr * cols, un);
+                scale[u] = scales[rr * blocks + scale_at];
+                raw[u] = load_unit<T>(grad_out + rr * row_bytes, un);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int rr = r + u * t.row_lanes;
+                if (rr >= end) break;
+                float v[kUnit], d[kUnit];
+                unpack_unit<T>(raw[u], d);
+                decode<FMT>(code[u], scale[u], b, v);
+#pragma unroll
+                for (int e = 0; e < kUnit; ++e) {
+                    const GeluPair p = gelu_pair(v[e]);
+                    acc[e] = fmaf(d[e], p.d, acc[e]);
+                    d[e] *= p.d;
+                    v[e] = p.y;
+                }
+                store_unit<T>(grad_in + rr * row_bytes, un, d);
+                if constexpr (ACT) store_unit<T>(act + rr * row_bytes, un, v);
+            }
         }
-        float v[kUnit], d[kUnit];
-        unpack_unit<T>(load_unit<T>(grad_out + r * row_bytes, un), d);
-        decode<FMT>(load_codes(q + static_cast<size_t>(r) * cols, un),
-                    scales[static_cast<size_t>(r) * blocks + un.col / kBlock], v);
+        const int width = t.lanes * kUnit;
+        float* mine = red + threadIdx.x * kUnit;
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e) {
-            const float u = v[e] + b[e];
-            d[e] *= gelu_grad(u);
-            acc[e] += d[e];
-            if constexpr (ACT) v[e] = gelu_fwd(u);
+        for (int e = 0; e < kUnit; ++e) mine[e] = acc[e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < width; c += kThreads) {
+            float s = red[c];
+            for (int l = 1; l < t.row_lanes; ++l) s += red[l * width + c];
+            if (t.tile * kTile + c < cols)
+                part[static_cast<size_t>(t.band + g) * cols + t.tile * kTile + c] = s;
         }
-        store_unit<T>(grad_in + r * row_bytes, un, d);
-        if constexpr (ACT) store_unit<T>(act + r * row_bytes, un, v);
-    }
-    if (g < groups) flush();
+        __syncthreads();
+    });
 }
 
-// dbias[g][c] += sum of group g's partial rows, in band order within 16 slices
-// and then over the slices.
-constexpr int kFinThreads = 512;
-constexpr int kFinCols = 32;
-constexpr int kFinSlices = kFinThreads / kFinCols;
-
-__global__ __launch_bounds__(kFinThreads) void group_sum_kernel(
-    const float* __restrict__ part, const int* __restrict__ offsets, float* __restrict__ dbias,
-    int rows, int cols, int band) {
-    __shared__ float tot[kFinSlices][kFinCols];
+// dbias[g][c] += sum of group g's partial rows: 64 columns a workgroup, its
+// waves each a consecutive slice of the partial rows in order, then the waves
+// in order.  Loads are issued 16 at a time.
+__global__ __launch_bounds__(1024) void group_sum_kernel(const float* __restrict__ part,
+                                                         const int* __restrict__ offsets,
+                                                         float* __restrict__ dbias, int rows,
+                                                         int cols, int band, int slices) {
+    constexpr int CH = 16;
+    __shared__ float tot[1024 / kWave][kWave];
     const int g = blockIdx.y;
     const int start = g == 0 ? first_row(offsets, rows) : group_end(offsets, g - 1, rows);
     const int end = group_end(offsets, g, rows);
     if (start >= end) return;
-    const int c = blockIdx.x * kFinCols + threadIdx.x % kFinCols;
-    const int slice = threadIdx.x / kFinCols;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int slice = threadIdx.x / kWave;
+    const int c = blockIdx.x * kWave + lane;
     const int first = start / band, n = (end - 1) / band - first + 1;
-    const int p0 = static_cast<int>(static_cast<long long>(slice) * n / kFinSlices);
-    const int p1 = static_cast<int>(static_cast<long long>(slice + 1) * n / kFinSlices);
+    const int p0 = static_cast<int>(static_cast<long long>(slice) * n / slices);
+    const int p1 = static_cast<int>(static_cast<long long>(slice + 1) * n / slices);
+    float* o = dbias + static_cast<size_t>(g) * cols + c;
+    const float old = slice == 0 && c < cols ? *o : 0.0f;
     float s = 0.0f;
-    if (c < cols)
-        for (int p = p0; p < p1; ++p) s += part[static_cast<size_t>(first + p + g) * cols + c];
-    tot[slice][threadIdx.x % kFinCols] = s;
+    if (c < cols) {
+        const float* col = part + static_cast<size_t>(first + g) * cols + c;
+        for (int p = p0; p < p1; p += CH) {
+            float v[CH];
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                v[i] = p + i < p1 ? col[static_cast<size_t>(p + i) * cols] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                if (p + i < p1) s += v[i];
+        }
+    }
+    tot[slice][lane] = s;
     __syncthreads();
     if (slice == 0 && c < cols) {
-        float t = tot[0][threadIdx.x];
-#pragma unroll
-        for (int w = 1; w < kFinSlices; ++w) t += tot[w][threadIdx.x];
-        dbias[static_cast<size_t>(g) * cols + c] += t;
+        float sum = tot[0][lane];
+        for (int w = 1; w < slices; ++w) sum += tot[w][lane];
+        *o = old + sum;
     }
 }
 
 struct Plan {
-    int band, bands, tiles;
+    int band, bands, tiles, last_lanes;
     unsigned grid;
 };
 
-// Rows per band: few enough that the waves fill the chip, and at most 64.
-Plan plan_ckpt8(int rows, int cols) {
-    const long long tiles = (static_cast<long long>(cols) + kTile - 1) / kTile;
-    long long band = static_cast<long long>(rows) * tiles / 8192;
-    band = std::min<long long>(std::max<long long>(band, 1), 64);
-    // the waves' number stays below 2^24
-    band = std::max(band, (static_cast<long long>(rows) * tiles >> 24) + 1);
-    const long long bands = (rows + band - 1) / band;
-    return {static_cast<int>(band), static_cast<int>(bands), static_cast<int>(tiles),
-            static_cast<unsigned>((bands * tiles + kWaves - 1) / kWaves)};
+// Row lanes of the narrowest tile; bands: at most `most` over the rows.
+Plan plan_ckpt8(int rows, int cols, int most, int least_trips) {
+    Plan p;
+    const int left = cols % kTile;
+    p.tiles = cols / kTile + (left ? 1 : 0);
+    p.last_lanes = kWave;
+    if (left) {
+        p.last_lanes = 4;
+        while (p.last_lanes * kUnit < left) p.last_lanes *= 2;
+    }
+    const int row_lanes = kThreads / (p.tiles == 1 ? p.last_lanes : kWave);
+    most = std::min(most, (1 << 23) / p.tiles);  // a legal grid
+    long long band = (static_cast<long long>(rows) + most - 1) / most;
+    band = std::max<long long>(band, least_trips * row_lanes);
+    p.band = static_cast<int>(band);
+    p.bands = static_cast<int>((rows + band - 1) / band);
+    p.grid = static_cast<unsigned>(static_cast<long long>(p.bands) * p.tiles);
+    return p;
+}
+
+// Forward: no sums, so bands are as short as keeps a lane a few rows.
+Plan plan_forward(int rows, int cols) { return plan_ckpt8(rows, cols, 4096, MI_CKPT8_FWD_TRIPS); }
+
+// Backward: every band leaves a partial row to add up.
+Plan plan_backward(int rows, int cols) {
+    const int tiles = (cols + kTile - 1) / kTile;
+    return plan_ckpt8(rows, cols, std::min(1024, std::max(256, 2048 / tiles)), 2);
 }
 
 int check_args(const char* name, int rows, int cols, int groups, int format, int type) {
@@ -429,14 +529,14 @@ template <bool GELU>
 int launch_to_ckpt8(const char* name, const void* in, const float* bias, const int* offsets,
                     void* out, void* q, void* scales, int rows, int cols, int groups, int format,
                     int type, hipStream_t st) {
-    const Plan p = plan_ckpt8(rows, cols);
+    const Plan p = plan_forward(rows, cols);
     with_row_type(type, [&](auto t) {
         with_format(format, [&](auto f) {
             hipLaunchKernelGGL((to_ckpt8_kernel<decltype(t)::value, decltype(f)::value, GELU>),
                                dim3(p.grid), dim3(kThreads), 0, st, static_cast<const char*>(in),
                                bias, offsets, static_cast<char*>(out), static_cast<uint8_t*>(q),
                                static_cast<uint8_t*>(scales), rows, cols, groups, p.band, p.tiles,
-                               p.bands);
+                               p.last_lanes);
         });
     });
     return check_launch(name);
@@ -465,13 +565,14 @@ int mi_ckpt8_to_float(const void* q, const void* scales, void* out, int rows, in
     if (int rc = check_args(name, rows, cols, 1, format, type)) return rc;
     if (rows == 0) return MI_OK;
     if (!q || !scales || !out) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
-    const Plan p = plan_ckpt8(rows, cols);
+    const Plan p = plan_forward(rows, cols);
     with_row_type(type, [&](auto t) {
         with_format(format, [&](auto f) {
             hipLaunchKernelGGL((from_ckpt8_kernel<decltype(t)::value, decltype(f)::value>),
                                dim3(p.grid), dim3(kThreads), 0, to_stream(stream),
                                static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales),
-                               static_cast<char*>(out), rows, cols, p.band, p.tiles, p.bands);
+                               static_cast<char*>(out), rows, cols, p.band, p.tiles,
+                               p.last_lanes);
         });
     });
     return check_launch(name);
@@ -493,7 +594,7 @@ int mi_bias_gelu_forward_ckpt8(const void* in, const float* bias, const int* off
 
 size_t mi_gelu_backward_ckpt8_workspace(int rows, int cols, int groups) {
     if (rows <= 0 || cols <= 0 || groups <= 0) return 0;
-    return colsum_bytes(plan_ckpt8(rows, cols).bands + groups - 1, cols);
+    return colsum_bytes(plan_backward(rows, cols).bands + groups - 1, cols);
 }
 
 int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales, const float* bias,
@@ -509,7 +610,7 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
     if (groups > 1 && !offsets)
         return set_error(MI_ERR_INVALID_ARG, "%s: %d groups need offsets", name, groups);
     hipStream_t st = to_stream(stream);
-    const Plan p = plan_ckpt8(rows, cols);
+    const Plan p = plan_backward(rows, cols);
     int err = MI_OK;
     char* ws = static_cast<char*>(
         workspace_get(mi_gelu_backward_ckpt8_workspace(rows, cols, groups), st, &err));
@@ -524,7 +625,7 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
                                    static_cast<const uint8_t*>(scales), bias, offsets,
                                    static_cast<const char*>(grad_out), static_cast<char*>(grad_in),
                                    static_cast<char*>(act), part, rows, cols, groups, p.band,
-                                   p.tiles, p.bands);
+                                   p.tiles, p.last_lanes);
             };
             if (act != nullptr)
                 launch(std::true_type());
@@ -533,8 +634,11 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
         });
     });
     if (int rc = check_launch(name)) return rc;
-    hipLaunchKernelGGL(group_sum_kernel, dim3((cols + kFinCols - 1) / kFinCols, groups),
-                       dim3(kFinThreads), 0, st, part, offsets, dbias, rows, cols, p.band);
+    const int each = p.bands / groups;  // partial rows of a group, about
+    const int slices = each >= 64 ? 16 : each >= 16 ? 8 : each >= 8 ? 4 : 1;
+    hipLaunchKernelGGL(group_sum_kernel, dim3((cols + kWave - 1) / kWave, groups),
+                       dim3(slices * kWave), 0, st, part, offsets, dbias, rows, cols, p.band,
+                       slices);
     return check_launch(name);
 }
 

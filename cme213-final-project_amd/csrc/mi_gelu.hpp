@@ -58,6 +58,24 @@ __device__ __forceinline__ float gelu_grad(float u) {
     return g.zero ? 0.0f : (g.e == 0.0f ? g.s : d);
 }
 
+// The same two functions where both are wanted, or where instructions count: u
+// is clamped, NaN kept, instead of the exponent, so no case is set apart.  Past
+// +-10 the exponent stays at +-125.97: above, s is 1 and gelu' is 1 to the last
+// bit; below, gelu and gelu' come out under 1e-34 in magnitude instead of 0.
+struct GeluPair {
+    float y;  // gelu(u)
+    float d;  // gelu'(u)
+};
+
+__device__ __forceinline__ GeluPair gelu_pair(float u) {
+    const float lo = __builtin_elementwise_maximum(u, -10.0f);
+    const float c = __builtin_elementwise_minimum(lo, 10.0f);
+    const float c2 = c * c;
+    const float e = __builtin_amdgcn_exp2f(c * fmaf(kT1, c2, kT0));
+    const float s = __builtin_amdgcn_rcpf(1.0f + e);
+    return {lo * s, s * fmaf(c * (e * s), fmaf(kD1, c2, kD0), 1.0f)};
+}
+
 }  // namespace
 
 }  // namespace mi
