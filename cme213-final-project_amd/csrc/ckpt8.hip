@@ -71,13 +71,13 @@ struct RawUnit {
     u32x4 a[kUnit / row_vec<T>()];
 };
 
-template <int T>
+template <int T, bool NT>
 __device__ __forceinline__ RawUnit<T> load_unit(const char* row, const Unit& un) {
     RawUnit<T> r;
     const char* p = row + static_cast<size_t>(un.col) * sizeof(row_elem<T>);
     if (un.n == kUnit) {
 #pragma unroll
-        for (int i = 0; i < kUnit / row_vec<T>(); ++i) r.a[i] = load16b(p + 16 * i);
+        for (int i = 0; i < kUnit / row_vec<T>(); ++i) r.a[i] = load16b<NT>(p + 16 * i);
     } else {
 #pragma unroll
         for (int i = 0; i < kUnit / row_vec<T>(); ++i) {
@@ -296,7 +296,7 @@ __device__ __forceinline__ void for_segments(const int* offsets, int groups, int
 // GELU: out = gelu(in + bias) and the checkpoint of in; else the checkpoint.
 // out may be in: a lane reads its units of the rows in hand before it writes
 // them.
-template <int T, int FMT, bool GELU>
+template <int T, int FMT, bool GELU, bool NT>
 __global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
     const char* in, const float* __restrict__ bias, const int* __restrict__ offsets, char* out,
     uint8_t* __restrict__ q, uint8_t* __restrict__ scales, int rows, int cols, int groups,
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int rr = r + u * t.row_lanes;
-                raw[u] = load_unit<T>(in + (rr < end ? rr : r) * row_bytes, un);
+                raw[u] = load_unit<T, NT>(in + (rr < end ? rr : r) * row_bytes, un);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
 // over the row lanes in order, go to partial row band + g.  Going down the
 // rows, band and g only grow, and one of them does with every new pair, so no
 // two pairs share a partial row.  grad_in may be grad_out.
-template <int T, int FMT, bool ACT>
+template <int T, int FMT, bool ACT, bool NT>
 __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
     const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales,
     const float* __restrict__ bias, const int* __restrict__ offsets, const char* grad_out,
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
                 const size_t rr = want < end ? want : r;
                 code[u] = load_codes(q + rr * cols, un);
                 scale[u] = scales[rr * blocks + scale_at];
-                raw[u] = load_unit<T>(grad_out + rr * row_bytes, un);
+                raw[u] = load_unit<T, NT>(grad_out + rr * row_bytes, un);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -530,13 +530,18 @@ int launch_to_ckpt8(const char* name, const void* in, const float* bias, const i
                     void* out, void* q, void* scales, int rows, int cols, int groups, int format,
                     int type, hipStream_t st) {
     const Plan p = plan_forward(rows, cols);
+    const double bytes =
+        static_cast<double>(rows) * cols * ((GELU ? 2 : 1) * row_type_size(type) + 1);
     with_row_type(type, [&](auto t) {
         with_format(format, [&](auto f) {
-            hipLaunchKernelGGL((to_ckpt8_kernel<decltype(t)::value, decltype(f)::value, GELU>),
-                               dim3(p.grid), dim3(kThreads), 0, st, static_cast<const char*>(in),
-                               bias, offsets, static_cast<char*>(out), static_cast<uint8_t*>(q),
-                               static_cast<uint8_t*>(scales), rows, cols, groups, p.band, p.tiles,
-                               p.last_lanes);
+            constexpr int T = decltype(t)::value, F = decltype(f)::value;
+            with_flag(stream_loads(bytes), [&](auto nt) {
+                hipLaunchKernelGGL((to_ckpt8_kernel<T, F, GELU, decltype(nt)::value>), dim3(p.grid),
+                                   dim3(kThreads), 0, st, static_cast<const char*>(in), bias,
+                                   offsets, static_cast<char*>(out), static_cast<uint8_t*>(q),
+                                   static_cast<uint8_t*>(scales), rows, cols, groups, p.band,
+                                   p.tiles, p.last_lanes);
+            });
         });
     });
     return check_launch(name);
@@ -568,11 +573,11 @@ int mi_ckpt8_to_float(const void* q, const void* scales, void* out, int rows, in
     const Plan p = plan_forward(rows, cols);
     with_row_type(type, [&](auto t) {
         with_format(format, [&](auto f) {
-            hipLaunchKernelGGL((from_ckpt8_kernel<decltype(t)::value, decltype(f)::value>),
-                               dim3(p.grid), dim3(kThreads), 0, to_stream(stream),
-                               static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales),
-                               static_cast<char*>(out), rows, cols, p.band, p.tiles,
-                               p.last_lanes);
+            constexpr int T = decltype(t)::value, F = decltype(f)::value;
+            hipLaunchKernelGGL((from_ckpt8_kernel<T, F>), dim3(p.grid), dim3(kThreads), 0,
+                               to_stream(stream), static_cast<const uint8_t*>(q),
+                               static_cast<const uint8_t*>(scales), static_cast<char*>(out), rows,
+                               cols, p.band, p.tiles, p.last_lanes);
         });
     });
     return check_launch(name);
@@ -616,21 +621,22 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
         workspace_get(mi_gelu_backward_ckpt8_workspace(rows, cols, groups), st, &err));
     if (!ws) return err;
     float* part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    const double bytes = static_cast<double>(rows) * cols *
+                         ((act != nullptr ? 3 : 2) * row_type_size(type) + 1);
     with_row_type(type, [&](auto t) {
         with_format(format, [&](auto f) {
             constexpr int T = decltype(t)::value, F = decltype(f)::value;
-            auto launch = [&](auto a) {
-                hipLaunchKernelGGL((gelu_bwd_ckpt8_kernel<T, F, decltype(a)::value>), dim3(p.grid),
-                                   dim3(kThreads), 0, st, static_cast<const uint8_t*>(q),
-                                   static_cast<const uint8_t*>(scales), bias, offsets,
-                                   static_cast<const char*>(grad_out), static_cast<char*>(grad_in),
-                                   static_cast<char*>(act), part, rows, cols, groups, p.band,
-                                   p.tiles, p.last_lanes);
-            };
-            if (act != nullptr)
-                launch(std::true_type());
-            else
-                launch(std::false_type());
+            with_flag(act != nullptr, [&](auto a) {
+                with_flag(stream_loads(bytes), [&](auto nt) {
+                    constexpr bool A = decltype(a)::value, NT = decltype(nt)::value;
+                    hipLaunchKernelGGL((gelu_bwd_ckpt8_kernel<T, F, A, NT>), dim3(p.grid),
+                                       dim3(kThreads), 0, st, static_cast<const uint8_t*>(q),
+                                       static_cast<const uint8_t*>(scales), bias, offsets,
+                                       static_cast<const char*>(grad_out),
+                                       static_cast<char*>(grad_in), static_cast<char*>(act), part,
+                                       rows, cols, groups, p.band, p.tiles, p.last_lanes);
+                });
+            });
         });
     });
     if (int rc = check_launch(name)) return rc;

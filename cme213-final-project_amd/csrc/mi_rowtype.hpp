@@ -51,12 +51,28 @@ __device__ __forceinline__ void row_put(void* p, size_t i, float v) {
     static_cast<row_elem<T>*>(p)[i] = static_cast<row_elem<T>>(v);
 }
 
+// NT: the line is not kept in the caches.
+template <bool NT>
 __device__ __forceinline__ u32x4 load16b(const void* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(static_cast<const u32x4_at2*>(p));
     return *static_cast<const u32x4_at2*>(p);
 }
 
 __device__ __forceinline__ void store16b(void* p, const u32x4& v) {
-    *static_cast<u32x4_at2*>(p) = v;
+    __builtin_nontemporal_store(v, static_cast<u32x4_at2*>(p));
+}
+
+#ifndef MI_STREAM_MB
+#define MI_STREAM_MB 128
+#endif
+inline bool stream_loads(double bytes) { return bytes > MI_STREAM_MB * 1048576.0; }
+
+template <class F>
+void with_flag(bool on, F f) {
+    if (on)
+        f(std::true_type());
+    else
+        f(std::false_type());
 }
 
 template <int T>

@@ -371,7 +371,7 @@ __global__ __launch_bounds__(kThreads) void scatter_rows_kernel(
         for (int u = 0; u < U; ++u) {
             ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * kWave + u * kWave + lane, chunks,
                               row_bytes);
-            if (ch[u].on) v[u] = load16b(src + ch[u].at);
+            if (ch[u].on) v[u] = load16b<false>(src + ch[u].at);
         }
         const int* pos = position + static_cast<size_t>(token) * k;
         for (int j = 0; j < k; ++j) {
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void scatter_rows_kernel(
 }
 
 // out[t] = sum over j, in order, of [w[t, j]] rows[position[t, j]].
-template <int T, int U, bool WEIGHTED>
+template <int T, int U, bool WEIGHTED, bool NT>
 __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
     const char* __restrict__ src, const int* __restrict__ position,
     const float* __restrict__ weights, char* __restrict__ out, int tokens, int k, int rows,
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
             for (int u = 0; u < U; ++u)
                 if (ch[u].on) {
                     float y[V];
-                    row_unpack<T>(load16b(r + ch[u].at), y);
+                    row_unpack<T>(load16b<NT>(r + ch[u].at), y);
 #pragma unroll
                     for (int e = 0; e < V; ++e)
                         acc[u][e] = WEIGHTED ? fmaf(w, y[e], acc[u][e]) : acc[u][e] + y[e];
@@ -432,16 +432,19 @@ __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
 
 // dy[position[t, j]] = w[t, j] dout[t]; dw[t, j] = dout[t] . y[position[t, j]].
 // One wave per token; KB is k rounded up, so that the k sums stay in registers.
-// A lane writes a chunk of dy after it has read the same chunk of y, and what
-// the moved-back last chunk shares with its neighbour is left out of the sums,
-// so dy may be y.
-template <int T, int KB>
+// All loads of a step (UC chunks of dout, KB of y for each) are issued before
+// its first store; a dropped slot reads dout's chunk in the place of y's.  A
+// lane writes a chunk of dy after it has read the same chunk of y, and what the
+// moved-back last chunk shares with its neighbour is left out of the sums, so
+// dy may be y.
+template <int T, int KB, bool NT>
 __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
     const char* __restrict__ dout, const char* y, const int* __restrict__ position,
     const float* __restrict__ weights, char* dy, float* __restrict__ dweights, int tokens, int k,
     int rows, int chunks, size_t row_bytes) {
     constexpr int V = row_vec<T>();
     constexpr int S = 16 / V;
+    constexpr int UC = KB >= 4 ? 1 : 4 / KB;
     const int lane = threadIdx.x & (kWave - 1);
     const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
                            __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -453,34 +456,52 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
         float w[KB], dot[KB];
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
-            pos[j] = j < k ? position[slot + j] : -1;
+            const int p = j < k ? position[slot + j] : -1;
+            pos[j] = p < rows ? p : -1;
             w[j] = j < k ? weights[slot + j] : 0.0f;
             dot[j] = 0.0f;
         }
-        for (int c = lane; c < chunks; c += kWave) {
-            const size_t at = row_chunk(c, chunks, row_bytes).at;
-            const int twice = static_cast<int>((static_cast<size_t>(c) * 16 - at) / S);
-            float g[V];
-            row_unpack<T>(load16b(g_row + at), g);
+        for (int c = lane; c < chunks; c += UC * kWave) {
+            size_t at[UC];
+            u32x4 graw[UC], yraw[UC][KB];
 #pragma unroll
-            for (int j = 0; j < KB; ++j) {
-                if (pos[j] < 0 || pos[j] >= rows) continue;
-                const size_t r = static_cast<size_t>(pos[j]) * row_bytes + at;
-                float v[V];
-                row_unpack<T>(load16b(y + r), v);
+            for (int u = 0; u < UC; ++u) {
+                at[u] = row_chunk(min(c + u * kWave, chunks - 1), chunks, row_bytes).at;
+                graw[u] = load16b<NT>(g_row + at[u]);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float term = g[e] * v[e];
-                    dot[j] += e < twice ? 0.0f : term;
-                    v[e] = w[j] * g[e];
+                for (int j = 0; j < KB; ++j) {
+                    const char* r =
+                        pos[j] < 0 ? g_row : y + static_cast<size_t>(pos[j]) * row_bytes;
+                    yraw[u][j] = load16b<NT>(r + at[u]);
                 }
-                store16b(dy + r, row_pack<T>(v));
+            }
+#pragma unroll
+            for (int u = 0; u < UC; ++u) {
+                const bool on = c + u * kWave < chunks;
+                const int first =
+                    on ? static_cast<int>((static_cast<size_t>(c + u * kWave) * 16 - at[u]) / S)
+                       : V;
+                float g[V];
+                row_unpack<T>(graw[u], g);
+#pragma unroll
+                for (int j = 0; j < KB; ++j) {
+                    float v[V];
+                    row_unpack<T>(yraw[u][j], v);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        dot[j] = e < first ? dot[j] : fmaf(g[e], v[e], dot[j]);
+                        v[e] = w[j] * g[e];
+                    }
+                    if (on && pos[j] >= 0)
+                        store16b(dy + static_cast<size_t>(pos[j]) * row_bytes + at[u],
+                                 row_pack<T>(v));
+                }
             }
         }
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
             const float s = wave_sum(dot[j]);
-            if (lane == 0 && j < k) dweights[slot + j] = s;
+            if (lane == 0 && j < k) dweights[slot + j] = pos[j] < 0 ? 0.0f : s;
         }
     }
 }
@@ -577,6 +598,12 @@ int check_rows_args(const char* name, int tokens, int k, int rows, int cols, int
     return MI_OK;
 }
 
+// Bytes of the token rows and of `times` the slots' rows.
+double moved_bytes(int tokens, int k, int rows, size_t row_bytes, int times) {
+    const double slots = std::min(static_cast<double>(tokens) * k, static_cast<double>(rows));
+    return (tokens + times * slots) * static_cast<double>(row_bytes);
+}
+
 template <bool WEIGHTED>
 int gather_sum(const char* name, const void* src, const int* position, const float* weights,
                void* out, int tokens, int k, int rows, int cols, int type, hipStream_t st) {
@@ -589,9 +616,13 @@ int gather_sum(const char* name, const void* src, const int* position, const flo
     const dim3 grid(token_grid(tokens), (chunks + u * kWave - 1) / (u * kWave));
     with_row_type(type, [&](auto t) {
         with_segment(u, [&](auto uu) {
-            hipLaunchKernelGGL((gather_sum_kernel<decltype(t)::value, decltype(uu)::value, WEIGHTED>),
-                               grid, dim3(kThreads), 0, st, static_cast<const char*>(src), position,
-                               weights, static_cast<char*>(out), tokens, k, rows, chunks, row_bytes);
+            with_flag(stream_loads(moved_bytes(tokens, k, rows, row_bytes, 1)), [&](auto nt) {
+                constexpr int T = decltype(t)::value, U = decltype(uu)::value;
+                hipLaunchKernelGGL((gather_sum_kernel<T, U, WEIGHTED, decltype(nt)::value>), grid,
+                                   dim3(kThreads), 0, st, static_cast<const char*>(src), position,
+                                   weights, static_cast<char*>(out), tokens, k, rows, chunks,
+                                   row_bytes);
+            });
         });
     });
     return check_launch(name);
@@ -765,11 +796,13 @@ int mi_moe_combine_backward(const void* dout, const void* y, const int* position
     with_row_type(type, [&](auto t) {
         constexpr int T = decltype(t)::value;
         auto launch = [&](auto kb) {
-            hipLaunchKernelGGL((combine_bwd_kernel<T, decltype(kb)::value>),
-                               dim3(token_grid(tokens)), dim3(kThreads), 0, st,
-                               static_cast<const char*>(dout), static_cast<const char*>(y),
-                               position, weights, static_cast<char*>(dy), dweights, tokens, k,
-                               rows, chunks, row_bytes);
+            with_flag(stream_loads(moved_bytes(tokens, k, rows, row_bytes, 2)), [&](auto nt) {
+                hipLaunchKernelGGL((combine_bwd_kernel<T, decltype(kb)::value, decltype(nt)::value>),
+                                   dim3(token_grid(tokens)), dim3(kThreads), 0, st,
+                                   static_cast<const char*>(dout), static_cast<const char*>(y),
+                                   position, weights, static_cast<char*>(dy), dweights, tokens, k,
+                                   rows, chunks, row_bytes);
+            });
         };
         if (k <= 1)
             launch(std::integral_constant<int, 1>());
