@@ -67,19 +67,6 @@ __device__ __forceinline__ Task workgroup_task(int cols, int tiles, int last_lan
     return t;
 }
 
-// Unaligned accesses of a piece of a row.
-template <class V>
-__device__ __forceinline__ V load_piece(const char* p) {
-    V v;
-    __builtin_memcpy(&v, p, sizeof(V));
-    return v;
-}
-
-template <class V>
-__device__ __forceinline__ void store_piece(char* p, const V& v) {
-    __builtin_memcpy(p, &v, sizeof(V));
-}
-
 // A unit of a row, in the row's type.  The row's last unit may be partial: it
 // is moved as its 4, 2 and 1 elements, whichever its number is made of, and the
 // elements behind it read as 0.

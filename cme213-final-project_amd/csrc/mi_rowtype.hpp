@@ -110,6 +110,47 @@ __device__ __forceinline__ u32x4 row_pack(const float (&v)[row_vec<T>()]) {
     }
 }
 
+// Unaligned accesses of sizeof(V) bytes.
+template <class V>
+__device__ __forceinline__ V load_piece(const char* p) {
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+
+template <class V>
+__device__ __forceinline__ void store_piece(char* p, const V& v) {
+    __builtin_memcpy(p, &v, sizeof(V));
+}
+
+// N consecutive elements, as one access; N a power of two and at most 16 bytes.
+template <int T, int N>
+__device__ __forceinline__ void row_get_n(const void* p, size_t i, float (&v)[N]) {
+    typedef row_elem<T> vec __attribute__((ext_vector_type(N)));
+    const char* at = static_cast<const char*>(p) + i * sizeof(row_elem<T>);
+    if constexpr (N == 1) {
+        v[0] = row_get<T>(p, i);
+    } else {
+        const vec x = load_piece<vec>(at);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = static_cast<float>(x[e]);
+    }
+}
+
+template <int T, int N>
+__device__ __forceinline__ void row_put_n(void* p, size_t i, const float (&v)[N]) {
+    typedef row_elem<T> vec __attribute__((ext_vector_type(N)));
+    char* at = static_cast<char*>(p) + i * sizeof(row_elem<T>);
+    if constexpr (N == 1) {
+        row_put<T>(p, i, v[0]);
+    } else {
+        vec x;
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = static_cast<row_elem<T>>(v[e]);
+        store_piece(at, x);
+    }
+}
+
 inline bool row_type_ok(int type) {
     return type == MI_TYPE_F32 || type == MI_TYPE_F16 || type == MI_TYPE_BF16;
 }

@@ -34,8 +34,12 @@ constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's secon
 // finds the largest key left (registers, then DPP over the lanes), the first
 // lane that holds it and its first element there: the lowest expert of that
 // logit.  The lane group's lane j keeps the key of round j.
+//
+// Bound by the rounds' instructions, not by memory; 16 lanes a row (four rows a
+// wave) share the steps between lanes among four rows.
 // ---------------------------------------------------------------------------
 constexpr int kNoKey = INT_MIN;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ int order_key(float f) {
     if (f != f) return INT_MAX;
@@ -49,15 +53,33 @@ __device__ __forceinline__ float key_value(int key) {
     return __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
 }
 
-template <int T, int L, int P>
+// Each lane's P consecutive logits, -inf behind the last expert.
+template <int T, int P>
 __device__ __forceinline__ void load_logits(const void* logits, size_t row, int gl, int experts,
                                             float (&v)[P]) {
+    constexpr int N = P < row_vec<T>() ? P : row_vec<T>();
     const size_t base = row * experts;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int e = gl * P + p;
-        v[p] = e < experts ? row_get<T>(logits, base + e) : -__builtin_inff();
+    for (int c = 0; c < P; c += N) {
+        const int e0 = gl * P + c;
+        float part[N];
+        if (e0 + N <= experts) {
+            row_get_n<T, N>(logits, base + e0, part);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                part[e] = e0 + e < experts ? row_get<T>(logits, base + e0 + e) : -__builtin_inff();
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[c + e] = part[e];
     }
+}
+
+// Of the lanes in `lanes`, the first of each row's group (each has one).
+template <int L>
+__device__ __forceinline__ bool first_of_group(unsigned long long lanes) {
+    const unsigned long long below = L == 64 ? lanes - 1 : lanes - 0x0001000100010001ull;
+    return __builtin_amdgcn_inverse_ballot_w64(lanes & ~below);
 }
 
 template <int T, int L, int P, bool RENORM>
@@ -66,20 +88,19 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
                                                             float* __restrict__ weights,
                                                             int tokens, int experts, int k) {
     constexpr int PER = kThreads / L;  // rows per workgroup
-    const int lane = threadIdx.x & (kWave - 1);
-    const int gl = lane & (L - 1);
-    for (long long first = static_cast<long long>(blockIdx.x) * PER; first < tokens;
-         first += static_cast<long long>(gridDim.x) * PER) {
-        const long long want = first + threadIdx.x / L;
+    const int gl = threadIdx.x & (L - 1);
+    for (long long base = static_cast<long long>(blockIdx.x) * PER; base < tokens;
+         base += static_cast<long long>(gridDim.x) * PER) {
+        const long long want = base + threadIdx.x / L;
         const bool valid = want < tokens;  // the others repeat the last row and store nothing
         const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
         float v[P];
-        load_logits<T, L, P>(logits, row, gl, experts, v);
+        load_logits<T, P>(logits, row, gl, experts, v);
         int key[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) key[p] = order_key(v[p]);
 
-        const size_t out = row * k;
+        int* out = ids + row * k;
         float top = 0.0f, total = 0.0f;
         int mine = kNoKey;
         for (int j = 0; j < k; ++j) {
@@ -88,45 +109,54 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
             for (int p = 1; p < P; ++p) local = max(local, key[p]);
             const int m = group_max<L>(local);
             if (j == 0) {
-                top = key_value(m);
+                top = m == kNoKey ? 0.0f : key_value(m);
                 if constexpr (!RENORM) {
                     float s = 0.0f;
 #pragma unroll
                     for (int p = 0; p < P; ++p)
-                        s += key[p] == kNoKey ? 0.0f : expf(key_value(key[p]) - top);
+                        s += __builtin_amdgcn_exp2f((v[p] - top) * kLog2e);
                     total = group_sum<L>(s);
                 }
             }
-            const unsigned long long holds = __ballot(local == m) >> (lane & ~(L - 1));
-            const bool winner = __ffsll(holds) - 1 == gl;
+            const bool winner = first_of_group<L>(__ballot(local == m));
             int at = 0;
+            bool found = false;
 #pragma unroll
-            for (int p = P - 1; p >= 0; --p) at = key[p] == m ? p : at;
-            if (winner && valid) ids[out + j] = m == kNoKey ? -1 : gl * P + at;
-#pragma unroll
-            for (int p = 0; p < P; ++p) key[p] = winner && p == at ? kNoKey : key[p];
+            for (int p = 0; p < P; ++p) {
+                const bool here = key[p] == m && !found;
+                found |= here;
+                at = here ? p : at;
+                key[p] = here && winner ? kNoKey : key[p];
+            }
+            if (winner && valid) out[j] = m == kNoKey ? -1 : gl * P + at;
             mine = gl == j ? m : mine;
         }
         const float e = mine == kNoKey ? 0.0f : expf(key_value(mine) - top);
         if constexpr (RENORM) total = group_sum<L>(e);
-        if (valid && gl < k) weights[out + gl] = mine == kNoKey ? 0.0f : e / total;
+        if (valid && gl < k) weights[row * k + gl] = mine == kNoKey ? 0.0f : e / total;
     }
 }
 
 // dl_e = sum over the slots j with id_j = e of w_j (dw_j [- d]) - p_e d, with
 // d = sum_j w_j dw_j; the term in p_e only where the weights are not
-// renormalised, [- d] only where they are.
+// renormalised, [- d] only where they are.  The slots' terms are added into a
+// row of zeros in LDS, slot after slot (a wave's LDS operations run in order),
+// which costs less than comparing every element's number with every slot's.
 template <int T, int L, int P, bool RENORM>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids,
     const float* __restrict__ weights, const float* __restrict__ dweights,
     void* __restrict__ dlogits, int tokens, int experts, int k) {
     constexpr int PER = kThreads / L;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int gl = lane & (L - 1);
-    for (long long first = static_cast<long long>(blockIdx.x) * PER; first < tokens;
-         first += static_cast<long long>(gridDim.x) * PER) {
-        const long long want = first + threadIdx.x / L;
+    constexpr int N = P < row_vec<T>() ? P : row_vec<T>();
+    __shared__ __align__(16) float terms[PER][L * P];
+    const int gl = threadIdx.x & (L - 1);
+    float* own = terms[threadIdx.x / L];
+#pragma unroll
+    for (int p = 0; p < P; ++p) own[gl * P + p] = 0.0f;
+    for (long long base = static_cast<long long>(blockIdx.x) * PER; base < tokens;
+         base += static_cast<long long>(gridDim.x) * PER) {
+        const long long want = base + threadIdx.x / L;
         const bool valid = want < tokens;
         const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
 
@@ -137,16 +167,16 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
             w = weights[row * k + gl];
             dw = dweights[row * k + gl];
         }
-        const float wd = id >= 0 ? w * dw : 0.0f;
-        const float d = group_sum<L>(wd);
-        const float term = RENORM ? (id >= 0 ? w * (dw - d) : 0.0f) : wd;
-
         float v[P];
-        if constexpr (RENORM) {
-#pragma unroll
-            for (int p = 0; p < P; ++p) v[p] = 0.0f;
-        } else {
-            load_logits<T, L, P>(logits, row, gl, experts, v);
+        if constexpr (!RENORM) load_logits<T, P>(logits, row, gl, experts, v);
+        const bool live = id >= 0 && id < experts;
+        const float wd = live ? w * dw : 0.0f;
+        const float d = group_sum<L>(wd);
+        const float term = RENORM ? w * (dw - d) : wd;
+        wave_order();
+        for (int j = 0; j < k; ++j)
+            if (gl == j && live) atomicAdd(&own[id], term);
+        if constexpr (!RENORM) {
             float top = v[0];
 #pragma unroll
             for (int p = 1; p < P; ++p) top = fmaxf(top, v[p]);
@@ -155,7 +185,7 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
             float s = 0.0f;
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                v[p] = v[p] == -__builtin_inff() ? 0.0f : expf(v[p] - top);
+                v[p] = __builtin_amdgcn_exp2f((v[p] - top) * kLog2e);
                 s += v[p];
             }
             s = group_sum<L>(s);
@@ -163,16 +193,28 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
 #pragma unroll
             for (int p = 0; p < P; ++p) v[p] *= scale;
         }
-        for (int j = 0; j < k; ++j) {
-            const int idj = __shfl(id, j, L);
-            const float tj = __shfl(term, j, L);
+        wave_order();
 #pragma unroll
-            for (int p = 0; p < P; ++p) v[p] += idj == gl * P + p ? tj : 0.0f;
+        for (int p = 0; p < P; ++p) {
+            const float t = own[gl * P + p];
+            v[p] = RENORM ? t : v[p] + t;
         }
-        if (!valid) continue;
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-            if (gl * P + p < experts) row_put<T>(dlogits, row * experts + gl * P + p, v[p]);
+        for (int p = 0; p < P; ++p) own[gl * P + p] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < P; c += N) {
+            const int e0 = gl * P + c;
+            float part[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) part[e] = v[c + e];
+            if (valid && e0 + N <= experts) {
+                row_put_n<T, N>(dlogits, row * experts + e0, part);
+            } else if (valid) {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e0 + e < experts) row_put<T>(dlogits, row * experts + e0 + e, part[e]);
+            }
+        }
     }
 }
 
@@ -209,40 +251,50 @@ unsigned gate_grid(int tokens, int lanes) {
 // one ballot per bit of the id, a slot's rank among them is the number of such
 // lanes before it, and the first of them advances the wave's count of that
 // expert.  Counts are whole numbers, so the result does not depend on timing.
+//
+// Latency-bound: a handful of memory and LDS round trips one after the other.
+// One chunk is one launch; more take a first launch that counts each chunk's
+// experts.  Slots a lane in a sort of several chunks, both launches: 262144 slots
+// of 256 experts one 17.0 us, two 12.5, four 12.0; 32768 of 64 6.9, 7.2, 8.8;
+// 65536 of 8 6.2, 6.7, 8.6.
 // ---------------------------------------------------------------------------
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr int kSortChunk = 4096;     // slots per workgroup, at least
+constexpr int kSortOneTrips = 4;  // slots of a lane in a sort of one chunk, at most
+constexpr int kSortTrips = 2;     // slots of a lane in one of several, at least
 constexpr int kSortMaxChunks = 256;
 
 struct SortPlan {
-    int chunk;   // slots per workgroup, a multiple of kSortThreads
+    int trips;   // slots of a lane
     int chunks;
+    long long chunk() const { return static_cast<long long>(trips) * kSortThreads; }
 };
 
 SortPlan plan_sort(int slots) {
-    long long chunk = (static_cast<long long>(slots) + kSortMaxChunks - 1) / kSortMaxChunks;
-    chunk = (chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
-    if (chunk < kSortChunk) chunk = kSortChunk;
-    return {static_cast<int>(chunk),
-            static_cast<int>((static_cast<long long>(slots) + chunk - 1) / chunk)};
+    auto parts = [&](long long of) {
+        return static_cast<int>((static_cast<long long>(slots) + of - 1) / of);
+    };
+    SortPlan p;
+    p.trips = std::max(1, parts(kSortThreads));
+    if (p.trips > kSortOneTrips)
+        p.trips = std::max(kSortTrips, parts(static_cast<long long>(kSortMaxChunks) * kSortThreads));
+    p.chunks = std::max(1, parts(p.chunk()));
+    return p;
 }
 
 // hist[c][e]: slots of expert e in chunk c.
 __global__ __launch_bounds__(kSortThreads) void sort_hist_kernel(const int* __restrict__ ids,
                                                                  int* __restrict__ hist,
                                                                  int slots, int experts,
-                                                                 int chunk) {
+                                                                 int trips) {
     extern __shared__ int count[];
     for (int e = threadIdx.x; e < experts; e += kSortThreads) count[e] = 0;
     __syncthreads();
-    const long long begin = static_cast<long long>(blockIdx.x) * chunk;
-    for (int i = threadIdx.x; i < chunk; i += kSortThreads) {
-        const long long s = begin + i;
-        if (s < slots) {
-            const int id = ids[s];
-            if (id >= 0 && id < experts) atomicAdd(&count[id], 1);
-        }
+    const long long begin = static_cast<long long>(blockIdx.x) * trips * kSortThreads;
+    for (int i = 0; i < trips; ++i) {
+        const long long s = begin + i * kSortThreads + threadIdx.x;
+        const int id = s < slots ? ids[s] : -1;
+        if (id >= 0 && id < experts) atomicAdd(&count[id], 1);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += kSortThreads)
@@ -260,43 +312,75 @@ __device__ __forceinline__ unsigned long long same_id(int id, bool has, int bits
     return m;
 }
 
-// hist == nullptr: there is one chunk.
+// hist == nullptr: there is one chunk.  NR: the lane's ids, up to NR of them,
+// stay in registers from the counting to the placing (0: they are read again).
+template <int NR>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(
     const int* __restrict__ ids, const int* __restrict__ hist, int* __restrict__ offsets,
-    int* __restrict__ order, int* __restrict__ position, int slots, int experts, int chunk,
+    int* __restrict__ order, int* __restrict__ position, int slots, int experts, int trips,
     int chunks, int bits) {
-    extern __shared__ int lds[];
-    int* count = lds;                          // [kSortWaves][experts]
+    extern __shared__ int count[];  // [kSortWaves][experts], then [2][experts] of the chunks
     __shared__ int wave_total[kSortWaves];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = threadIdx.x / kWave;
-    for (int i = threadIdx.x; i < kSortWaves * experts; i += kSortThreads) count[i] = 0;
-    __syncthreads();
-
-    const int part = chunk / kSortWaves;  // a multiple of 64
-    const long long begin = static_cast<long long>(blockIdx.x) * chunk +
-                            static_cast<long long>(wave) * part;
-    int* mine = count + wave * experts;
-    for (int i = 0; i < part; i += kWave) {
-        const long long s = begin + i + lane;
+    const long long begin =
+        static_cast<long long>(blockIdx.x) * trips * kSortThreads +
+        static_cast<long long>(wave) * trips * kWave + lane;
+    auto slot_id = [&](int i) {
+        const long long s = begin + i * kWave;
         const int id = s < slots ? ids[s] : -1;
-        if (id >= 0 && id < experts) atomicAdd(&mine[id], 1);
-    }
-    __syncthreads();
+        return id < experts ? id : -1;
+    };
+    int held[NR ? NR : 1];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) held[i] = i < trips ? slot_id(i) : -1;
 
-    // Thread e owns expert e (experts <= kSortThreads): its slots in this
-    // chunk by wave, in the chunks before and in all of them.
-    const int e = threadIdx.x;
-    int total = 0, before = 0;
-    if (e < experts) {
-        if (hist == nullptr) {
-            for (int w = 0; w < kSortWaves; ++w) total += count[w * experts + e];
-        } else {
-            for (int c = 0; c < chunks; ++c) {
-                const int h = hist[static_cast<size_t>(c) * experts + e];
+    int* totals = count + kSortWaves * experts;  // slots of each expert in all chunks
+    int* befores = totals + experts;             // and in the chunks before this one
+    const int cells = (kSortWaves + (hist == nullptr ? 0 : 2)) * experts;
+    for (int i = threadIdx.x; i < cells; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+    int* mine = count + wave * experts;
+    if constexpr (NR > 0) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (held[i] >= 0) atomicAdd(&mine[held[i]], 1);
+    } else {
+        for (int i = 0; i < trips; ++i) {
+            const int id = slot_id(i);
+            if (id >= 0) atomicAdd(&mine[id], 1);
+        }
+    }
+    if (hist != nullptr) {
+        // as many threads an expert as there are, each some of the chunks
+        const int per = kSortThreads / experts;
+        const int part = threadIdx.x / experts, x = threadIdx.x % experts;
+        if (part < per) {
+            int total = 0, before = 0;
+#pragma unroll 4
+            for (int c = part; c < chunks; c += per) {
+                const int h = hist[static_cast<size_t>(c) * experts + x];
                 before += c < static_cast<int>(blockIdx.x) ? h : 0;
                 total += h;
             }
+            atomicAdd(&totals[x], total);
+            atomicAdd(&befores[x], before);
+        }
+    }
+    __syncthreads();
+
+    // Thread e owns expert e (experts <= kSortThreads).
+    const int e = threadIdx.x;
+    int n[kSortWaves], total = 0, before = 0;
+    if (e < experts) {
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) n[w] = count[w * experts + e];
+        if (hist != nullptr) {
+            total = totals[e];
+            before = befores[e];
+        } else {
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) total += n[w];
         }
     }
     // exclusive sum of the totals over the experts
@@ -307,26 +391,25 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(
     }
     if (lane == kWave - 1) wave_total[wave] = incl;
     __syncthreads();
-    int first = incl - total;
-    for (int w = 0; w < wave; ++w) first += wave_total[w];
     if (e < experts) {
+        int first = incl - total;
+        for (int w = 0; w < wave; ++w) first += wave_total[w];
         if (blockIdx.x == 0) {
             offsets[e] = first;
             if (e == experts - 1) offsets[experts] = first + total;
         }
         int at = first + before;
+#pragma unroll
         for (int w = 0; w < kSortWaves; ++w) {
-            const int n = count[w * experts + e];
             count[w * experts + e] = at;
-            at += n;
+            at += n[w];
         }
     }
     __syncthreads();
 
-    for (int i = 0; i < part; i += kWave) {
-        const long long s = begin + i + lane;
-        const int id = s < slots ? ids[s] : -1;
-        const bool has = id >= 0 && id < experts;
+    auto place = [&](int i, int id) {
+        const long long s = begin + i * kWave;
+        const bool has = id >= 0;
         const unsigned long long same = same_id(id, has, bits);
         const int rank = __popcll(same & ((1ull << lane) - 1));
         const int at = has ? mine[id] : 0;
@@ -335,6 +418,13 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(
         wave_order();
         if (s < slots) position[s] = has ? at + rank : -1;
         if (has && order != nullptr) order[at + rank] = static_cast<int>(s);
+    };
+    if constexpr (NR > 0) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (i < trips) place(i, held[i]);
+    } else {
+        for (int i = 0; i < trips; ++i) place(i, slot_id(i));
     }
 }
 
@@ -715,23 +805,34 @@ int mi_moe_sort(const int* ids, int* offsets, int* order, int* position, int slo
     if (!offsets || (slots > 0 && (!ids || !position)))
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     hipStream_t st = to_stream(stream);
-    SortPlan p = plan_sort(slots);
-    if (p.chunks < 1) p.chunks = 1;  // no slots: the offsets are written all the same
+    const SortPlan p = plan_sort(slots);
     int* hist = nullptr;
     if (p.chunks > 1) {
         int err = MI_OK;
-        char* ws = static_cast<char*>(workspace_get(mi_moe_sort_workspace(slots, experts), st, &err));
+        char* ws =
+            static_cast<char*>(workspace_get(mi_moe_sort_workspace(slots, experts), st, &err));
         if (!ws) return err;
         hist = reinterpret_cast<int*>(ws + colsum_part_offset());
         hipLaunchKernelGGL(sort_hist_kernel, dim3(p.chunks), dim3(kSortThreads),
-                           experts * sizeof(int), st, ids, hist, slots, experts, p.chunk);
+                           experts * sizeof(int), st, ids, hist, slots, experts, p.trips);
         if (int rc = check_launch(name)) return rc;
     }
     int bits = 0;
     while ((1 << bits) < experts) ++bits;
-    hipLaunchKernelGGL(sort_place_kernel, dim3(p.chunks), dim3(kSortThreads),
-                       kSortWaves * experts * sizeof(int), st, ids, hist, offsets, order, position,
-                       slots, experts, p.chunk, p.chunks, bits);
+    const size_t lds = (kSortWaves + (hist ? 2 : 0)) * experts * sizeof(int);
+    auto place = [&](auto nr) {
+        hipLaunchKernelGGL((sort_place_kernel<decltype(nr)::value>), dim3(p.chunks),
+                           dim3(kSortThreads), lds, st, ids, hist, offsets, order, position, slots,
+                           experts, p.trips, p.chunks, bits);
+    };
+    if (p.trips == 1)
+        place(std::integral_constant<int, 1>());
+    else if (p.trips == 2)
+        place(std::integral_constant<int, 2>());
+    else if (p.trips <= 4)
+        place(std::integral_constant<int, 4>());
+    else
+        place(std::integral_constant<int, 0>());
     return check_launch(name);
 }
 
