@@ -234,7 +234,8 @@ __device__ __forceinline__ void decode(const u32x2& q, int scale, const float (&
         float x[4];
         if constexpr (FMT == MI_CKPT8_INT8) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
+            for (int e = 0; e < 4; ++e)
+                x[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
         } else {
             x[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
             x[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);

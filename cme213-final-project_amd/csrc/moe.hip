@@ -277,7 +277,8 @@ SortPlan plan_sort(int slots) {
     SortPlan p;
     p.trips = std::max(1, parts(kSortThreads));
     if (p.trips > kSortOneTrips)
-        p.trips = std::max(kSortTrips, parts(static_cast<long long>(kSortMaxChunks) * kSortThreads));
+        p.trips =
+            std::max(kSortTrips, parts(static_cast<long long>(kSortMaxChunks) * kSortThreads));
     p.chunks = std::max(1, parts(p.chunk()));
     return p;
 }
@@ -431,9 +432,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(
 // ---------------------------------------------------------------------------
 // Rows moved between token order and expert order.  A wave takes one token
 // and a segment of U * 64 16-byte chunks of its row, so the token's positions
-// are wave-uniform.  Where the row is no multiple of 16 bytes the last chunk
-// is moved back to end with the row: the elements that it shares with the one
-// before are computed twice, with the same result.
+// are wave-uniform; of rows of at most 16 or 32 chunks it takes as many tokens as
+// fit, LT = 16 or 32 lanes each.  Where the row is no multiple of 16 bytes the
+// last chunk is moved back to end with the row: the elements that it shares with
+// the one before are computed twice, with the same result.
+//
+// Memory-bound: 5.3 to 6.1 TB/s on tensors past the last-level cache.
 // ---------------------------------------------------------------------------
 struct Chunk {
     bool on;
@@ -445,21 +449,32 @@ __device__ __forceinline__ Chunk row_chunk(int c, int chunks, size_t row_bytes) 
     return {c < chunks, at < row_bytes - 16 ? at : row_bytes - 16};
 }
 
-template <int U>
+// The first token of this lane, and the tokens of a workgroup.
+template <int LT>
+constexpr int workgroup_tokens() {
+    return kThreads / LT;
+}
+
+template <int LT>
+__device__ __forceinline__ long long first_token() {
+    const int in = LT == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / LT)
+                               : static_cast<int>(threadIdx.x / LT);
+    return static_cast<long long>(blockIdx.x) * workgroup_tokens<LT>() + in;
+}
+
+template <int U, int LT>
 __global__ __launch_bounds__(kThreads) void scatter_rows_kernel(
     const char* __restrict__ x, const int* __restrict__ position, char* __restrict__ out,
     int tokens, int k, int rows, int chunks, size_t row_bytes) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
-                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (long long token = wave; token < tokens;
-         token += static_cast<long long>(gridDim.x) * kWaves) {
+    const int lane = threadIdx.x & (LT - 1);
+    for (long long token = first_token<LT>(); token < tokens;
+         token += static_cast<long long>(gridDim.x) * workgroup_tokens<LT>()) {
         const char* src = x + static_cast<size_t>(token) * row_bytes;
         u32x4 v[U];
         Chunk ch[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * kWave + u * kWave + lane, chunks,
+            ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * LT + u * LT + lane, chunks,
                               row_bytes);
             if (ch[u].on) v[u] = load16b<false>(src + ch[u].at);
         }
@@ -476,22 +491,20 @@ __global__ __launch_bounds__(kThreads) void scatter_rows_kernel(
 }
 
 // out[t] = sum over j, in order, of [w[t, j]] rows[position[t, j]].
-template <int T, int U, bool WEIGHTED, bool NT>
+template <int T, int U, int LT, bool WEIGHTED, bool NT>
 __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
     const char* __restrict__ src, const int* __restrict__ position,
     const float* __restrict__ weights, char* __restrict__ out, int tokens, int k, int rows,
     int chunks, size_t row_bytes) {
     constexpr int V = row_vec<T>();
-    const int lane = threadIdx.x & (kWave - 1);
-    const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
-                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (long long token = wave; token < tokens;
-         token += static_cast<long long>(gridDim.x) * kWaves) {
+    const int lane = threadIdx.x & (LT - 1);
+    for (long long token = first_token<LT>(); token < tokens;
+         token += static_cast<long long>(gridDim.x) * workgroup_tokens<LT>()) {
         Chunk ch[U];
         float acc[U][V];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * kWave + u * kWave + lane, chunks,
+            ch[u] = row_chunk(static_cast<int>(blockIdx.y) * U * LT + u * LT + lane, chunks,
                               row_bytes);
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[u][e] = 0.0f;
@@ -521,25 +534,29 @@ __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
 }
 
 // dy[position[t, j]] = w[t, j] dout[t]; dw[t, j] = dout[t] . y[position[t, j]].
-// One wave per token; KB is k rounded up, so that the k sums stay in registers.
-// All loads of a step (UC chunks of dout, KB of y for each) are issued before
-// its first store; a dropped slot reads dout's chunk in the place of y's.  A
-// lane writes a chunk of dy after it has read the same chunk of y, and what the
-// moved-back last chunk shares with its neighbour is left out of the sums, so
-// dy may be y.
-template <int T, int KB, bool NT>
-__global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
+// G waves, or LT lanes of one, per token; KB is k rounded up, so that the k sums
+// stay in registers.  All loads of a step (UC chunks of dout, KB of y for each)
+// are issued before its first store; a dropped slot reads dout's chunk in the
+// place of y's, and what the moved-back last chunk shares with its neighbour is
+// left out of its sums.  dy may be y: a chunk of dy is written after the same chunk
+// of y was read, by the same lane; a moved-back chunk also writes into its
+// neighbour's, so the two must not lie in different waves (see combine_waves): in
+// one wave, its loads of both come before its stores of the later one.
+template <int T, int KB, int G, int LT, bool NT>
+__global__ __launch_bounds__(G > kWaves ? G * kWave : kThreads) void combine_bwd_kernel(
     const char* __restrict__ dout, const char* y, const int* __restrict__ position,
     const float* __restrict__ weights, char* dy, float* __restrict__ dweights, int tokens, int k,
     int rows, int chunks, size_t row_bytes) {
     constexpr int V = row_vec<T>();
     constexpr int S = 16 / V;
     constexpr int UC = KB >= 4 ? 1 : 4 / KB;
-    const int lane = threadIdx.x & (kWave - 1);
-    const long long wave = static_cast<long long>(blockIdx.x) * kWaves +
-                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (long long token = wave; token < tokens;
-         token += static_cast<long long>(gridDim.x) * kWaves) {
+    static_assert(G == 1 || (G >= kWaves && LT == kWave), "several waves: one token a workgroup");
+    constexpr int TOKENS = G > 1 ? 1 : workgroup_tokens<LT>();
+    __shared__ float sums[G][KB];  // used where G > 1
+    const int lane = threadIdx.x & (LT - 1);
+    const int part = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : 0;
+    for (long long token = G > 1 ? static_cast<long long>(blockIdx.x) : first_token<LT>();
+         token < tokens; token += static_cast<long long>(gridDim.x) * TOKENS) {
         const size_t slot = static_cast<size_t>(token) * k;
         const char* g_row = dout + static_cast<size_t>(token) * row_bytes;
         int pos[KB];
@@ -551,12 +568,12 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
             w[j] = j < k ? weights[slot + j] : 0.0f;
             dot[j] = 0.0f;
         }
-        for (int c = lane; c < chunks; c += UC * kWave) {
+        for (int c = part * LT + lane; c < chunks; c += UC * G * LT) {
             size_t at[UC];
             u32x4 graw[UC], yraw[UC][KB];
 #pragma unroll
             for (int u = 0; u < UC; ++u) {
-                at[u] = row_chunk(min(c + u * kWave, chunks - 1), chunks, row_bytes).at;
+                at[u] = row_chunk(min(c + u * G * LT, chunks - 1), chunks, row_bytes).at;
                 graw[u] = load16b<NT>(g_row + at[u]);
 #pragma unroll
                 for (int j = 0; j < KB; ++j) {
@@ -567,9 +584,9 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
             }
 #pragma unroll
             for (int u = 0; u < UC; ++u) {
-                const bool on = c + u * kWave < chunks;
+                const bool on = c + u * G * LT < chunks;
                 const int first =
-                    on ? static_cast<int>((static_cast<size_t>(c + u * kWave) * 16 - at[u]) / S)
+                    on ? static_cast<int>((static_cast<size_t>(c + u * G * LT) * 16 - at[u]) / S)
                        : V;
                 float g[V];
                 row_unpack<T>(graw[u], g);
@@ -590,8 +607,26 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(
         }
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
-            const float s = wave_sum(dot[j]);
-            if (lane == 0 && j < k) dweights[slot + j] = pos[j] < 0 ? 0.0f : s;
+            float s = group_sum<LT == 32 ? 16 : LT>(dot[j]);
+            if constexpr (LT == 32) s += __shfl_xor(s, 16);
+            if constexpr (G > 1) {
+                if (lane == 0) sums[part][j] = s;
+            } else if (lane == 0 && j < k) {
+                dweights[slot + j] = pos[j] < 0 ? 0.0f : s;
+            }
+        }
+        if constexpr (G > 1) {
+            // one token a workgroup: its waves are here together
+            __syncthreads();
+            if (static_cast<int>(threadIdx.x) < k) {
+                const int j = threadIdx.x;
+                const int p = position[slot + j];
+                float s = sums[0][j];
+#pragma unroll
+                for (int g = 1; g < G; ++g) s += sums[g][j];
+                dweights[slot + j] = p >= 0 && p < rows ? s : 0.0f;
+            }
+            __syncthreads();
         }
     }
 }
@@ -643,7 +678,8 @@ template <Narrow OP>
 int launch_narrow(const char* name, const void* a, const void* y, const int* position,
                   const float* weights, void* out, float* dweights, int tokens, int k, int rows,
                   int cols, int type, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>((static_cast<long long>(tokens) + kThreads - 1) / kThreads));
+    const dim3 grid(
+        static_cast<unsigned>((static_cast<long long>(tokens) + kThreads - 1) / kThreads));
     with_row_type(type, [&](auto t) {
         hipLaunchKernelGGL((narrow_kernel<decltype(t)::value, OP>), grid, dim3(kThreads), 0, st, a,
                            y, position, weights, out, dweights, tokens, k, rows, cols);
@@ -651,27 +687,53 @@ int launch_narrow(const char* name, const void* a, const void* y, const int* pos
     return check_launch(name);
 }
 
-unsigned token_grid(int tokens) {
-    return static_cast<unsigned>(
-        std::min<long long>((static_cast<long long>(tokens) + kWaves - 1) / kWaves, kMaxGrid));
+unsigned token_grid(int tokens, int per_workgroup) {
+    return static_cast<unsigned>(std::min<long long>(
+        (static_cast<long long>(tokens) + per_workgroup - 1) / per_workgroup, kMaxGrid));
 }
 
-// Chunks per lane: as many as keep a few thousand waves in flight.
-int segment_chunks(int tokens, int chunks) {
-    const long long one = static_cast<long long>(tokens) * ((chunks + kWave - 1) / kWave);
-    if (one >= 8192 && chunks > 2 * kWave) return 4;
-    if (one >= 4096 && chunks > kWave) return 2;
-    return 1;
-}
+// Lanes of a token, and its chunks a lane has in hand.
+struct RowShape {
+    int lanes, u;
+};
 
+// f(lanes, u) and the launch's grid for rows of `chunks` chunks.
 template <class F>
-void with_segment(int u, F f) {
-    if (u == 4)
-        f(std::integral_constant<int, 4>());
-    else if (u == 2)
-        f(std::integral_constant<int, 2>());
+void with_row_shape(RowShape shape, int tokens, int chunks, F f) {
+    using std::integral_constant;
+    const dim3 grid(token_grid(tokens, kThreads / shape.lanes),
+                    (chunks + shape.u * shape.lanes - 1) / (shape.u * shape.lanes));
+    if (shape.lanes == 16)
+        f(integral_constant<int, 16>(), integral_constant<int, 1>(), grid);
+    else if (shape.lanes == 32)
+        f(integral_constant<int, 32>(), integral_constant<int, 1>(), grid);
+    else if (shape.u == 1)
+        f(integral_constant<int, 64>(), integral_constant<int, 1>(), grid);
+    else if (shape.u == 2)
+        f(integral_constant<int, 64>(), integral_constant<int, 2>(), grid);
     else
-        f(std::integral_constant<int, 1>());
+        f(integral_constant<int, 64>(), integral_constant<int, 4>(), grid);
+}
+
+int row_lanes(int chunks) { return chunks <= 16 ? 16 : chunks <= 32 ? 32 : 64; }
+
+// Segments of the copies' rows: short ones while there are few waves.
+RowShape scatter_shape(int tokens, int chunks) {
+    const long long waves = static_cast<long long>(tokens) * ((chunks + kWave - 1) / kWave);
+    if (waves >= 8192 && chunks > 2 * kWave) return {64, 4};
+    if (waves >= 4096 && chunks > kWave) return {64, 2};
+    return {row_lanes(chunks), 1};
+}
+
+// Of the sums' rows, where each lane has a load for every choice besides: bf16
+// [1024 tokens, 4 choices] of 4096 columns in segments of one, two, four chunks a lane
+// 6.9, 7.1, 8.9 us, [4096, 8] of 2048 33.7, 24.9, 28.8, fp32 [8192, 6] of 1600 72.3, 67.7,
+// 62.1.
+RowShape gather_shape(int tokens, int chunks) {
+    const long long waves = static_cast<long long>(tokens) * ((chunks + kWave - 1) / kWave);
+    if (waves >= 32768 && chunks > 2 * kWave) return {64, 4};
+    if (waves >= 4096 && chunks > kWave) return {64, 2};
+    return {row_lanes(chunks), 1};
 }
 
 int check_rows_args(const char* name, int tokens, int k, int rows, int cols, int type) {
@@ -702,20 +764,34 @@ int gather_sum(const char* name, const void* src, const int* position, const flo
         return launch_narrow<WEIGHTED ? Narrow::WeightedSum : Narrow::Sum>(
             name, src, nullptr, position, weights, out, nullptr, tokens, k, rows, cols, type, st);
     const int chunks = static_cast<int>((row_bytes + 15) / 16);
-    const int u = segment_chunks(tokens, chunks);
-    const dim3 grid(token_grid(tokens), (chunks + u * kWave - 1) / (u * kWave));
+    const bool stream = stream_loads(moved_bytes(tokens, k, rows, row_bytes, 1));
     with_row_type(type, [&](auto t) {
-        with_segment(u, [&](auto uu) {
-            with_flag(stream_loads(moved_bytes(tokens, k, rows, row_bytes, 1)), [&](auto nt) {
-                constexpr int T = decltype(t)::value, U = decltype(uu)::value;
-                hipLaunchKernelGGL((gather_sum_kernel<T, U, WEIGHTED, decltype(nt)::value>), grid,
-                                   dim3(kThreads), 0, st, static_cast<const char*>(src), position,
-                                   weights, static_cast<char*>(out), tokens, k, rows, chunks,
-                                   row_bytes);
+        with_row_shape(gather_shape(tokens, chunks), tokens, chunks,
+                       [&](auto lanes, auto u, dim3 grid) {
+            constexpr int T = decltype(t)::value, LT = decltype(lanes)::value;
+            constexpr int U = decltype(u)::value;
+            with_flag(stream, [&](auto nt) {
+                hipLaunchKernelGGL((gather_sum_kernel<T, U, LT, WEIGHTED, decltype(nt)::value>),
+                                   grid, dim3(kThreads), 0, st, static_cast<const char*>(src),
+                                   position, weights, static_cast<char*>(out), tokens, k, rows,
+                                   chunks, row_bytes);
             });
         });
     });
     return check_launch(name);
+}
+
+// Waves a token in combine's gradient: one where a wave has the row in few
+// steps, more where rows are long (bf16 [8192 tokens, 4 choices] of 2048 columns 63.4
+// -> 54.4 us, of 4096 125 -> 110; 1600 columns 21.6 -> 22.3, 16384 tokens of 1024 28.8
+// -> 40.7) or tokens few (8 tokens of 6152 fp32 32.2 us by one, 11.4 by four, 6.5 by
+// 16; 67 of 896, 8 choices, 8.9 -> 4.8).  Past 8 choices 16 waves lack registers.
+// In place, a moved-back last chunk that would fall to another wave than its
+// neighbour takes one wave.
+int combine_waves(int tokens, int k, int chunks, bool in_place, bool ragged) {
+    if (in_place && ragged && (chunks - 1) % kWave == 0) return 1;
+    if (tokens < 512 && chunks > 4 * kWave && k <= 8) return 16;
+    return chunks >= 4 * kWave || (tokens < 512 && chunks > kWave) ? 4 : 1;
 }
 
 int check_gate_args(const char* name, int tokens, int experts, int k, int type) {
@@ -848,12 +924,11 @@ int mi_moe_dispatch_forward(const void* x, const int* position, void* out, int t
         return launch_narrow<Narrow::Scatter>(name, x, nullptr, position, nullptr, out, nullptr,
                                               tokens, k, rows, cols, type, st);
     const int chunks = static_cast<int>((row_bytes + 15) / 16);
-    const int u = segment_chunks(tokens, chunks);
-    const dim3 grid(token_grid(tokens), (chunks + u * kWave - 1) / (u * kWave));
-    with_segment(u, [&](auto uu) {
-        hipLaunchKernelGGL((scatter_rows_kernel<decltype(uu)::value>), grid, dim3(kThreads), 0, st,
-                           static_cast<const char*>(x), position, static_cast<char*>(out), tokens,
-                           k, rows, chunks, row_bytes);
+    with_row_shape(scatter_shape(tokens, chunks), tokens, chunks,
+                   [&](auto lanes, auto u, dim3 grid) {
+        hipLaunchKernelGGL((scatter_rows_kernel<decltype(u)::value, decltype(lanes)::value>), grid,
+                           dim3(kThreads), 0, st, static_cast<const char*>(x), position,
+                           static_cast<char*>(out), tokens, k, rows, chunks, row_bytes);
     });
     return check_launch(name);
 }
@@ -897,13 +972,37 @@ int mi_moe_combine_backward(const void* dout, const void* y, const int* position
     with_row_type(type, [&](auto t) {
         constexpr int T = decltype(t)::value;
         auto launch = [&](auto kb) {
-            with_flag(stream_loads(moved_bytes(tokens, k, rows, row_bytes, 2)), [&](auto nt) {
-                hipLaunchKernelGGL((combine_bwd_kernel<T, decltype(kb)::value, decltype(nt)::value>),
-                                   dim3(token_grid(tokens)), dim3(kThreads), 0, st,
+            constexpr int KB = decltype(kb)::value;
+            auto with_waves = [&](auto g, auto lanes, auto nt) {
+                constexpr int G = decltype(g)::value, LT = decltype(lanes)::value;
+                const dim3 grid(token_grid(tokens, G > 1 ? 1 : kThreads / LT));
+                hipLaunchKernelGGL((combine_bwd_kernel<T, KB, G, LT, decltype(nt)::value>), grid,
+                                   dim3(G > kWaves ? G * kWave : kThreads), 0, st,
                                    static_cast<const char*>(dout), static_cast<const char*>(y),
                                    position, weights, static_cast<char*>(dy), dweights, tokens, k,
                                    rows, chunks, row_bytes);
-            });
+            };
+            using std::integral_constant;
+            const int g = combine_waves(tokens, k, chunks, dy == y, row_bytes % 16 != 0);
+            const bool stream = stream_loads(moved_bytes(tokens, k, rows, row_bytes, 2));
+            if constexpr (KB <= 8)
+                if (g == 16)
+                    return with_waves(integral_constant<int, 16>(), integral_constant<int, 64>(),
+                                      std::false_type());
+            if (g == 4)
+                with_flag(stream, [&](auto nt) {
+                    with_waves(integral_constant<int, 4>(), integral_constant<int, 64>(), nt);
+                });
+            else if (row_lanes(chunks) == 16)
+                with_waves(integral_constant<int, 1>(), integral_constant<int, 16>(),
+                           std::false_type());
+            else if (row_lanes(chunks) == 32)
+                with_waves(integral_constant<int, 1>(), integral_constant<int, 32>(),
+                           std::false_type());
+            else
+                with_flag(stream, [&](auto nt) {
+                    with_waves(integral_constant<int, 1>(), integral_constant<int, 64>(), nt);
+                });
         };
         if (k <= 1)
             launch(std::integral_constant<int, 1>());
