@@ -369,13 +369,14 @@ __global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
 // gelu(u); the column sums of grad_in over the band's rows of group g, added
 // over the row lanes in order, go to partial row band + g.  Going down the
 // rows, band and g only grow, and one of them does with every new pair, so no
-// two pairs share a partial row.  grad_in may be grad_out.
+// two pairs share a partial row.  With part == nullptr there is one band, and its
+// sums are added to dbias at once.  grad_in may be grad_out.
 template <int T, int FMT, bool ACT, bool NT>
 __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
     const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales,
     const float* __restrict__ bias, const int* __restrict__ offsets, const char* grad_out,
-    char* grad_in, char* __restrict__ act, float* __restrict__ part, int rows, int cols,
-    int groups, int band, int tiles, int last_lanes) {
+    char* grad_in, char* __restrict__ act, float* __restrict__ part, float* __restrict__ dbias,
+    int rows, int cols, int groups, int band, int tiles, int last_lanes) {
     constexpr int U = kRowsInHand;
     __shared__ float red[kThreads * kUnit];
     const Task t = workgroup_task(cols, tiles, last_lanes);
@@ -436,7 +437,11 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
             float sum = red[c];
             for (int l = 1; l < t.row_lanes; ++l) sum += red[l * width + c];
             const int col = t.tile * kTile + c;
-            if (col < cols) part[static_cast<size_t>(t.band + g) * cols + col] = sum;
+            if (col >= cols) continue;
+            if (part == nullptr)
+                dbias[static_cast<size_t>(g) * cols + col] += sum;
+            else
+                part[static_cast<size_t>(t.band + g) * cols + col] = sum;
         }
         __syncthreads();
     });
@@ -524,8 +529,11 @@ Plan plan_forward(int rows, int cols) { return plan_ckpt8(rows, cols, 4096, 2, 4
 // Backward: every band leaves a partial row to write and add up, so bands are
 // longer: [4096, 1024] bf16 in 2048 workgroups of one row a lane 13.8 + 5.9 us (the
 // sums), in 512 of four 8.8 + 3.9.  Too few workgroups starve the memory: [16384,
-// 6400] bf16 in 520 198 us, 1027 159, 2054 153, 3328 148.
-Plan plan_backward(int rows, int cols) {
+// 6400] bf16 in 520 198 us, 1027 159, 2054 153, 3328 148.  Few rows are one band,
+// whose sums go to dbias without the second launch: step of [16, 4096] bf16 10.0 -> 7.7
+// us, of 32 rows 10.0 -> 10.4.
+Plan plan_backward(int rows, int cols, int groups) {
+    if (rows <= 16 && groups <= 4) return plan_ckpt8(rows, cols, 1, 1, INT_MAX, 1);
     return plan_ckpt8(rows, cols, 8192, 4, INT_MAX, 1024);
 }
 
@@ -625,7 +633,8 @@ int mi_bias_gelu_forward_ckpt8(const void* in, const float* bias, const int* off
 
 size_t mi_gelu_backward_ckpt8_workspace(int rows, int cols, int groups) {
     if (rows <= 0 || cols <= 0 || groups <= 0) return 0;
-    return colsum_bytes(plan_backward(rows, cols).bands + groups - 1, cols);
+    const int bands = plan_backward(rows, cols, groups).bands;
+    return bands > 1 ? colsum_bytes(bands + groups - 1, cols) : 0;
 }
 
 int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales, const float* bias,
@@ -641,12 +650,15 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
     if (groups > 1 && !offsets)
         return set_error(MI_ERR_INVALID_ARG, "%s: %d groups need offsets", name, groups);
     hipStream_t st = to_stream(stream);
-    const Plan p = plan_backward(rows, cols);
-    int err = MI_OK;
-    char* ws = static_cast<char*>(
-        workspace_get(mi_gelu_backward_ckpt8_workspace(rows, cols, groups), st, &err));
-    if (!ws) return err;
-    float* part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    const Plan p = plan_backward(rows, cols, groups);
+    float* part = nullptr;
+    if (p.bands > 1) {
+        int err = MI_OK;
+        char* ws = static_cast<char*>(
+            workspace_get(mi_gelu_backward_ckpt8_workspace(rows, cols, groups), st, &err));
+        if (!ws) return err;
+        part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    }
     const double bytes = static_cast<double>(rows) * cols *
                          ((act != nullptr ? 3 : 2) * row_type_size(type) + 1);
     with_row_type(type, [&](auto t) {
@@ -660,11 +672,12 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
                                        static_cast<const uint8_t*>(scales), bias, offsets,
                                        static_cast<const char*>(grad_out),
                                        static_cast<char*>(grad_in), static_cast<char*>(act), part,
-                                       rows, cols, groups, p.band, p.tiles, p.last_lanes);
+                                       dbias, rows, cols, groups, p.band, p.tiles, p.last_lanes);
                 });
             });
         });
     });
+    if (p.bands == 1) return check_launch(name);
     if (int rc = check_launch(name)) return rc;
     const int each = p.bands / groups;  // partial rows of a group, about
     const int slices = each >= 64 ? 16 : each >= 16 ? 8 : each >= 8 ? 4 : 1;
