@@ -49,9 +49,14 @@ struct Unit {
     int n;    // columns of it inside the row, 0 to 8
 };
 
+// The units of a workgroup's lanes: all whole; whole or empty; one of them partial.
+// The first two have accesses without branches on the unit's length.
+enum class Units { Whole, WholeOrEmpty, Partial };
+
 struct Task {
     int tile, band;
     int lanes, row_lanes, row_lane;
+    Units units;
     Unit un;
 };
 
@@ -64,6 +69,9 @@ __device__ __forceinline__ Task workgroup_task(int cols, int tiles, int last_lan
     t.row_lane = static_cast<int>(threadIdx.x) / t.lanes;
     t.un.col = t.tile * kTile + static_cast<int>(threadIdx.x & (t.lanes - 1)) * kUnit;
     t.un.n = max(0, min(kUnit, cols - t.un.col));
+    t.units = cols - t.tile * kTile >= t.lanes * kUnit ? Units::Whole
+              : cols % kUnit == 0                      ? Units::WholeOrEmpty
+                                                       : Units::Partial;
     return t;
 }
 
@@ -75,14 +83,17 @@ struct RawUnit {
     u32x4 a[kUnit / row_vec<T>()];
 };
 
-template <int T, bool NT>
+template <int T, Units UN, bool NT>
 __device__ __forceinline__ RawUnit<T> load_unit(const char* row, const Unit& un) {
     RawUnit<T> r;
     const char* p = row + static_cast<size_t>(un.col) * sizeof(row_elem<T>);
     const int n = un.n;
-    if (n == kUnit) {
+    if (UN == Units::Whole || n == kUnit) {
 #pragma unroll
         for (int i = 0; i < kUnit / row_vec<T>(); ++i) r.a[i] = load16b<NT>(p + 16 * i);
+    } else if constexpr (UN == Units::WholeOrEmpty) {
+#pragma unroll
+        for (int i = 0; i < kUnit / row_vec<T>(); ++i) r.a[i] = u32x4{0, 0, 0, 0};
     } else if constexpr (T == MI_TYPE_F32) {
         const u32x4 p4 = n & 4 ? load16b<NT>(p) : u32x4{0, 0, 0, 0};
         const u32x2 p2 = n & 2 ? load_piece<u32x2>(p + (n & 4) * 4) : u32x2{0, 0};
@@ -111,7 +122,7 @@ __device__ __forceinline__ void unpack_unit(const RawUnit<T>& r, float (&v)[kUni
     }
 }
 
-template <int T>
+template <int T, Units UN>
 __device__ __forceinline__ void store_unit(char* row, const Unit& un, const float (&v)[kUnit]) {
     char* p = row + static_cast<size_t>(un.col) * sizeof(row_elem<T>);
     const int n = un.n;
@@ -123,9 +134,11 @@ __device__ __forceinline__ void store_unit(char* row, const Unit& un, const floa
         for (int e = 0; e < row_vec<T>(); ++e) part[e] = v[i * row_vec<T>() + e];
         a[i] = row_pack<T>(part);
     }
-    if (n == kUnit) {
+    if (UN == Units::Whole || n == kUnit) {
 #pragma unroll
         for (int i = 0; i < kUnit / row_vec<T>(); ++i) store16b(p + 16 * i, a[i]);
+    } else if constexpr (UN == Units::WholeOrEmpty) {
+        return;
     } else if constexpr (T == MI_TYPE_F32) {
         const u32x4 rest = n & 4 ? a[1] : a[0];
         if (n & 4) store16b(p, a[0]);
@@ -139,10 +152,12 @@ __device__ __forceinline__ void store_unit(char* row, const Unit& un, const floa
     }
 }
 
+template <Units UN>
 __device__ __forceinline__ u32x2 load_codes(const uint8_t* row, const Unit& un) {
     const char* p = reinterpret_cast<const char*>(row) + un.col;
     const int n = un.n;
-    if (n == kUnit) return load_piece<u32x2>(p);
+    if (UN == Units::Whole || n == kUnit) return load_piece<u32x2>(p);
+    if constexpr (UN == Units::WholeOrEmpty) return u32x2{0, 0};
     const uint32_t p4 = n & 4 ? load_piece<uint32_t>(p) : 0;
     const uint32_t p2 = n & 2 ? load_piece<uint16_t>(p + (n & 4)) : 0;
     const uint32_t p1 = n & 1 ? load_piece<uint8_t>(p + (n & 6)) : 0;
@@ -150,12 +165,13 @@ __device__ __forceinline__ u32x2 load_codes(const uint8_t* row, const Unit& un) 
     return n & 4 ? u32x2{p4, rest} : u32x2{rest, 0};
 }
 
+template <Units UN>
 __device__ __forceinline__ void store_codes(uint8_t* row, const Unit& un, const u32x2& q) {
     char* p = reinterpret_cast<char*>(row) + un.col;
     const int n = un.n;
-    if (n == kUnit) {
+    if (UN == Units::Whole || n == kUnit) {
         store_piece(p, q);
-    } else {
+    } else if constexpr (UN == Units::Partial) {
         const uint32_t rest = n & 4 ? q.y : q.x;
         if (n & 4) store_piece<uint32_t>(p, q.x);
         if (n & 2) store_piece(p + (n & 4), static_cast<uint16_t>(rest));
@@ -225,9 +241,10 @@ __device__ __forceinline__ u32x2 encode(const float (&v)[kUnit], int scale) {
 template <int FMT>
 __device__ __forceinline__ void decode(const u32x2& q, int scale, const float (&add)[kUnit],
                                        float (&v)[kUnit]) {
-    const float step = scale == 255
-                           ? __int_as_float(0x7fc00000)
-                           : __builtin_ldexpf(1.0f, scale - (FMT == MI_CKPT8_INT8 ? 133 : 135));
+    // hidden from the compiler, which else tests every element for the NaN
+    const float step =
+        rounded(scale == 255 ? __int_as_float(0x7fc00000)
+                             : __builtin_ldexpf(1.0f, scale - (FMT == MI_CKPT8_INT8 ? 133 : 135)));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int w = static_cast<int>(q[h]);
@@ -262,11 +279,12 @@ __device__ __forceinline__ int first_row(const int* offsets, int rows) {
     return offsets == nullptr ? 0 : max(0, min(offsets[0], rows));
 }
 
+template <Units UN>
 __device__ __forceinline__ void load_bias(const float* bias, int g, int cols, const Unit& un,
                                           float (&b)[kUnit]) {
     const float* row = bias + static_cast<size_t>(g) * cols;
     unpack_unit<MI_TYPE_F32>(
-        load_unit<MI_TYPE_F32, false>(reinterpret_cast<const char*>(row), un), b);
+        load_unit<MI_TYPE_F32, UN, false>(reinterpret_cast<const char*>(row), un), b);
 }
 
 // f(g, a, b) for the rows a .. b - 1 of group g inside r0 .. r1 - 1.  Everything
@@ -298,8 +316,20 @@ __device__ __forceinline__ void for_segments(const int* offsets, int groups, int
 }
 
 // Rows of a lane that are in hand together: their loads are issued before the
-// first is computed.  One, two or four measured alike on large tensors.
+// first is computed.  Backward of [16384, 6400], [16384, 4096] bf16 by one 105.8,
+// 64.0 us, two 103.9, 61.7, four 108.9, 61.9; with the next rows' loads issued before
+// these are computed 115.8, 63.4 (fewer waves fit).
 constexpr int kRowsInHand = 2;
+
+template <class F>
+__device__ __forceinline__ void by_units(Units units, F body) {
+    if (units == Units::Whole)
+        body(std::integral_constant<Units, Units::Whole>());
+    else if (units == Units::WholeOrEmpty)
+        body(std::integral_constant<Units, Units::WholeOrEmpty>());
+    else
+        body(std::integral_constant<Units, Units::Partial>());
+}
 
 // GELU: out = gelu(in + bias) and the checkpoint of in; else the checkpoint.
 // out may be in: a lane reads its units of the rows in hand before it writes
@@ -315,34 +345,38 @@ __global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
     const size_t row_bytes = static_cast<size_t>(cols) * sizeof(row_elem<T>);
     const int blocks = (cols + kBlock - 1) / kBlock;
     const int r0 = t.band * band, r1 = min(r0 + band, rows);
-    for_segments(offsets, groups, rows, r0, r1, [&](int g, int a, int end) {
-        float b[kUnit];
-        if constexpr (GELU) load_bias(bias, g, cols, un, b);
-        for (int r = a + t.row_lane; r < end; r += U * t.row_lanes) {
-            RawUnit<T> raw[U];
+    by_units(t.units, [&](auto units) {
+        constexpr Units UN = decltype(units)::value;
+        for_segments(offsets, groups, rows, r0, r1, [&](int g, int a, int end) {
+            float b[kUnit];
+            if constexpr (GELU) load_bias<UN>(bias, g, cols, un, b);
+            for (int r = a + t.row_lane; r < end; r += U * t.row_lanes) {
+                RawUnit<T> raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int rr = r + u * t.row_lanes;
-                raw[u] = load_unit<T, NT>(in + (rr < end ? rr : r) * row_bytes, un);
-            }
+                for (int u = 0; u < U; ++u) {
+                    const int rr = r + u * t.row_lanes;
+                    raw[u] = load_unit<T, UN, NT>(in + (rr < end ? rr : r) * row_bytes, un);
+                }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int rr = r + u * t.row_lanes;
-                if (rr >= end) break;
-                const int scale = block_scale<T>(raw[u]);
-                float v[kUnit];
-                unpack_unit<T>(raw[u], v);
-                store_codes(q + static_cast<size_t>(rr) * cols, un, encode<FMT>(v, scale));
-                if (un.n > 0 && un.col % kBlock == 0)
-                    scales[static_cast<size_t>(rr) * blocks + un.col / kBlock] =
-                        static_cast<uint8_t>(scale);
-                if constexpr (GELU) {
+                for (int u = 0; u < U; ++u) {
+                    const int rr = r + u * t.row_lanes;
+                    if (rr >= end) break;
+                    const int scale = block_scale<T>(raw[u]);
+                    float v[kUnit];
+                    unpack_unit<T>(raw[u], v);
+                    store_codes<UN>(q + static_cast<size_t>(rr) * cols, un,
+                                      encode<FMT>(v, scale));
+                    if (un.n > 0 && un.col % kBlock == 0)
+                        scales[static_cast<size_t>(rr) * blocks + un.col / kBlock] =
+                            static_cast<uint8_t>(scale);
+                    if constexpr (GELU) {
 #pragma unroll
-                    for (int e = 0; e < kUnit; ++e) v[e] = gelu_pair(v[e] + b[e]).y;
-                    store_unit<T>(out + rr * row_bytes, un, v);
+                        for (int e = 0; e < kUnit; ++e) v[e] = gelu_pair(v[e] + b[e]).y;
+                        store_unit<T, UN>(out + rr * row_bytes, un, v);
+                    }
                 }
             }
-        }
+        });
     });
 }
 
@@ -357,13 +391,25 @@ __global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
     const int blocks = (cols + kBlock - 1) / kBlock;
     const int r0 = t.band * band, r1 = min(r0 + band, rows);
     const float none[kUnit] = {};
-    for (int r = r0 + t.row_lane; r < r1; r += t.row_lanes) {
-        float v[kUnit];
-        decode<FMT>(load_codes(q + static_cast<size_t>(r) * cols, un),
-                    scales[static_cast<size_t>(r) * blocks + un.col / kBlock], none, v);
-        store_unit<T>(out + r * row_bytes, un, v);
-    }
+    // the empty lanes are gone
+    by_units(t.units == Units::Partial ? Units::Partial : Units::Whole, [&](auto units) {
+        constexpr Units UN = decltype(units)::value;
+        for (int r = r0 + t.row_lane; r < r1; r += t.row_lanes) {
+            float v[kUnit];
+            decode<FMT>(load_codes<UN>(q + static_cast<size_t>(r) * cols, un),
+                        scales[static_cast<size_t>(r) * blocks + un.col / kBlock], none, v);
+            store_unit<T, UN>(out + r * row_bytes, un, v);
+        }
+    });
 }
+
+// What the backward pass reads of a row.
+template <int T>
+struct HeldRow {
+    RawUnit<T> grad;
+    u32x2 code;
+    int scale;
+};
 
 // u = value of the checkpoint + bias; grad_in = grad_out gelu'(u); act =
 // gelu(u); the column sums of grad_in over the band's rows of group g, added
@@ -385,38 +431,37 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
     const int blocks = (cols + kBlock - 1) / kBlock;
     const int scale_at = min(un.col / kBlock, blocks - 1);
     const int r0 = t.band * band, r1 = min(r0 + band, rows);
-    for_segments(offsets, groups, rows, r0, r1, [&](int g, int a, int end) {
+    auto segment = [&](auto units, int g, int a, int end) {
+        constexpr Units UN = decltype(units)::value;
         float b[kUnit], acc[kUnit];
-        load_bias(bias, g, cols, un, b);
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e) acc[e] = 0.0f;
+        for (int e = 0; e < kUnit; ++e) b[e] = acc[e] = 0.0f;
+        if (un.n > 0) load_bias<UN>(bias, g, cols, un, b);
         // The rows are taken in turn from a place that differs from band to band:
         // bands that are all at the same row of theirs touch the same memory
         // channels where a band is a power of two of bytes ([8192, 4096] fp32 85
         // us in step, 67 so; other sizes alike).
         const int trips = (end - a + U * t.row_lanes - 1) / (U * t.row_lanes);
         int trip = static_cast<int>(static_cast<unsigned>(t.band) * 3u % trips);
-        for (int i = 0; i < trips; ++i, trip = trip + 1 < trips ? trip + 1 : 0) {
-            const int r = a + t.row_lane + trip * U * t.row_lanes;
-            if (r >= end) continue;
-            RawUnit<T> raw[U];
-            u32x2 code[U];
-            int scale[U];
+        auto row_of = [&](int of, int u) { return a + t.row_lane + (of * U + u) * t.row_lanes; };
+        // Rows behind the segment's last read the last one and are not used.
+        auto load = [&](int of, HeldRow<T> (&h)[U]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int want = r + u * t.row_lanes;
-                const size_t rr = want < end ? want : r;
-                code[u] = load_codes(q + rr * cols, un);
-                scale[u] = scales[rr * blocks + scale_at];
-                raw[u] = load_unit<T, NT>(grad_out + rr * row_bytes, un);
+                const size_t r = min(row_of(of, u), end - 1);
+                h[u].code = load_codes<UN>(q + r * cols, un);
+                h[u].scale = scales[r * blocks + scale_at];
+                h[u].grad = load_unit<T, UN, NT>(grad_out + r * row_bytes, un);
             }
+        };
+        auto use = [&](int of, const HeldRow<T> (&h)[U]) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int rr = r + u * t.row_lanes;
-                if (rr >= end) break;
+                const int r = row_of(of, u);
+                if (r >= end) break;
                 float v[kUnit], d[kUnit];
-                unpack_unit<T>(raw[u], d);
-                decode<FMT>(code[u], scale[u], b, v);
+                unpack_unit<T>(h[u].grad, d);
+                decode<FMT>(h[u].code, h[u].scale, b, v);
 #pragma unroll
                 for (int e = 0; e < kUnit; ++e) {
                     const GeluPair p = gelu_pair(v[e]);
@@ -424,10 +469,16 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
                     d[e] *= p.d;
                     v[e] = p.y;
                 }
-                store_unit<T>(grad_in + rr * row_bytes, un, d);
-                if constexpr (ACT) store_unit<T>(act + rr * row_bytes, un, v);
+                store_unit<T, UN>(grad_in + r * row_bytes, un, d);
+                if constexpr (ACT) store_unit<T, UN>(act + r * row_bytes, un, v);
             }
-        }
+        };
+        if (un.n > 0)
+            for (int i = 0; i < trips; ++i, trip = trip + 1 < trips ? trip + 1 : 0) {
+                HeldRow<T> held[U];
+                load(trip, held);
+                use(trip, held);
+            }
         const int width = t.lanes * kUnit;
         float* mine = red + threadIdx.x * kUnit;
 #pragma unroll
@@ -444,6 +495,11 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
                 part[static_cast<size_t>(t.band + g) * cols + col] = sum;
         }
         __syncthreads();
+    };
+    // empty lanes only take part in the sums, so units are whole or partial
+    by_units(t.units == Units::Partial ? Units::Partial : Units::Whole, [&](auto units) {
+        for_segments(offsets, groups, rows, r0, r1,
+                     [&](int g, int a, int end) { segment(units, g, a, end); });
     });
 }
 
