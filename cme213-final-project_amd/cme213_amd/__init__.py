@@ -215,6 +215,18 @@ def _resolve_current_stream():
 _current_stream = _resolve_current_stream()
 
 
+def _resolve_current_device():
+    """Returns a function that gives torch's current device number, the same way."""
+    try:
+        import torch
+    except ImportError:
+        return lambda: None
+    return getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+_current_device = _resolve_current_device()
+
+
 def _stream(stream):
     if stream is not None:
         return stream
@@ -525,15 +537,14 @@ def _buf(x, count, *dtypes):
     least that many elements, or a raw int address."""
     if x is None or isinstance(x, int):
         return x
-    import torch
     p = _ptr(x)
     if x.dtype not in dtypes:
         raise ValueError(f"tensor dtype {x.dtype}, expected {' or '.join(map(str, dtypes))}")
     if x.numel() < count:
         raise ValueError(f"tensor of {x.numel()} elements, at least {count} are needed")
-    if x.get_device() != torch.cuda.current_device():
+    if x.get_device() != _current_device():
         raise ValueError(f"tensor on cuda:{x.get_device()}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+                         f"cuda:{_current_device()}")
     return p
 
 

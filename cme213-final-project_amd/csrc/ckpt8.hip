@@ -321,6 +321,9 @@ __device__ __forceinline__ void for_segments(const int* offsets, int groups, int
 // these are computed 115.8, 63.4 (fewer waves fit).
 constexpr int kRowsInHand = 2;
 
+// The kernels take first what they use first: their leading 14 dwords of arguments
+// are in registers when a wave starts.
+
 template <class F>
 __device__ __forceinline__ void by_units(Units units, F body) {
     if (units == Units::Whole)
@@ -336,9 +339,9 @@ __device__ __forceinline__ void by_units(Units units, F body) {
 // them.
 template <int T, int FMT, bool GELU, bool NT>
 __global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
-    const char* in, const float* __restrict__ bias, const int* __restrict__ offsets, char* out,
-    uint8_t* __restrict__ q, uint8_t* __restrict__ scales, int rows, int cols, int groups,
-    int band, int tiles, int last_lanes) {
+    int cols, int tiles, int last_lanes, int band, int rows, int groups, const char* in,
+    const int* __restrict__ offsets, const float* __restrict__ bias, char* out,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
     constexpr int U = kRowsInHand;
     const Task t = workgroup_task(cols, tiles, last_lanes);
     const Unit un = t.un;
@@ -419,10 +422,11 @@ struct HeldRow {
 // sums are added to dbias at once.  grad_in may be grad_out.
 template <int T, int FMT, bool ACT, bool NT>
 __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
-    const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales,
-    const float* __restrict__ bias, const int* __restrict__ offsets, const char* grad_out,
-    char* grad_in, char* __restrict__ act, float* __restrict__ part, float* __restrict__ dbias,
-    int rows, int cols, int groups, int band, int tiles, int last_lanes) {
+    int cols, int tiles, int last_lanes, int band, int rows, int groups,
+    const int* __restrict__ offsets, const float* __restrict__ bias,
+    const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, const char* grad_out,
+    char* grad_in, char* __restrict__ act, float* __restrict__ part,
+    float* __restrict__ dbias) {
     constexpr int U = kRowsInHand;
     __shared__ float red[kThreads * kUnit];
     const Task t = workgroup_task(cols, tiles, last_lanes);
@@ -627,10 +631,10 @@ int launch_to_ckpt8(const char* name, const void* in, const float* bias, const i
             constexpr int T = decltype(t)::value, F = decltype(f)::value;
             with_flag(stream_loads(bytes), [&](auto nt) {
                 hipLaunchKernelGGL((to_ckpt8_kernel<T, F, GELU, decltype(nt)::value>), dim3(p.grid),
-                                   dim3(kThreads), 0, st, static_cast<const char*>(in), bias,
-                                   offsets, static_cast<char*>(out), static_cast<uint8_t*>(q),
-                                   static_cast<uint8_t*>(scales), rows, cols, groups, p.band,
-                                   p.tiles, p.last_lanes);
+                                   dim3(kThreads), 0, st, cols, p.tiles, p.last_lanes, p.band,
+                                   rows, groups, static_cast<const char*>(in), offsets, bias,
+                                   static_cast<char*>(out), static_cast<uint8_t*>(q),
+                                   static_cast<uint8_t*>(scales));
             });
         });
     });
@@ -724,11 +728,13 @@ int mi_gelu_backward_with_bias_backward_ckpt8(const void* q, const void* scales,
                 with_flag(stream_loads(bytes), [&](auto nt) {
                     constexpr bool A = decltype(a)::value, NT = decltype(nt)::value;
                     hipLaunchKernelGGL((gelu_bwd_ckpt8_kernel<T, F, A, NT>), dim3(p.grid),
-                                       dim3(kThreads), 0, st, static_cast<const uint8_t*>(q),
-                                       static_cast<const uint8_t*>(scales), bias, offsets,
+                                       dim3(kThreads), 0, st, cols, p.tiles, p.last_lanes, p.band,
+                                       rows, groups, offsets, bias,
+                                       static_cast<const uint8_t*>(q),
+                                       static_cast<const uint8_t*>(scales),
                                        static_cast<const char*>(grad_out),
                                        static_cast<char*>(grad_in), static_cast<char*>(act), part,
-                                       dbias, rows, cols, groups, p.band, p.tiles, p.last_lanes);
+                                       dbias);
                 });
             });
         });

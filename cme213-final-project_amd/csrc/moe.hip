@@ -192,7 +192,8 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
         for (int j = 0; j < k; ++j) {
             const double m = group_max_d<L>(rank[0]);
             const bool won = rank[0] == m;
-            move_up<D>(rank, won, rank_of(kNoKey, 1023.0), std::make_integer_sequence<int, D - 1>());
+            move_up<D>(rank, won, rank_of(kNoKey, 1023.0),
+                       std::make_integer_sequence<int, D - 1>());
             first = j == 0 ? m : first;
             mine = gl == j ? m : mine;
         }
@@ -620,9 +621,9 @@ __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
 // one wave, its loads of both come before its stores of the later one.
 template <int T, int KB, int G, int LT, bool NT>
 __global__ __launch_bounds__(G > kWaves ? G * kWave : kThreads) void combine_bwd_kernel(
-    const char* __restrict__ dout, const char* y, const int* __restrict__ position,
-    const float* __restrict__ weights, char* dy, float* __restrict__ dweights, int tokens, int k,
-    int rows, int chunks, size_t row_bytes) {
+    int tokens, int k, int rows, int chunks, size_t row_bytes, const int* __restrict__ position,
+    const float* __restrict__ weights, const char* __restrict__ dout, const char* y, char* dy,
+    float* __restrict__ dweights) {
     constexpr int V = row_vec<T>();
     constexpr int S = 16 / V;
     constexpr int UC = KB >= 4 ? 1 : 4 / KB;
@@ -1057,10 +1058,10 @@ int mi_moe_combine_backward(const void* dout, const void* y, const int* position
                 constexpr int G = decltype(g)::value, LT = decltype(lanes)::value;
                 const dim3 grid(token_grid(tokens, G > 1 ? 1 : kThreads / LT));
                 hipLaunchKernelGGL((combine_bwd_kernel<T, KB, G, LT, decltype(nt)::value>), grid,
-                                   dim3(G > kWaves ? G * kWave : kThreads), 0, st,
+                                   dim3(G > kWaves ? G * kWave : kThreads), 0, st, tokens, k,
+                                   rows, chunks, row_bytes, position, weights,
                                    static_cast<const char*>(dout), static_cast<const char*>(y),
-                                   position, weights, static_cast<char*>(dy), dweights, tokens, k,
-                                   rows, chunks, row_bytes);
+                                   static_cast<char*>(dy), dweights);
             };
             using std::integral_constant;
             const int g = combine_waves(tokens, k, chunks, dy == y, row_bytes % 16 != 0);

@@ -248,6 +248,13 @@ def test_calls_refuse_what_they_cannot_take(dev):
         M.float_to_ckpt8(x, q, s[:3], 4, 8)
     M.float_to_ckpt8(x, q.view(torch.int8), s, 4, 8)
     M.float_to_ckpt8(x, q.view(torch.float8_e4m3fn), s, 4, 8, M.CKPT8_E4M3)
+    current = M._current_device
+    try:
+        M._current_device = lambda: 1  # as if another device were the current one
+        with pytest.raises(ValueError, match="the current device is cuda:1"):
+            M.float_to_ckpt8(x, q, s, 4, 8)
+    finally:
+        M._current_device = current
     big = torch.zeros(2001, dtype=torch.int32, device=dev)
     with pytest.raises(M.MIError, match="experts"):
         M.moe_sort(pos, big, None, pos, 4, 2000)
