@@ -218,7 +218,8 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
 // d = sum_j w_j dw_j; the term in p_e only where the weights are not
 // renormalised, [- d] only where they are.  The slots' terms are added into a
 // row of zeros in LDS, slot after slot (a wave's LDS operations run in order),
-// which costs less than comparing every element's number with every slot's.
+// which costs less than comparing every element's number with every slot's (32768 x
+// 256 fp32, 8 slots: 51.0 -> 18.4 us, where the bytes take 14).
 template <int T, int L, int P, bool RENORM>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids,

@@ -362,8 +362,8 @@ int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens
                         int k, int renormalise, int type, void* stream);
 
 /* dlogits (overwritten, all of [tokens, experts]) from dweights [tokens, k],
- * with ids and weights as the forward call returned them.  Slots with id -1
- * take no part.  logits may be NULL if renormalise != 0. */
+ * with ids and weights as the forward call returned them.  Slots with an id
+ * outside [0, experts) take no part; slots of one expert add up.  logits may be NULL if renormalise != 0. */
 int mi_moe_gate_backward(const void* logits, const int* ids, const float* weights,
                          const float* dweights, void* dlogits, int tokens, int experts, int k,
                          int renormalise, int type, void* stream);
@@ -379,7 +379,7 @@ size_t mi_moe_sort_workspace(int slots, int experts);
 
 /* out[position[t * k + j], :] = x[t, :].  x is [tokens, cols], out [rows,
  * cols]; a slot whose position is outside [0, rows) is dropped, and rows that no
- * slot has are left as they were. */
+ * slot has are left as they were.  No two slots may have the same row. */
 int mi_moe_dispatch_forward(const void* x, const int* position, void* out, int tokens, int k,
                             int rows, int cols, int type, void* stream);
 

@@ -322,3 +322,57 @@ def test_checkpoint_past_2_31_elements(dev):
         if part.start:
             last = g[-50:]
             R.near("dbias", host(db[1]), last.sum(0), 1e-4 * np.sqrt((last ** 2).sum(0)) + 1e-5)
+
+
+@pytest.mark.parametrize("n,c", [(17_000_003, 8), (4_300_001, 264)])
+def test_more_tokens_than_the_grid_has_room_for(dev, n, c):
+    """Tokens past the workgroups of one launch are taken in strides: the router (17 million
+    rows) and one choice's rows there and back, by an index that reverses them."""
+    note(f"{n} tokens of {c}")
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    if c == 8:
+        l = torch.randn(n, 2, device=dev, generator=gen, dtype=torch.float16)
+        ids = torch.empty(n, 1, dtype=torch.int32, device=dev)
+        w = torch.empty(n, 1, device=dev)
+        M.moe_gate_forward(l, ids, w, n, 2, 1, False)
+        lf = l.float()
+        assert torch.equal(ids[:, 0], (lf[:, 1] > lf[:, 0]).int())
+        p = torch.softmax(lf, 1)
+        assert (w[:, 0] - p.amax(1)).abs().max() <= 16 * R.U
+        dl, dw = torch.empty_like(l), torch.ones(n, 1, device=dev)
+        M.moe_gate_backward(l, ids, w, dw, dl, n, 2, 1, False)
+        # p (1 - p) up to its own rounding and fp16's
+        want = (p[:, 0] * p[:, 1]) * torch.where(ids[:, 0] == 0, 1.0, -1.0)
+        assert (dl[:, 0].float() - want).abs().max() <= 0.25 * 2.0 ** -11 + 32 * R.U
+    x = torch.randn(n, c, device=dev, generator=gen, dtype=torch.bfloat16)
+    pos = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=dev)
+    out, one = torch.empty_like(x), torch.ones(n, 1, device=dev)
+    M.moe_dispatch_forward(x, pos, out, n, 1, n, c)
+    assert torch.equal(out, x.flip(0))
+    back = torch.empty_like(x)
+    M.moe_dispatch_backward(out, pos, back, n, 1, n, c)
+    assert torch.equal(back, x)
+    M.moe_combine_forward(out, pos, one, back.zero_(), n, 1, n, c)
+    assert torch.equal(back, x)
+    dw = torch.empty(n, 1, device=dev)
+    M.moe_combine_backward(x, out, pos, one, out, dw, n, 1, n, c)
+    assert torch.equal(out, x.flip(0))
+    want = torch.empty(n, device=dev)
+    for i in range(0, n, 1 << 20):
+        want[i:i + (1 << 20)] = x[i:i + (1 << 20)].double().square().sum(1)
+    assert ((dw[:, 0] - want).abs() <= (c / 64 + 24) * R.U * want).all()
+
+
+def test_narrow_rows_of_many_tokens(dev):
+    """Rows of less than 16 bytes, one thread a token, past one launch's first million."""
+    n, k, c = 3_000_001, 2, 3
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(n, c, device=dev, generator=gen)
+    pos = torch.randperm(n * k, device=dev, generator=gen).to(torch.int32)
+    out = torch.empty(n * k, c, device=dev)
+    M.moe_dispatch_forward(x, pos, out, n, k, n * k, c)
+    assert torch.equal(out[pos.view(n, k)[:, 1].long()], x)
+    w = torch.full((n, k), 0.5, device=dev)
+    back = torch.empty_like(x)
+    M.moe_combine_forward(out, pos, w, back, n, k, n * k, c)
+    assert torch.equal(back, x)
