@@ -607,12 +607,16 @@ Plan plan_forward(int rows, int cols) { return plan_ckpt8(rows, cols, 4096, 2, 4
 // Backward: every band leaves a partial row to write and add up, so bands are
 // longer: [4096, 1024] bf16 in 2048 workgroups of one row a lane 13.8 + 5.9 us (the
 // sums), in 512 of four 8.8 + 3.9.  Too few workgroups starve the memory: [16384,
-// 6400] bf16 in 520 198 us, 1027 159, 2054 153, 3328 148.  Few rows are one band,
-// whose sums go to dbias without the second launch: step of [16, 4096] bf16 10.0 -> 7.7
-// us, of 32 rows 10.0 -> 10.4.
+// 6400] bf16 in 520 198 us, 1027 159, 2054 153, 3328 148 (of an earlier kernel); and
+// 8192 waves or 32768 as the target: bf16 with act [16384, 6400] 148 -> 139 us, 8192
+// columns 178 -> 165.  Six trips a row lane instead of four where the tensor is large:
+// fp32 [8192, 4096] with act 101 -> 94 us, but [4096, 1024] bf16 step 15.4 -> 16.5.
+// Few rows are one band, whose sums go to dbias without the second launch: step of
+// [16, 4096] bf16 10.0 -> 7.7 us, of 32 rows 10.0 -> 10.4.
 Plan plan_backward(int rows, int cols, int groups) {
     if (rows <= 16 && groups <= 4) return plan_ckpt8(rows, cols, 1, 1, INT_MAX, 1);
-    return plan_ckpt8(rows, cols, 8192, 4, INT_MAX, 1024);
+    const bool large = static_cast<long long>(rows) * cols >= 65536ll * kTile;
+    return plan_ckpt8(rows, cols, 32768, large ? 6 : 4, INT_MAX, 1024);
 }
 
 int check_args(const char* name, int rows, int cols, int groups, int format, int type) {
