@@ -30,6 +30,7 @@ constexpr int kThreads = 256;
 constexpr int kUnit = 8;              // consecutive columns of one lane
 constexpr int kTile = kUnit * kWave;  // columns of a full tile
 constexpr int kBlock = MI_CKPT8_BLOCK;  // four lanes
+constexpr int kLine = 64;  // columns: rows of codes are whole halves of cache lines
 constexpr int kMaxGroups = 1024;
 constexpr int kMaxRows = 1 << 30;  // keep row and column numbers, one tile or band
 constexpr int kMaxCols = 1 << 24;  // further on, inside an int, and the grids legal
@@ -63,12 +64,22 @@ struct Task {
 // The tile beside the full ones, last_lanes units wide (0: there is none), has the
 // first last_bands workgroups.  Begun last, its short rows were what the others had
 // to be waited for with: step of [16384, 1600] bf16 61.9 -> 57.7 us, of [6007, 2049]
-// fp16 37.3 -> 33.1.
+// fp16 37.3 -> 33.1.  The full tiles go along a band; where rows are not whole cache
+// lines, along eight bands side by side, since consecutive workgroups are on different
+// XCDs: the line that two tiles of a row share is then in one L2 (step of [6007, 2064]
+// fp16 35.9 -> 32.5 us, [8192, 6152] bf16 125.6 -> 120.2; but [4096, 4096] bf16 40.0 ->
+// 45.9).
 __device__ __forceinline__ Task workgroup_task(int cols, int full_tiles, int last_lanes,
                                                int last_bands) {
     Task t;
-    const int w = static_cast<int>(blockIdx.x) - last_bands;
+    int w = static_cast<int>(blockIdx.x) - last_bands;
     if (w >= 0) {
+        if (cols % kLine != 0) {
+            const int eight = 8 * full_tiles;
+            const int begin = w / eight * eight, i = w - begin;
+            if (begin + eight <= static_cast<int>(gridDim.x) - last_bands)
+                w = begin + i % 8 * full_tiles + i / 8;
+        }
         t.band = w / full_tiles;
         t.first_col = (w - t.band * full_tiles) * kTile;
         t.lanes = kWave;
@@ -575,8 +586,16 @@ struct Plan {
 // more than `most` bands.
 Plan plan_ckpt8(int rows, int cols, int waves, int least_trips, int most_trips, int most) {
     Plan p;
-    const int left = cols % kTile;
+    int left = cols % kTile;
     p.full_tiles = cols / kTile;
+    // A tile of 64 units that are whole or empty goes with the full ones where these
+    // take bands side by side: step of [20000, 2000] bf16 101.1 -> 96.6 us, [30000, 776]
+    // 70.4 -> 67.5 (1632 columns 73.0 -> 72.2 to 77; with a partial unit 777 columns 84.0
+    // -> 89.7).
+    if (cols % kLine != 0 && cols % kUnit == 0 && left > kTile / 2) {
+        left = 0;
+        ++p.full_tiles;
+    }
     p.last_lanes = 0;
     if (left) {
         p.last_lanes = 4;

@@ -192,6 +192,16 @@ def test_bias_gelu_checkpoint(dev, rows, cols, groups, how, t, fmt):
     assert_exact("dbias again", host(db2), host(db))
 
 
+# Rows that end inside a cache line: several tiles and bands, the last tile wide and of whole
+# units, wide with a partial one, narrow; a number of bands that is no multiple of eight.
+@pytest.mark.parametrize("t", list(R.TYPES))
+@pytest.mark.parametrize("rows,cols,groups,how", [(613, 1000, 3, "short"), (337, 2008, 2, "even"),
+                                                  (901, 1799, 5, "late"), (45, 5160, 1, None)])
+def test_rows_that_end_inside_a_line(dev, rows, cols, groups, how, t):
+    test_bias_gelu_checkpoint(dev, rows, cols, groups, how, t, "int8")
+    test_checkpoint(dev, rows, cols, t, "e4m3", False)
+
+
 @pytest.mark.parametrize("fmt", list(FORMATS))
 def test_bias_gelu_checkpoint_non_finite(dev, fmt):
     """Infinite and NaN inputs: out as gelu defines it; the block they are in reads as NaN in
