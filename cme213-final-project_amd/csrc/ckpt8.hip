@@ -48,11 +48,12 @@ static_assert(kBlock == 4 * kUnit, "a block's lanes are one DPP quad");
 struct Unit {
     int col;  // first column
     int n;    // columns of it inside the row, 0 to 8
+    int from, back;  // of Units::Partial: the eight columns from `from` on, `back` before col
 };
 
-// The units of a workgroup's lanes: all whole; whole or empty; one of them partial.
-// The first two have accesses without branches on the unit's length.
-enum class Units { Whole, WholeOrEmpty, Partial };
+// The units of a workgroup's lanes: all whole; whole or empty; one of them partial, in
+// rows of at least a unit; the partial unit that is all of a shorter row.
+enum class Units { Whole, WholeOrEmpty, Partial, Short };
 
 struct Task {
     int first_col, band;
@@ -94,13 +95,28 @@ __device__ __forceinline__ Task workgroup_task(int cols, int full_tiles, int las
     t.un.n = max(0, min(kUnit, cols - t.un.col));
     t.units = cols - t.first_col >= t.lanes * kUnit ? Units::Whole
               : cols % kUnit == 0                   ? Units::WholeOrEmpty
-                                                    : Units::Partial;
+              : cols > kUnit                        ? Units::Partial
+                                                    : Units::Short;
+    t.un.from = min(t.un.col, cols - kUnit);
+    t.un.back = min(t.un.col - t.un.from, kUnit);
     return t;
 }
 
-// A unit of a row, in the row's type.  The row's last unit may be partial: it
-// is moved as its 4, 2 and 1 elements, whichever its number is made of, and the
-// elements behind it read as 0.
+// A unit of a row, in the row's type.  The row's last unit may be partial: the
+// elements behind it read as 0.  It is read with as many elements before it as it lacks
+// and moved down, so that its wave's loads all go out together: read as its 4, 2 and 1
+// elements, as it is written, step of [30000, 777] bf16 84.2 us, 77.3 so, of [5000, 769]
+// fp32 27.7, 25.5, of [6007, 2049] fp16 33.9, 33.4.
+template <int N>
+__device__ __forceinline__ void move_down(uint32_t (&a)[N], int dwords) {
+#pragma unroll
+    for (int step = N; step >= 1; step /= 2) {
+        const bool on = dwords & step;
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] = on ? (i + step < N ? a[i + step] : 0u) : a[i];
+    }
+}
+
 template <int T>
 struct RawUnit {
     u32x4 a[kUnit / row_vec<T>()];
@@ -109,9 +125,30 @@ struct RawUnit {
 template <int T, Units UN, bool NT>
 __device__ __forceinline__ RawUnit<T> load_unit(const char* row, const Unit& un) {
     RawUnit<T> r;
-    const char* p = row + static_cast<size_t>(un.col) * sizeof(row_elem<T>);
+    const char* p = row + static_cast<size_t>(UN == Units::Partial ? un.from : un.col) *
+                              sizeof(row_elem<T>);
     const int n = un.n;
-    if (UN == Units::Whole || n == kUnit) {
+    if constexpr (UN == Units::Partial) {
+        constexpr int N = 4 * (kUnit / row_vec<T>());
+        uint32_t a[N];
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const u32x4 v = load16b<NT>(p + 16 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[4 * i + e] = v[e];
+        }
+        if constexpr (T == MI_TYPE_F32) {
+            move_down(a, un.back);
+        } else {
+            move_down(a, un.back / 2);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                a[i] = un.back & 1 ? a[i] >> 16 | (i + 1 < N ? a[i + 1] << 16 : 0u) : a[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i)
+            r.a[i] = u32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
+    } else if (UN == Units::Whole || n == kUnit) {
 #pragma unroll
         for (int i = 0; i < kUnit / row_vec<T>(); ++i) r.a[i] = load16b<NT>(p + 16 * i);
     } else if constexpr (UN == Units::WholeOrEmpty) {
@@ -179,6 +216,11 @@ template <Units UN>
 __device__ __forceinline__ u32x2 load_codes(const uint8_t* row, const Unit& un) {
     const char* p = reinterpret_cast<const char*>(row) + un.col;
     const int n = un.n;
+    if constexpr (UN == Units::Partial) {
+        const u32x2 v = load_piece<u32x2>(reinterpret_cast<const char*>(row) + un.from);
+        const uint64_t w = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(u32x2, un.back < kUnit ? w >> (8 * un.back) : 0);
+    }
     if (UN == Units::Whole || n == kUnit) return load_piece<u32x2>(p);
     if constexpr (UN == Units::WholeOrEmpty) return u32x2{0, 0};
     const uint32_t p4 = n & 4 ? load_piece<uint32_t>(p) : 0;
@@ -194,7 +236,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, const Unit& un, const 
     const int n = un.n;
     if (UN == Units::Whole || n == kUnit) {
         store_piece(p, q);
-    } else if constexpr (UN == Units::Partial) {
+    } else if constexpr (UN == Units::Partial || UN == Units::Short) {
         const uint32_t rest = n & 4 ? q.y : q.x;
         if (n & 4) store_piece<uint32_t>(p, q.x);
         if (n & 2) store_piece(p + (n & 4), static_cast<uint16_t>(rest));
@@ -353,8 +395,10 @@ __device__ __forceinline__ void by_units(Units units, F body) {
         body(std::integral_constant<Units, Units::Whole>());
     else if (units == Units::WholeOrEmpty)
         body(std::integral_constant<Units, Units::WholeOrEmpty>());
-    else
+    else if (units == Units::Partial)
         body(std::integral_constant<Units, Units::Partial>());
+    else
+        body(std::integral_constant<Units, Units::Short>());
 }
 
 // GELU: out = gelu(in + bias) and the checkpoint of in; else the checkpoint.
@@ -420,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
     const int r0 = t.band * band, r1 = min(r0 + band, rows);
     const float none[kUnit] = {};
     // the empty lanes are gone
-    by_units(t.units == Units::Partial ? Units::Partial : Units::Whole, [&](auto units) {
+    by_units(t.units == Units::WholeOrEmpty ? Units::Whole : t.units, [&](auto units) {
         constexpr Units UN = decltype(units)::value;
         for (int r = r0 + t.row_lane; r < r1; r += t.row_lanes) {
             float v[kUnit];
@@ -526,7 +570,7 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
         __syncthreads();
     };
     // empty lanes only take part in the sums, so units are whole or partial
-    by_units(t.units == Units::Partial ? Units::Partial : Units::Whole, [&](auto units) {
+    by_units(t.units == Units::WholeOrEmpty ? Units::Whole : t.units, [&](auto units) {
         for_segments(offsets, groups, rows, r0, r1,
                      [&](int g, int a, int end) { segment(units, g, a, end); });
     });
@@ -590,8 +634,8 @@ Plan plan_ckpt8(int rows, int cols, int waves, int least_trips, int most_trips, 
     p.full_tiles = cols / kTile;
     // A tile of 64 units that are whole or empty goes with the full ones where these
     // take bands side by side: step of [20000, 2000] bf16 101.1 -> 96.6 us, [30000, 776]
-    // 70.4 -> 67.5 (1632 columns 73.0 -> 72.2 to 77; with a partial unit 777 columns 84.0
-    // -> 89.7).
+    // 70.4 -> 67.5; with a partial unit [30000, 777] 77.0 -> 74.3, but [9000, 777] 28.3 ->
+    // 30.2.
     if (cols % kLine != 0 && cols % kUnit == 0 && left > kTile / 2) {
         left = 0;
         ++p.full_tiles;

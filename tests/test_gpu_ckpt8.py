@@ -193,10 +193,12 @@ def test_bias_gelu_checkpoint(dev, rows, cols, groups, how, t, fmt):
 
 
 # Rows that end inside a cache line: several tiles and bands, the last tile wide and of whole
-# units, wide with a partial one, narrow; a number of bands that is no multiple of eight.
+# units, wide with a partial one, narrow; a number of bands that is no multiple of eight; rows
+# of one unit and a part.
 @pytest.mark.parametrize("t", list(R.TYPES))
 @pytest.mark.parametrize("rows,cols,groups,how", [(613, 1000, 3, "short"), (337, 2008, 2, "even"),
-                                                  (901, 1799, 5, "late"), (45, 5160, 1, None)])
+                                                  (901, 1799, 5, "late"), (45, 5160, 1, None),
+                                                  (33, 9, 2, "even"), (20, 15, 1, None)])
 def test_rows_that_end_inside_a_line(dev, rows, cols, groups, how, t):
     test_bias_gelu_checkpoint(dev, rows, cols, groups, how, t, "int8")
     test_checkpoint(dev, rows, cols, t, "e4m3", False)
