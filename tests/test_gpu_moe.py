@@ -274,6 +274,14 @@ def test_rows_many_tokens(dev, n, k, c, t):
     R.near("sum", _h64(back), want, 2 * k * R.U * size + R.half_step(t, want) * (1 + 2.0 ** -10))
 
 
+@pytest.mark.parametrize("n,k,c,t", [(9001, 2, 2050, "f32"), (4100, 1, 1100, "f32"),
+                                     (1500, 2, 700, "f32"), (37, 3, 1500, "f16"),
+                                     (1, 2, 20000, "bf16")])
+def test_rows_in_segments(dev, n, k, c, t):
+    """Rows that several workgroups share, of a number of tokens that fills no last round."""
+    test_rows_many_tokens(dev, n, k, c, t)
+
+
 def test_rows_without_any(dev):
     """No rows at all: dispatch writes nothing, the sums are zero, their gradients too."""
     n, k, c = 7, 2, 40
