@@ -28,8 +28,7 @@ constexpr int kMaxGrid = 1 << 20;  // workgroups over the tokens, which are take
 constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's second dimension
 
 // ---------------------------------------------------------------------------
-// Router.  A row's E logits lie in the registers of L lanes, P consecutive
-// ones in each.  A logit becomes an integer key of the same order: the bits,
+// Router.  A row's E logits lie in the registers of L lanes, P in each.  A logit becomes an integer key of the same order: the bits,
 // the lower 31 inverted for negative numbers, -0 made +0; NaN ranks above all
 // and -inf is the lowest key, which is never chosen.  Key and expert make one
 // double, key * 1024 - expert: exact, all different, and in the order wanted,
@@ -38,7 +37,7 @@ constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's secon
 // ones (DPP) and the lane that held it moves up.  Lane j of the group keeps the
 // double of round j.
 //
-// Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 13.0 us,
+// Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 12.7 us,
 // its 36 MB take 7); 16 lanes a row (four rows a wave) share the steps between lanes
 // among four rows.  Rounds that search each lane's logits for the largest key
 // instead took 17.6 us there, and 6.9 instead of 4.3 for 1024 rows.
@@ -57,16 +56,27 @@ __device__ __forceinline__ float key_value(int key) {
     return __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
 }
 
-// Each lane's P consecutive logits, -inf behind the last expert.  Accesses may run
-// into the next row, and are cut to single elements only at the tensor's end.
+// A lane's logits of a row: P, in pieces of one access that it takes in turn with the row's
+// other lanes.  Their experts are gl * N, N = kPiece, and the steps that step_expert gives.
 template <int T, int P>
+constexpr int kPiece = P < row_vec<T>() ? P : row_vec<T>();
+
+template <int T, int L, int P>
+constexpr int step_expert(int p) {
+    constexpr int N = kPiece<T, P>;
+    return p / N * (N * L) + p % N;
+}
+
+// Loads them, -inf behind the last expert.  Accesses may run into the next row, and are
+// cut to single elements only at the tensor's end.
+template <int T, int L, int P>
 __device__ __forceinline__ void load_logits(const void* logits, size_t row, size_t rows, int gl,
                                             int experts, float (&v)[P]) {
-    constexpr int N = P < row_vec<T>() ? P : row_vec<T>();
+    constexpr int N = kPiece<T, P>;
     const size_t base = row * experts, total = rows * experts;
 #pragma unroll
     for (int c = 0; c < P; c += N) {
-        const int e0 = gl * P + c;
+        const int e0 = gl * N + step_expert<T, L, P>(c);
         float part[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) part[e] = 0.0f;
@@ -92,6 +102,18 @@ __device__ __forceinline__ double dpp_move_d(double v) {
     return __builtin_bit_cast(double, r);
 }
 
+// The last lane of a row of 16 (CTRL 0x142) or of 32 (0x143) to the rows behind it that
+// ROWS names; the others keep v.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_bcast_d(double v) {
+    const u32x2 b = __builtin_bit_cast(u32x2, v);
+    const int x = static_cast<int>(b.x), y = static_cast<int>(b.y);
+    const u32x2 r = {
+        static_cast<uint32_t>(__builtin_amdgcn_update_dpp(x, x, CTRL, ROWS, 0xF, false)),
+        static_cast<uint32_t>(__builtin_amdgcn_update_dpp(y, y, CTRL, ROWS, 0xF, false))};
+    return __builtin_bit_cast(double, r);
+}
+
 __device__ __forceinline__ double readlane_d(double v, int lane) {
     const u32x2 b = __builtin_bit_cast(u32x2, v);
     const u32x2 r = {
@@ -106,9 +128,11 @@ __device__ __forceinline__ double group_max_d(double v) {
     v = fmax(v, dpp_move_d<0x4E>(v));
     v = fmax(v, dpp_move_d<0x141>(v));
     v = fmax(v, dpp_move_d<0x140>(v));
-    if constexpr (L == 64)
-        v = fmax(fmax(readlane_d(v, 0), readlane_d(v, 16)),
-                 fmax(readlane_d(v, 32), readlane_d(v, 48)));
+    if constexpr (L == 64) {
+        v = fmax(v, dpp_bcast_d<0x142, 0xA>(v));
+        v = fmax(v, dpp_bcast_d<0x143, 0xC>(v));
+        v = readlane_d(v, 63);
+    }
     return v;
 }
 
@@ -128,7 +152,7 @@ __device__ __forceinline__ int rank_expert(double rank, int key) {
 // order, as pairs of places.
 template <int P>
 struct SortNet {
-    int lo[P * 4 + 1] = {}, hi[P * 4 + 1] = {};
+    int lo[P * 8] = {}, hi[P * 8] = {};
     int n = 0;
     constexpr SortNet() {
         for (int p = 1; p < P; p *= 2)
@@ -181,11 +205,12 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
         const bool valid = want < tokens;  // the others repeat the last row and store nothing
         const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
         float v[P];
-        load_logits<T, P>(logits, row, tokens, gl, experts, v);
+        load_logits<T, L, P>(logits, row, tokens, gl, experts, v);
         double rank[P];
-        const double own = gl * P;  // the lane's first expert
+        const double own = gl * kPiece<T, P>;  // the lane's first expert
 #pragma unroll
-        for (int p = 0; p < P; ++p) rank[p] = rank_of(order_key(v[p]), own) - p;
+        for (int p = 0; p < P; ++p)
+            rank[p] = rank_of(order_key(v[p]), own) - step_expert<T, L, P>(p);
         sort_falling(rank);
 
         double first = 0.0, mine = rank_of(kNoKey, 0.0);
@@ -219,19 +244,21 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
 // renormalised, [- d] only where they are.  The slots' terms are added into a
 // row of zeros in LDS, slot after slot (a wave's LDS operations run in order),
 // which costs less than comparing every element's number with every slot's (32768 x
-// 256 fp32, 8 slots: 51.0 -> 18.4 us, where the bytes take 14).
+// 256 fp32, 8 slots: 51.0 -> 18.4 us, where the bytes take 14).  A row's lanes take its
+// pieces in turn, so that their accesses, of LDS too, are consecutive: with 16 numbers of
+// a lane side by side 32768 x 256 bf16 took 14.7 us, 10.5 so, renormalised 13.8, 8.7.
 template <int T, int L, int P, bool RENORM>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids,
     const float* __restrict__ weights, const float* __restrict__ dweights,
     void* __restrict__ dlogits, int tokens, int experts, int k) {
     constexpr int PER = kThreads / L;
-    constexpr int N = P < row_vec<T>() ? P : row_vec<T>();
+    constexpr int N = kPiece<T, P>;
     __shared__ __align__(16) float terms[PER][L * P];
     const int gl = threadIdx.x & (L - 1);
     float* own = terms[threadIdx.x / L];
 #pragma unroll
-    for (int p = 0; p < P; ++p) own[gl * P + p] = 0.0f;
+    for (int p = 0; p < P; ++p) own[gl * N + step_expert<T, L, P>(p)] = 0.0f;
     for (long long base = static_cast<long long>(blockIdx.x) * PER; base < tokens;
          base += static_cast<long long>(gridDim.x) * PER) {
         const long long want = base + threadIdx.x / L;
@@ -246,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
             dw = dweights[row * k + gl];
         }
         float v[P];
-        if constexpr (!RENORM) load_logits<T, P>(logits, row, tokens, gl, experts, v);
+        if constexpr (!RENORM) load_logits<T, L, P>(logits, row, tokens, gl, experts, v);
         const bool live = id >= 0 && id < experts;
         const float wd = live ? w * dw : 0.0f;
         const float d = group_sum<L>(wd);
@@ -274,14 +301,14 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
         wave_order();
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const float t = own[gl * P + p];
+            const float t = own[gl * N + step_expert<T, L, P>(p)];
             v[p] = RENORM ? t : v[p] + t;
         }
 #pragma unroll
-        for (int p = 0; p < P; ++p) own[gl * P + p] = 0.0f;
+        for (int p = 0; p < P; ++p) own[gl * N + step_expert<T, L, P>(p)] = 0.0f;
 #pragma unroll
         for (int c = 0; c < P; c += N) {
-            const int e0 = gl * P + c;
+            const int e0 = gl * N + step_expert<T, L, P>(c);
             float part[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) part[e] = v[c + e];
@@ -296,10 +323,14 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     }
 }
 
-// f(L, P): 16 lanes a row up to 256 experts, 64 lanes above.
-template <class F>
-void with_gate_shape(int experts, F f) {
+// f(L, P): 16 lanes a row up to 256 experts, 64 lanes above; where `wide`, 16 up to 512.
+template <bool MAY_BE_WIDE, class F>
+void with_gate_shape(int experts, bool wide, F f) {
     using std::integral_constant;
+    if constexpr (MAY_BE_WIDE) {
+        if (wide && experts > 256 && experts <= 512)
+            return f(integral_constant<int, 16>(), integral_constant<int, 32>());
+    }
     if (experts <= 16)
         f(integral_constant<int, 16>(), integral_constant<int, 1>());
     else if (experts <= 32)
@@ -916,7 +947,9 @@ int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens
     if (!logits || !ids || !weights)
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     with_row_type(type, [&](auto t) {
-        with_gate_shape(experts, [&](auto l, auto p) {
+        // 512 experts, 8 chosen: 32768 tokens 30.5 us by 64 lanes a row, 23.7 by 16, 8192
+        // 9.8, 6.9, 3000 5.3, 5.2, but 1024 4.1, 5.0; 2 chosen, 32768 tokens 17.9, 20.0
+        with_gate_shape<true>(experts, tokens >= 4096 && k > 2, [&](auto l, auto p) {
             constexpr int T = decltype(t)::value, L = decltype(l)::value, P = decltype(p)::value;
             auto launch = [&](auto d, auto renorm) {
                 hipLaunchKernelGGL((gate_fwd_kernel<T, L, P, decltype(d)::value,
@@ -928,7 +961,7 @@ int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens
                 if constexpr (P > 8) {
                     if (k <= 8) return launch(std::integral_constant<int, 8>(), renorm);
                 }
-                launch(std::integral_constant<int, P>(), renorm);
+                launch(std::integral_constant<int, std::min(P, kMaxChoices)>(), renorm);
             });
         });
     });
@@ -944,7 +977,7 @@ int mi_moe_gate_backward(const void* logits, const int* ids, const float* weight
     if ((!logits && !renormalise) || !ids || !weights || !dweights || !dlogits)
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     with_row_type(type, [&](auto t) {
-        with_gate_shape(experts, [&](auto l, auto p) {
+        with_gate_shape<false>(experts, false, [&](auto l, auto p) {
             constexpr int T = decltype(t)::value, L = decltype(l)::value, P = decltype(p)::value;
             if (renormalise)
                 hipLaunchKernelGGL((gate_bwd_kernel<T, L, P, true>), dim3(gate_grid(tokens, L)),

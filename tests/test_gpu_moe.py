@@ -74,6 +74,14 @@ def test_gate_forward(dev, n, e, k, t, renorm):
 
 @pytest.mark.parametrize("renorm", [True, False])
 @pytest.mark.parametrize("t", list(R.TYPES))
+@pytest.mark.parametrize("n,e,k", [(4096, 512, 8), (4099, 257, 16)])
+def test_gate_of_many_tokens(dev, n, e, k, t, renorm):
+    """Between 256 and 512 experts, where many tokens share a wave."""
+    test_gate_forward(dev, n, e, k, t, renorm)
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("t", list(R.TYPES))
 @pytest.mark.parametrize("n,e,k", GATE_SHAPES)
 def test_gate_backward(dev, n, e, k, t, renorm):
     note(f"gate backward {n}x{e} k={k} {t} renorm={renorm}")
