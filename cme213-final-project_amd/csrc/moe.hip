@@ -37,7 +37,7 @@ constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's secon
 // ones (DPP) and the lane that held it moves up.  Lane j of the group keeps the
 // double of round j.
 //
-// Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 12.7 us,
+// Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 12.2 us,
 // its 36 MB take 7); 16 lanes a row (four rows a wave) share the steps between lanes
 // among four rows.  Rounds that search each lane's logits for the largest key
 // instead took 17.6 us there, and 6.9 instead of 4.3 for 1024 rows.
@@ -244,9 +244,9 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
 // renormalised, [- d] only where they are.  The slots' terms are added into a
 // row of zeros in LDS, slot after slot (a wave's LDS operations run in order),
 // which costs less than comparing every element's number with every slot's (32768 x
-// 256 fp32, 8 slots: 51.0 -> 18.4 us, where the bytes take 14).  A row's lanes take its
+// 256 fp32, 8 slots: 51.0 -> 18.4 us).  A row's lanes take its
 // pieces in turn, so that their accesses, of LDS too, are consecutive: with 16 numbers of
-// a lane side by side 32768 x 256 bf16 took 14.7 us, 10.5 so, renormalised 13.8, 8.7.
+// a lane side by side it took 18.0 us, 11.7 so (6.0 TB/s), bf16 14.7, 10.5, renormalised 13.8, 8.7.
 template <int T, int L, int P, bool RENORM>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids,
