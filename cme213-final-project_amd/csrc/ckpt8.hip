@@ -578,7 +578,7 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
 
 // dbias[g][c] += sum of group g's partial rows: 64 columns a workgroup, its
 // waves each a consecutive slice of the partial rows in order, then the waves
-// in order.  Loads are issued 16 at a time.  Latency-bound (3 to 5 us); 32 or 16
+// in order.  Loads are issued 16 at a time.  Latency-bound (4 to 7 us); 32 or 16
 // columns a workgroup and more slices were no faster, and slower for many groups.
 __global__ __launch_bounds__(1024) void group_sum_kernel(const float* __restrict__ part,
                                                          const int* __restrict__ offsets,

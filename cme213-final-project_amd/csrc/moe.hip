@@ -28,14 +28,14 @@ constexpr int kMaxGrid = 1 << 20;  // workgroups over the tokens, which are take
 constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's second dimension
 
 // ---------------------------------------------------------------------------
-// Router.  A row's E logits lie in the registers of L lanes, P in each.  A logit becomes an integer key of the same order: the bits,
-// the lower 31 inverted for negative numbers, -0 made +0; NaN ranks above all
-// and -inf is the lowest key, which is never chosen.  Key and expert make one
-// double, key * 1024 - expert: exact, all different, and in the order wanted,
-// equal logits by rising expert.  Each lane sorts its P doubles once, by a
-// network of minima and maxima; a round takes the largest of the lanes' first
-// ones (DPP) and the lane that held it moves up.  Lane j of the group keeps the
-// double of round j.
+// Router.  A row's E logits lie in the registers of L lanes, P in each.  A logit
+// becomes an integer key of the same order: the bits, the lower 31 inverted for
+// negative numbers, -0 made +0; NaN ranks above all and -inf is the lowest key,
+// which is never chosen.  Key and expert make one double, key * 1024 - expert:
+// exact, all different, and in the order wanted, equal logits by rising expert.
+// Each lane sorts its P doubles once, by a network of minima and maxima; a round
+// takes the largest of the lanes' first ones (DPP) and the lane that held it
+// moves up.  Lane j of the group keeps the double of round j.
 //
 // Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 12.2 us,
 // its 36 MB take 7); 16 lanes a row (four rows a wave) share the steps between lanes
@@ -244,9 +244,9 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
 // renormalised, [- d] only where they are.  The slots' terms are added into a
 // row of zeros in LDS, slot after slot (a wave's LDS operations run in order),
 // which costs less than comparing every element's number with every slot's (32768 x
-// 256 fp32, 8 slots: 51.0 -> 18.4 us).  A row's lanes take its
-// pieces in turn, so that their accesses, of LDS too, are consecutive: with 16 numbers of
-// a lane side by side it took 18.0 us, 11.7 so (6.0 TB/s), bf16 14.7, 10.5, renormalised 13.8, 8.7.
+// 256 fp32, 8 slots: 51.0 -> 18.4 us).  A row's lanes take its pieces in turn, so that
+// their accesses, of LDS too, are consecutive: with 16 numbers of a lane side by side it
+// took 18.0 us, 11.7 so (6.0 TB/s), bf16 14.7, 10.5, renormalised 13.8, 8.7.
 template <int T, int L, int P, bool RENORM>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids,
