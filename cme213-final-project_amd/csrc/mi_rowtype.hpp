@@ -193,18 +193,6 @@ __device__ __forceinline__ int dpp_move_i(int v) {
 }
 
 template <int L>
-__device__ __forceinline__ int group_max(int v) {
-    v = max(v, dpp_move_i<0xB1>(v));
-    v = max(v, dpp_move_i<0x4E>(v));
-    v = max(v, dpp_move_i<0x141>(v));
-    v = max(v, dpp_move_i<0x140>(v));
-    if constexpr (L == 64)
-        v = max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
-                max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-    return v;
-}
-
-template <int L>
 __device__ __forceinline__ float group_max(float v) {
     v = fmaxf(v, dpp_move<0xB1>(v));
     v = fmaxf(v, dpp_move<0x4E>(v));
