@@ -363,7 +363,8 @@ int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens
 
 /* dlogits (overwritten, all of [tokens, experts]) from dweights [tokens, k],
  * with ids and weights as the forward call returned them.  Slots with an id
- * outside [0, experts) take no part; slots of one expert add up.  logits may be NULL if renormalise != 0. */
+ * outside [0, experts) take no part; slots of one expert add up.  logits may be
+ * NULL if renormalise != 0. */
 int mi_moe_gate_backward(const void* logits, const int* ids, const float* weights,
                          const float* dweights, void* dlogits, int tokens, int experts, int k,
                          int renormalise, int type, void* stream);
@@ -395,7 +396,9 @@ int mi_moe_combine_forward(const void* y, const int* position, const float* weig
 
 /* dy[position[t * k + j], :] = weights[t, j] dout[t, :] (other rows are left as
  * they were); dweights[t, j] = the product of dout[t, :] and y[position[t * k +
- * j], :], 0 for a dropped slot.  dy may be y. */
+ * j], :], 0 for a dropped slot.  dy may be y: dy is the same bits then, dweights
+ * may be added in another order.  No two slots may have the same row (the two sums
+ * above read rows only and take the same row twice). */
 int mi_moe_combine_backward(const void* dout, const void* y, const int* position,
                             const float* weights, void* dy, float* dweights, int tokens, int k,
                             int rows, int cols, int type, void* stream);

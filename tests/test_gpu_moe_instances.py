@@ -1,7 +1,8 @@
 """Every kernel instance that the row calls of a mixture-of-experts layer and the 8-bit
 checkpoints can select: lanes and waves a token, sums held for 1, 2, 4, 8 or 16 choices,
 loads that stay in the caches or do not (tensors past 128 MB), whole and partial units,
-each row type and format; and bias gradients of segments of very different lengths.
+each row type and format.  Also bias gradients of segments of very different lengths, one
+row named by several slots of a sum.
 Compared with the formulas in 64 bits (elementary torch operations on the device), with
 moe_ref.py's bounds."""
 import math
@@ -234,3 +235,25 @@ def test_bias_gradients_of_uneven_segments(dev, rows, cols, groups, longest, t):
     length[longest] += rows - length.sum()
     assert length[longest] > 0.9 * rows
     _check_checkpoint(dev, rows, cols, [0] + np.cumsum(length).tolist(), t, "int8", False)
+
+
+@pytest.mark.parametrize("t", list(R.TYPES))
+@pytest.mark.parametrize("c", [3, 40, 1030])
+def test_sums_take_one_row_twice(dev, c, t):
+    """Slots that name the same row, of one token and of several: each adds it."""
+    n, k, rows = 5, 3, 4
+    note(f"one row twice c={c} {t}")
+    r = np.random.default_rng(c)
+    pos = np.array([2, 2, 2, 0, 1, 0, 3, 3, -1, 4, 1, 1, 0, 2, 3], np.int32)
+    y = torch.from_numpy(r.standard_normal((rows, c))).to(R.TYPES[t])
+    w = r.standard_normal((n, k)).astype(np.float32)
+    P, Y, W = torch.from_numpy(pos).to(dev), y.to(dev), torch.from_numpy(w).to(dev)
+    for name, weights in (("dispatch gradient", None), ("combine", w.astype(np.float64))):
+        out = torch.full((n, c), 77.0, dtype=R.TYPES[t], device=dev)
+        if weights is None:
+            M.moe_dispatch_backward(Y, P, out, n, k, rows, c)
+        else:
+            M.moe_combine_forward(Y, P, W, out, n, k, rows, c)
+        ref, size = R.gather_sum(y.double().numpy(), pos, weights, n, k, rows)
+        R.near(name, host(out.double()), ref,
+               2 * k * R.U * size + R.half_step(t, ref) * (1 + 2.0 ** -10))
