@@ -8,7 +8,8 @@
 // block of a row may be shorter).  With e = max(floor(log2 max |x|), -118) the
 // scale byte is e + 127; 255 marks a block that holds a NaN or an infinity, and
 // all of it reads as NaN.  An element is
-//   int8:  q = rint(x 2^(6-e)), at most 127, of value q 2^(e-6);
+//   int8:  q = rint(x 2^(6-e)), -128 to 127, of value q 2^(e-6) (-128 in the topmost block
+//          of a type is -2^(e+1), which rounds to -inf in it);
 //   e4m3:  q = e4m3(x 2^(8-e)), at most 448 in magnitude, of value q 2^(e-8).
 // The scaling is exact and the rounding (to nearest even) the only one, so a
 // value has one code whatever computes it: off by at most 2^(e-7) for int8

@@ -412,7 +412,10 @@ int mi_moe_combine_backward(const void* dout, const void* y, const int* position
  *   MI_CKPT8_E4M3: the OCP e4m3 number nearest to x 2^(8-e), cut at +-448, of
  *                  value q 2^(e-8).
  * A block with a NaN or an infinity has scale byte 255 and reads as NaN.  Half
- * values round to even.  rows at most 2^30, cols at most 2^24; no alignment
+ * values round to even.  The lowest integer is -128, of value -2^(e+1), which
+ * mi_ckpt8_to_float rounds to -inf where it is beyond the type: fp16 elements from
+ * -65280 down, fp32 and bf16 ones from -2^128 (1 - 2^-8) down (their gelu and its
+ * slope vanish either way).  rows at most 2^30, cols at most 2^24; no alignment
  * beyond the element's is needed. */
 #define MI_CKPT8_BLOCK 32
 #define MI_CKPT8_INT8 0

@@ -2,7 +2,7 @@
 checkpoints can select: lanes and waves a token, sums held for 1, 2, 4, 8 or 16 choices,
 loads that stay in the caches or do not (tensors past 128 MB), whole and partial units,
 each row type and format.  Also bias gradients of segments of very different lengths, one
-row named by several slots of a sum.
+row named by several slots of a sum, the lowest and largest values of a type.
 Compared with the formulas in 64 bits (elementary torch operations on the device), with
 moe_ref.py's bounds."""
 import math
@@ -257,3 +257,37 @@ def test_sums_take_one_row_twice(dev, c, t):
         ref, size = R.gather_sum(y.double().numpy(), pos, weights, n, k, rows)
         R.near(name, host(out.double()), ref,
                2 * k * R.U * size + R.half_step(t, ref) * (1 + 2.0 ** -10))
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("t", list(R.TYPES))
+def test_lowest_and_largest_values_of_a_type(dev, t, fmt):
+    """Elements of the type's lowest value, as masks have them: gelu and its slope are zero
+    there (to 1e-30), those of its largest value 1 times them, and nothing is NaN."""
+    rows, cols = 6, 64
+    note(f"lowest values {t} {fmt}")
+    fi = torch.finfo(R.TYPES[t])
+    x = torch.zeros(rows, cols, dtype=R.TYPES[t], device=dev)
+    x[1:4, 5], x[2, 40:], x[4, 7] = fi.min, fi.min, fi.max
+    low, high = x == fi.min, x == fi.max
+    b = torch.linspace(-1, 1, cols, device=dev)[None].contiguous()
+    q = torch.empty(rows, cols, dtype=torch.uint8, device=dev)
+    s = torch.empty(rows, 2, dtype=torch.uint8, device=dev)
+    out, gin, act = (torch.full_like(x, 77.0) for _ in range(3))
+    M.bias_gelu_forward_ckpt8(x, b, None, out, q, s, rows, cols, 1, FORMATS[fmt])
+    db = torch.zeros(1, cols, device=dev)
+    M.gelu_backward_with_bias_backward_ckpt8(q, s, b, None, torch.ones_like(x), gin, act, db, rows,
+                                             cols, 1, FORMATS[fmt])
+    for name, v in (("out", out), ("grad_in", gin), ("act", act)):
+        assert (v[low].abs() <= 1e-30).all(), name
+        assert not v.isnan().any(), name
+    assert (gin[high] == 1).all() and (out[high] == fi.max).all()
+    # the largest value's code is 127 of 128 (int8) or 448 of 512 (e4m3) of the next power
+    part = 127 / 128 if fmt == "int8" else 448 / 512
+    power = 2.0 ** (16 if t == "f16" else 128)
+    assert (act[high].double() == part * power).all()
+    # all other elements are zero: their column's slope is gelu'(b), once for each
+    zeros = (~(low | high)).sum(0).double()
+    d = _gelu64(b[0].double())[1]
+    _near("dbias", db[0], zeros * d + high.sum(0),
+          rows * (BWD_ATOL + BWD_RTOL * d.abs()) + 8 * R.U * rows)
