@@ -451,8 +451,11 @@ __global__ __launch_bounds__(kThreads) void to_ckpt8_kernel(
     });
 }
 
-// Memory-bound: [16384, 6400] to bf16 54.6 us (5.8 TB/s), to fp32 120.3 (4.4, of which
-// four of five bytes are stores); the checkpoint alone of bf16 58.4 (5.4), fp32 103.1.
+// Memory-bound: [16384, 6400] to bf16 54.8 us (5.8 TB/s), the checkpoint alone of it 59.9
+// (5.3).  fp32 rows are slower in every kernel here: to fp32 120.1 us (4.4), the checkpoint
+// of it 104.5 (5.05).  A unit of them is two accesses of 16 bytes, 32 bytes from those
+// of the next lane; a plain copy in this form reaches 3.98 TB/s, with each access side by
+// side 6.5.
 template <int T, int FMT>
 __global__ __launch_bounds__(kThreads) void from_ckpt8_kernel(
     const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, char* __restrict__ out,
@@ -579,8 +582,11 @@ __global__ __launch_bounds__(kThreads) void gelu_bwd_ckpt8_kernel(
 
 // dbias[g][c] += sum of group g's partial rows: 64 columns a workgroup, its
 // waves each a consecutive slice of the partial rows in order, then the waves
-// in order.  Loads are issued 16 at a time.  Latency-bound (4 to 7 us); 32 or 16
-// columns a workgroup and more slices were no faster, and slower for many groups.
+// in order.  Loads are issued 16 at a time.  Latency-bound: 4 to 7 us where segments are of
+// about one length.  The slices go by the average: a segment that holds nine tenths
+// of [16384, 1600] in 128 groups has one slice for its 950 partial rows, 47 us (5 where
+// the groups are even).  32 or 16 columns a workgroup and more slices were no faster, and
+// slower for many groups.
 __global__ __launch_bounds__(1024) void group_sum_kernel(const float* __restrict__ part,
                                                          const int* __restrict__ offsets,
                                                          float* __restrict__ dbias, int rows,

@@ -37,10 +37,12 @@ constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's secon
 // takes the largest of the lanes' first ones (DPP) and the lane that held it
 // moves up.  Lane j of the group keeps the double of round j.
 //
-// Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 12.2 us,
-// its 36 MB take 7); 16 lanes a row (four rows a wave) share the steps between lanes
-// among four rows.  Rounds that search each lane's logits for the largest key
-// instead took 17.6 us there, and 6.9 instead of 4.3 for 1024 rows.
+// Bound by these instructions, not by memory (32768 x 256 fp32, 8 chosen: 12.2 us, its
+// 36 MB take 7; bf16 12.4, for half the bytes): comparisons are of 64 bits, and the
+// network sorts all of a lane's logits however few are chosen (2 chosen 9.4 us, 1 7.6).
+// 16 lanes a row (four rows a wave) share the steps between lanes among four rows.
+// Rounds that search each lane's logits for the largest key instead took 17.6 us
+// there, and 6.9 instead of 4.3 for 1024 rows.
 // ---------------------------------------------------------------------------
 constexpr int kNoKey = static_cast<int>(0xff800000u ^ 0x7fffffffu);  // of -inf
 constexpr float kLog2e = 1.4426950408889634f;
@@ -246,7 +248,8 @@ __global__ __launch_bounds__(kThreads) void gate_fwd_kernel(const void* __restri
 // which costs less than comparing every element's number with every slot's (32768 x
 // 256 fp32, 8 slots: 51.0 -> 18.4 us).  A row's lanes take its pieces in turn, so that
 // their accesses, of LDS too, are consecutive: with 16 numbers of a lane side by side it
-// took 18.0 us, 11.7 so (6.0 TB/s), bf16 14.7, 10.5, renormalised 13.8, 8.7.
+// took 18.0 us, 11.7 so (6.0 TB/s), bf16 14.7, 10.5, renormalised 13.8, 8.7.  16-bit rows
+// (3.5 TB/s) are bound by instructions: every element passes through the row in LDS.
 template <int T, int L, int P, bool RENORM>
 __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids,
@@ -546,7 +549,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(
 // last chunk is moved back to end with the row: the elements that it shares with
 // the one before are computed twice, with the same result.
 //
-// Memory-bound: 5.3 to 6.1 TB/s on tensors past the last-level cache.
+// Memory-bound: 4.6 to 6.1 TB/s on tensors past the last-level cache.
 // ---------------------------------------------------------------------------
 struct Chunk {
     bool on;
@@ -612,7 +615,10 @@ __global__ __launch_bounds__(kThreads) void scatter_rows_kernel(
     }
 }
 
-// out[t] = sum over j, in order, of [w[t, j]] rows[position[t, j]].
+// out[t] = sum over j, in order, of [w[t, j]] rows[position[t, j]].  A choice's position,
+// then its chunks one by one are waited for before the next is loaded, so that nothing
+// of a dropped slot is read; many waves hide this ([8192 tokens, 8 choices] of 4096 bf16
+// 99 us, 6.1 TB/s), few do not (16 tokens of it 3.8 us; the shortest kernel here 1.4).
 template <int T, int U, int LT, bool WEIGHTED, bool NT>
 __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
     const char* __restrict__ src, const int* __restrict__ position,
@@ -656,8 +662,10 @@ __global__ __launch_bounds__(kThreads) void gather_sum_kernel(
 }
 
 // dy[position[t, j]] = w[t, j] dout[t]; dw[t, j] = dout[t] . y[position[t, j]].
-// G waves, or LT lanes of one, per token; KB is k rounded up, so that the k sums
-// stay in registers.  All loads of a step (UC chunks of dout, KB of y for each)
+// G waves, or LT lanes of one, per token; KB is k rounded up to a power of two, so that
+// the k sums stay in registers: a slot that does not exist costs a cached load and FMAs
+// (bf16 [8192 tokens] of 1024 columns, 4 choices 29.5 us, 5.1 TB/s, 5 38.2, 4.8, 8 56.9,
+// 5.0, 9 67.4, 4.7, 16 115.6, 4.8).  All loads of a step (UC chunks of dout, KB of y for each)
 // are issued before its first store; a dropped slot reads dout's chunk in the
 // place of y's, and what the moved-back last chunk shares with its neighbour is
 // left out of its sums.  dy may be y: a chunk of dy is written after the same chunk
@@ -815,7 +823,7 @@ unsigned token_grid(int tokens, int per_workgroup) {
         (static_cast<long long>(tokens) + per_workgroup - 1) / per_workgroup, kMaxGrid));
 }
 
-// Lanes of a token, and its chunks a lane has in hand.
+// Lanes of a token, and its chunks a lane takes.
 struct RowShape {
     int lanes, u;
 };
@@ -848,7 +856,7 @@ RowShape scatter_shape(int tokens, int chunks) {
     return {row_lanes(chunks), 1};
 }
 
-// Of the sums' rows, where each lane has a load for every choice besides: bf16
+// Of the sums' rows, whose chunks a lane takes one after another for every choice: bf16
 // [1024 tokens, 4 choices] of 4096 columns in segments of one, two, four chunks a lane
 // 6.9, 7.1, 8.9 us, [4096, 8] of 2048 33.7, 24.9, 28.8, fp32 [8192, 6] of 1600 72.3, 67.7,
 // 62.1.
