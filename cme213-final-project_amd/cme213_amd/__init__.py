@@ -85,6 +85,17 @@ _SIGS = {
     "mi_layernorm_backward": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, P]),
     "mi_layernorm_backward_residual": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, P]),
     "mi_layernorm_backward_noalloc": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, P]),
+    # RMS norm
+    "mi_rmsnorm_forward": (c_int, [P, P, P, P, c_int, c_int, c_float, c_int, P]),
+    "mi_residual_rmsnorm_forward":
+        (c_int, [P, P, P, P, P, P, c_int, c_int, c_float, c_int, P]),
+    "mi_rmsnorm_forward_row8":
+        (c_int, [P, P, P, P, P, P, c_int, c_int, c_float, c_int, c_int, c_int, P]),
+    "mi_residual_rmsnorm_forward_row8":
+        (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_float, c_int, c_int, c_int, P]),
+    "mi_rmsnorm_backward": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, P]),
+    "mi_rmsnorm_backward_residual": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, P]),
+    "mi_rmsnorm_backward_workspace": (c_size_t, [c_int, c_int, c_int]),
     # residual / bias / activations
     "mi_residual_add": (c_int, [P, P, P, c_longlong, P]),
     "mi_residual_add_with_bias": (c_int, [P, P, P, P, c_int, c_int, P]),
@@ -117,6 +128,11 @@ _SIGS = {
     "mi_adam_update": (c_int, [P, P, P, P, c_longlong, c_float, c_float, c_float, c_float, c_int,
                                c_float, P, P, P]),
     "mi_norm_sq_workspace": (c_size_t, [c_longlong]),
+    # gradients in many tensors
+    "mi_tensors_norm_sq_acc": (c_int, [P, P, P, c_int, P, P]),
+    "mi_tensors_scale": (c_int, [P, P, P, P, c_int, P, P]),
+    "mi_tensors_clip": (c_int, [P, P, P, P, c_int, c_float, P, P, P]),
+    "mi_tensors_workspace": (c_size_t, [c_int]),
     # 16-bit storage
     "mi_float_to_half": (c_int, [P, P, c_longlong, P]),
     "mi_half_to_float": (c_int, [P, P, c_longlong, P]),
@@ -129,6 +145,11 @@ _SIGS = {
     # mixture of experts
     "mi_moe_gate_forward": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
     "mi_moe_gate_backward": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "mi_moe_balance_forward":
+        (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_float, c_int, P]),
+    "mi_moe_balance_backward":
+        (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_float, c_int, c_int, P]),
+    "mi_moe_balance_workspace": (c_size_t, [c_int, c_int]),
     "mi_moe_sort": (c_int, [P, P, P, P, c_int, c_int, P]),
     "mi_moe_sort_workspace": (c_size_t, [c_int, c_int]),
     "mi_moe_dispatch_forward": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
@@ -558,6 +579,163 @@ def _codes_dtypes(fmt):
     return (torch.uint8, torch.int8 if fmt == CKPT8_INT8 else torch.float8_e4m3fn)
 
 
+# ----- RMS norm ---------------------------------------------------------------------
+
+ROW8_INT8, ROW8_E4M3 = 0, 1
+ROW8_BLOCK = 128
+
+
+def row8_scales(rows, cols, block=0) -> int:
+    """Scales of rows in 8 bits: one a row (block 0), or one for each 128 columns of it."""
+    return rows * (-(-cols // ROW8_BLOCK) if block else 1)
+
+
+def _row8_dtypes(fmt):
+    import torch
+    return (torch.uint8, torch.int8 if fmt == ROW8_INT8 else torch.float8_e4m3fn)
+
+
+def rmsnorm_forward(x, gamma, out, inv_rms, rows, cols, eps=1e-5, type=None, stream=None):
+    """out = x * r * gamma with r = 1 / sqrt(mean(x^2) + eps), kept in inv_rms [rows] (may be
+    None)."""
+    import torch
+    t = _type_of(x, type)
+    _check(lib.mi_rmsnorm_forward(_buf(x, rows * cols, _row_dtype(t)),
+                                  _buf(gamma, cols, torch.float32),
+                                  _buf(out, rows * cols, _row_dtype(t)),
+                                  _buf(inv_rms, rows, torch.float32), rows, cols, eps, t,
+                                  _stream(stream)))
+
+
+def residual_rmsnorm_forward(a, b, gamma, residual_out, out, inv_rms, rows, cols, eps=1e-5,
+                             type=None, stream=None):
+    """residual_out = a + b, out = rmsnorm_forward of it."""
+    import torch
+    t = _type_of(a, type)
+    n, d = rows * cols, _row_dtype(t)
+    _check(lib.mi_residual_rmsnorm_forward(_buf(a, n, d), _buf(b, n, d),
+                                           _buf(gamma, cols, torch.float32),
+                                           _buf(residual_out, n, d), _buf(out, n, d),
+                                           _buf(inv_rms, rows, torch.float32), rows, cols, eps, t,
+                                           _stream(stream)))
+
+
+def rmsnorm_forward_row8(x, gamma, q, scales, out, inv_rms, rows, cols, eps=1e-5, block=0,
+                         fmt=ROW8_E4M3, type=None, stream=None):
+    """rmsnorm_forward with the result in 8 bits: codes q [rows, cols] and fp32 scales (one a
+    row, or one for each 128 columns where block is ROW8_BLOCK); out and inv_rms may be None."""
+    import torch
+    t = _type_of(x, type)
+    n, d = rows * cols, _row_dtype(t)
+    _check(lib.mi_rmsnorm_forward_row8(_buf(x, n, d), _buf(gamma, cols, torch.float32),
+                                       _buf(q, n, *_row8_dtypes(fmt)),
+                                       _buf(scales, row8_scales(rows, cols, block), torch.float32),
+                                       _buf(out, n, d), _buf(inv_rms, rows, torch.float32), rows,
+                                       cols, eps, block, fmt, t, _stream(stream)))
+
+
+def residual_rmsnorm_forward_row8(a, b, gamma, residual_out, q, scales, out, inv_rms, rows, cols,
+                                  eps=1e-5, block=0, fmt=ROW8_E4M3, type=None, stream=None):
+    """residual_out = a + b, and rmsnorm_forward_row8 of it."""
+    import torch
+    t = _type_of(a, type)
+    n, d = rows * cols, _row_dtype(t)
+    _check(lib.mi_residual_rmsnorm_forward_row8(
+        _buf(a, n, d), _buf(b, n, d), _buf(gamma, cols, torch.float32), _buf(residual_out, n, d),
+        _buf(q, n, *_row8_dtypes(fmt)),
+        _buf(scales, row8_scales(rows, cols, block), torch.float32), _buf(out, n, d),
+        _buf(inv_rms, rows, torch.float32), rows, cols, eps, block, fmt, t, _stream(stream)))
+
+
+def _rmsnorm_backward(fn, grad_out, x, inv_rms, gamma, dx, dgamma, rows, cols, type, stream):
+    import torch
+    t = _type_of(grad_out, type)
+    n, d = rows * cols, _row_dtype(t)
+    _check(fn(_buf(grad_out, n, d), _buf(x, n, d), _buf(inv_rms, rows, torch.float32),
+              _buf(gamma, cols, torch.float32), _buf(dx, n, d), _buf(dgamma, cols, torch.float32),
+              rows, cols, t, _stream(stream)))
+
+
+def rmsnorm_backward(grad_out, x, inv_rms, gamma, grad_x, dgamma, rows, cols, type=None,
+                     stream=None):
+    """grad_x (overwritten) and dgamma +=; x is what was normalised."""
+    _rmsnorm_backward(lib.mi_rmsnorm_backward, grad_out, x, inv_rms, gamma, grad_x, dgamma, rows,
+                      cols, type, stream)
+
+
+def rmsnorm_backward_residual(grad_out, x, inv_rms, gamma, grad_residual, dgamma, rows, cols,
+                              type=None, stream=None):
+    """grad_residual += the rows' gradient, dgamma +=."""
+    _rmsnorm_backward(lib.mi_rmsnorm_backward_residual, grad_out, x, inv_rms, gamma,
+                      grad_residual, dgamma, rows, cols, type, stream)
+
+
+# ----- gradients in many tensors ----------------------------------------------------
+
+class TensorList:
+    """A program's gradients (float32, float16 and bfloat16 CUDA tensors, contiguous, on one
+    device) as the mi_tensors_* calls take them, and where their clipped values go: `outs`,
+    float32 tensors of as many elements each, or None for in place.  The tensors are kept alive
+    with the list; it is made once and used every step."""
+
+    def __init__(self, tensors, outs=None):
+        import torch
+        self.tensors = list(tensors)
+        self.count = len(self.tensors)
+        self.out_tensors = None if outs is None else list(outs)
+        if outs is not None and len(self.out_tensors) != self.count:
+            raise ValueError(f"{self.count} tensors and {len(self.out_tensors)} outs")
+        self._data = (c_void_p * self.count)(*[_ptr(t) or None for t in self.tensors])
+        self._sizes = (c_longlong * self.count)(*[t.numel() for t in self.tensors])
+        self._types = (c_int * self.count)(*[_type_of(t, None) for t in self.tensors])
+        self._outs = None
+        if outs is not None:
+            for t, o in zip(self.tensors, self.out_tensors):
+                if o.numel() != t.numel():
+                    raise ValueError(f"an out of {o.numel()} elements for {t.numel()}")
+            self._outs = (c_void_p * self.count)(*[_ptr(o, torch.float32) or None
+                                                   for o in self.out_tensors])
+        devices = {t.get_device() for t in self.tensors + (self.out_tensors or [])}
+        if len(devices) > 1:
+            raise ValueError(f"tensors on several devices: {sorted(devices)}")
+        self.device = devices.pop() if devices else None
+
+    def args(self):
+        """tensors, outs, sizes, types and count, for bind()."""
+        return (ctypes.addressof(self._data),
+                None if self._outs is None else ctypes.addressof(self._outs),
+                ctypes.addressof(self._sizes), ctypes.addressof(self._types), self.count)
+
+    def _here(self):
+        if self.device is not None and self.device != _current_device():
+            raise ValueError(f"tensors on cuda:{self.device}, the current device is "
+                             f"cuda:{_current_device()}")
+        return self.args()
+
+
+def tensors_norm_sq_acc(tensors, result, stream=None):
+    """result += the sum of the squares of all elements of a TensorList."""
+    import torch
+    data, _, sizes, types, count = tensors._here()
+    _check(lib.mi_tensors_norm_sq_acc(data, sizes, types, count, _buf(result, 1, torch.float32),
+                                      _stream(stream)))
+
+
+def tensors_scale(tensors, scale, stream=None):
+    """Every tensor of a TensorList times the device scalar, in place or into its outs."""
+    import torch
+    _check(lib.mi_tensors_scale(*tensors._here(), _buf(scale, 1, torch.float32),
+                                _stream(stream)))
+
+
+def tensors_clip(tensors, max_norm, norm_sq, clip_scale, stream=None):
+    """Clips a TensorList by its global norm: norm_sq and clip_scale are overwritten, then every
+    tensor is scaled, in place or into its outs."""
+    import torch
+    _check(lib.mi_tensors_clip(*tensors._here(), max_norm, _buf(norm_sq, 1, torch.float32),
+                               _buf(clip_scale, 1, torch.float32), _stream(stream)))
+
+
 # ----- mixture of experts ----------------------------------------------------------
 
 def moe_gate_forward(logits, ids, weights, tokens, experts, k, renormalise=True, type=None,
@@ -583,6 +761,36 @@ def moe_gate_backward(logits, ids, weights, dweights, dlogits, tokens, experts, 
                                     _buf(dweights, tokens * k, torch.float32),
                                     _buf(dlogits, tokens * experts, _row_dtype(t)), tokens,
                                     experts, k, int(renormalise), t, _stream(stream)))
+
+
+def moe_balance_forward(logits, ids, valid, counts, probs, loss, tokens, experts, k, coef,
+                        type=None, stream=None):
+    """The router's balance loss: counts [experts + 1] (int32; the slots of each expert and the
+    number of valid tokens), probs [experts] (their mean probabilities) and the loss.  valid
+    (uint8 or bool, a byte a token, None: all) leaves padding out."""
+    import torch
+    t = _type_of(logits, type)
+    _check(lib.mi_moe_balance_forward(_buf(logits, tokens * experts, _row_dtype(t)),
+                                      _buf(ids, tokens * k, torch.int32),
+                                      _buf(valid, tokens, torch.uint8, torch.bool),
+                                      _buf(counts, experts + 1, torch.int32),
+                                      _buf(probs, experts, torch.float32),
+                                      _buf(loss, 1, torch.float32), tokens, experts, k, coef, t,
+                                      _stream(stream)))
+
+
+def moe_balance_backward(logits, valid, counts, dloss, dlogits, tokens, experts, k, coef,
+                         accumulate=True, type=None, stream=None):
+    """The loss's gradient times dloss (a device scalar; None: 1), added to dlogits
+    (accumulate) or written to it."""
+    import torch
+    t = _type_of(dlogits, type)
+    _check(lib.mi_moe_balance_backward(_buf(logits, tokens * experts, _row_dtype(t)),
+                                       _buf(valid, tokens, torch.uint8, torch.bool),
+                                       _buf(counts, experts + 1, torch.int32),
+                                       _buf(dloss, 1, torch.float32),
+                                       _buf(dlogits, tokens * experts, _row_dtype(t)), tokens,
+                                       experts, k, coef, int(accumulate), t, _stream(stream)))
 
 
 def moe_sort(ids, offsets, order, position, slots, experts, stream=None):

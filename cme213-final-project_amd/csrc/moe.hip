@@ -14,14 +14,13 @@
 #include <utility>
 
 #include "mi_common.hpp"
+#include "mi_logits.hpp"
 #include "mi_rowtype.hpp"
 
 namespace mi {
 
 namespace {
 
-constexpr int kMaxExperts = 1024;
-constexpr int kMaxChoices = 16;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxGrid = 1 << 20;  // workgroups over the tokens, which are taken in strides
@@ -45,7 +44,6 @@ constexpr int kMaxCols = 1 << 22;  // keeps a row's segments in the grid's secon
 // there, and 6.9 instead of 4.3 for 1024 rows.
 // ---------------------------------------------------------------------------
 constexpr int kNoKey = static_cast<int>(0xff800000u ^ 0x7fffffffu);  // of -inf
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ int order_key(float f) {
     const int b = __float_as_int(f + 0.0f);
@@ -56,44 +54,6 @@ __device__ __forceinline__ int order_key(float f) {
 // The logit of a key (NaN for NaN's key).
 __device__ __forceinline__ float key_value(int key) {
     return __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
-}
-
-// A lane's logits of a row: P, in pieces of one access that it takes in turn with the row's
-// other lanes.  Their experts are gl * N, N = kPiece, and the steps that step_expert gives.
-template <int T, int P>
-constexpr int kPiece = P < row_vec<T>() ? P : row_vec<T>();
-
-template <int T, int L, int P>
-constexpr int step_expert(int p) {
-    constexpr int N = kPiece<T, P>;
-    return p / N * (N * L) + p % N;
-}
-
-// Loads them, -inf behind the last expert.  Accesses may run into the next row, and are
-// cut to single elements only at the tensor's end.
-template <int T, int L, int P>
-__device__ __forceinline__ void load_logits(const void* logits, size_t row, size_t rows, int gl,
-                                            int experts, float (&v)[P]) {
-    constexpr int N = kPiece<T, P>;
-    const size_t base = row * experts, total = rows * experts;
-#pragma unroll
-    for (int c = 0; c < P; c += N) {
-        const int e0 = gl * N + step_expert<T, L, P>(c);
-        float part[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) part[e] = 0.0f;
-        if (e0 < experts) {
-            if (base + e0 + N <= total) {
-                row_get_n<T, N>(logits, base + e0, part);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e0 + e < experts) part[e] = row_get<T>(logits, base + e0 + e);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[c + e] = e0 + e < experts ? part[e] : -__builtin_inff();
-    }
 }
 
 template <int CTRL>
@@ -324,30 +284,6 @@ __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(
             }
         }
     }
-}
-
-// f(L, P): 16 lanes a row up to 256 experts, 64 lanes above; where `wide`, 16 up to 512.
-template <bool MAY_BE_WIDE, class F>
-void with_gate_shape(int experts, bool wide, F f) {
-    using std::integral_constant;
-    if constexpr (MAY_BE_WIDE) {
-        if (wide && experts > 256 && experts <= 512)
-            return f(integral_constant<int, 16>(), integral_constant<int, 32>());
-    }
-    if (experts <= 16)
-        f(integral_constant<int, 16>(), integral_constant<int, 1>());
-    else if (experts <= 32)
-        f(integral_constant<int, 16>(), integral_constant<int, 2>());
-    else if (experts <= 64)
-        f(integral_constant<int, 16>(), integral_constant<int, 4>());
-    else if (experts <= 128)
-        f(integral_constant<int, 16>(), integral_constant<int, 8>());
-    else if (experts <= 256)
-        f(integral_constant<int, 16>(), integral_constant<int, 16>());
-    else if (experts <= 512)
-        f(integral_constant<int, 64>(), integral_constant<int, 8>());
-    else
-        f(integral_constant<int, 64>(), integral_constant<int, 16>());
 }
 
 unsigned gate_grid(int tokens, int lanes) {
@@ -923,21 +859,6 @@ int combine_waves(int tokens, int k, int chunks, bool in_place, bool ragged) {
     if (in_place && ragged && (chunks - 1) % kWave == 0) return 1;
     if (tokens < 512 && chunks > 4 * kWave && k <= 8) return 16;
     return chunks >= 4 * kWave || (tokens < 512 && chunks > kWave) ? 4 : 1;
-}
-
-int check_gate_args(const char* name, int tokens, int experts, int k, int type) {
-    if (tokens < 0 || experts < 1 || experts > kMaxExperts || k < 1 || k > kMaxChoices ||
-        k > experts)
-        return set_error(MI_ERR_INVALID_ARG,
-                         "%s: invalid shape tokens=%d experts=%d k=%d (experts is 1 to %d, k 1 to "
-                         "%d and at most experts)",
-                         name, tokens, experts, k, kMaxExperts, kMaxChoices);
-    if (static_cast<long long>(tokens) * k > INT_MAX)
-        return set_error(MI_ERR_INVALID_ARG, "%s: tokens * k = %lld slots exceed an int", name,
-                         static_cast<long long>(tokens) * k);
-    if (!row_type_ok(type))
-        return set_error(MI_ERR_INVALID_ARG, "%s: unknown type %d", name, type);
-    return MI_OK;
 }
 
 }  // namespace

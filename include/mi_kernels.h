@@ -140,6 +140,53 @@ int mi_layernorm_backward_noalloc(const float* grad_out, const float* x,
                                   float* dgamma, float* dbeta,
                                   int rows, int cols, void* stream);
 
+/* ----- RMS norm ------------------------------------------------------------ */
+/* Beside the LayerNorm calls above; the reference has no RMS norm.  With h = x, or
+ * a + b, and r = 1 / sqrt(mean(h^2) + eps) per row:  out = h r gamma.  Rows are fp32,
+ * fp16 or bf16 (`type`, MI_TYPE_* below), passed as void*; gamma, inv_rms (r) and dgamma
+ * are fp32.  Everything is computed in fp32, the squares' sum too (it has to stay in that
+ * range), and rounded to its type at the end; out is that of the unrounded sum a + b, residual_out the rounded
+ * sum.  cols is 1 to 2^24, eps finite and not negative; no alignment beyond the element's is
+ * needed.  inv_rms may be NULL.  out may be x, residual_out may be a or b; other buffers must
+ * not overlap.  Every result is the same bits on every call. */
+int mi_rmsnorm_forward(const void* x, const float* gamma, void* out, float* inv_rms, int rows,
+                       int cols, float eps, int type, void* stream);
+int mi_residual_rmsnorm_forward(const void* a, const void* b, const float* gamma,
+                                void* residual_out, void* out, float* inv_rms, int rows, int cols,
+                                float eps, int type, void* stream);
+
+/* The same with y = h r gamma in 8 bits, for a product that takes scaled operands: q [rows,
+ * cols] (bytes) holds the codes of y / s, s the fp32 scale that a row's columns share
+ * (block = 0: scales is [rows]) or that 128 consecutive ones do (block = MI_ROW8_BLOCK:
+ * [rows, ceil(cols / 128)], the last one of what is left).  With m the largest magnitude among
+ * them, and no less than 2^-100:
+ *   MI_ROW8_INT8: s = m / 127, code = the integer nearest to y 127 / m;
+ *   MI_ROW8_E4M3: s = m / 448, code = the OCP e4m3 number nearest to y 448 / m.
+ * Half values round to even.  Where a NaN or an infinity is among them, s is NaN and the codes
+ * are 0.  out (y as rows; NULL: not wanted) may be x. */
+#define MI_ROW8_BLOCK 128
+#define MI_ROW8_INT8 0
+#define MI_ROW8_E4M3 1
+int mi_rmsnorm_forward_row8(const void* x, const float* gamma, void* q, float* scales, void* out,
+                            float* inv_rms, int rows, int cols, float eps, int block, int format,
+                            int type, void* stream);
+int mi_residual_rmsnorm_forward_row8(const void* a, const void* b, const float* gamma,
+                                     void* residual_out, void* q, float* scales, void* out,
+                                     float* inv_rms, int rows, int cols, float eps, int block,
+                                     int format, int type, void* stream);
+
+/* With n = x inv_rms and g = grad_out gamma:  dx = inv_rms (g - n mean(g n)), in grad_x
+ * (overwritten; it may be grad_out) or added to grad_residual;  dgamma += sum over the rows of
+ * grad_out n (fp32, deterministic, through the library workspace).  x is the forward call's
+ * x or residual_out. */
+int mi_rmsnorm_backward(const void* grad_out, const void* x, const float* inv_rms,
+                        const float* gamma, void* grad_x, float* dgamma, int rows, int cols,
+                        int type, void* stream);
+int mi_rmsnorm_backward_residual(const void* grad_out, const void* x, const float* inv_rms,
+                                 const float* gamma, void* grad_residual, float* dgamma, int rows,
+                                 int cols, int type, void* stream);
+size_t mi_rmsnorm_backward_workspace(int rows, int cols, int type);
+
 /* ----- residual / bias / ReLU ------------------------------------------- */
 
 /* out = a + b over n elements; out may alias a or b.  Replaces residual_add
@@ -302,6 +349,35 @@ int mi_adam_update(float* param, const float* grad, float* m, float* v, long lon
 /* Workspace bytes mi_buffer_norm_sq_acc / mi_adam_update need for n floats. */
 size_t mi_norm_sq_workspace(long long n);
 
+/* ----- gradients in many tensors ------------------------------------------- */
+/* A model's gradients as `count` tensors: tensors[i] points to sizes[i] elements of types[i]
+ * (MI_TYPE_* below; types NULL: all fp32).  tensors, outs, sizes and types are host arrays,
+ * read before the call returns; their entries are baked into a captured graph.  A tensor of
+ * no elements may be NULL.  No alignment beyond the element's is needed.  Squares and sums are
+ * formed in fp32, and the last sum in 64 bits, in an order fixed by the sizes and types. */
+
+/* *d_result += sum of all elements' squares (fp32). */
+int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, const int* types,
+                           int count, float* d_result, void* stream);
+
+/* Every element times *d_scale: in place, rounded to its type (outs NULL; nothing is read
+ * or written where the scale is 1), or as fp32 in outs[i] (e.g. pieces of the flat buffer that
+ * mi_adam_clipped takes).  Tensors to be scaled in place must not overlap each other, outs
+ * neither each other nor the tensors. */
+int mi_tensors_scale(const void* const* tensors, void* const* outs, const long long* sizes,
+                     const int* types, int count, const float* d_scale, void* stream);
+
+/* Clipping by the global norm: *d_norm_sq = sum of all elements' squares (overwritten),
+ * *d_clip_scale as mi_compute_clip_scale's, then mi_tensors_scale with it.  An infinite norm
+ * gives the scale 0, a NaN the scale 1, as there. */
+int mi_tensors_clip(const void* const* tensors, void* const* outs, const long long* sizes,
+                    const int* types, int count, float max_norm, float* d_norm_sq,
+                    float* d_clip_scale, void* stream);
+
+/* Workspace bytes mi_tensors_norm_sq_acc / mi_tensors_clip need, at most, for `count`
+ * tensors. */
+size_t mi_tensors_workspace(int count);
+
 /* ----- 16-bit activation storage ----------------------------------------- */
 /* Half buffers hold IEEE binary16 values, bf16 buffers the upper 16 bits of
  * fp32; both are passed as void* (2 bytes per element).  Conversions round
@@ -368,6 +444,26 @@ int mi_moe_gate_forward(const void* logits, int* ids, float* weights, int tokens
 int mi_moe_gate_backward(const void* logits, const int* ids, const float* weights,
                          const float* dweights, void* dlogits, int tokens, int experts, int k,
                          int renormalise, int type, void* stream);
+
+/* The router's balance loss.  Of the tokens with valid[t] != 0 (bytes; NULL: all), n in number:
+ * counts[e] = their slots with id e (slots with an id outside [0, experts) are not counted) and
+ * counts[experts] = n; probs[e] = the mean of their p_te, the softmax of their logits over all
+ * experts (0 for a row of -inf alone); *loss = coef experts / (k n) sum_e counts[e] probs[e],
+ * 0 where n is 0.  counts is [experts + 1].  All three are overwritten; sums over the tokens
+ * are formed in fp32 in a fixed order, through the library workspace. */
+int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned char* valid,
+                           int* counts, float* probs, float* loss, int tokens, int experts, int k,
+                           float coef, int type, void* stream);
+
+/* The loss's gradient times *dloss (device; NULL: 1):
+ * dlogits[t, e] = dloss coef experts / (k n^2) p_te (counts[e] - sum_f p_tf counts[f]), with
+ * counts as the forward call wrote them, or summed over several processes.  accumulate != 0:
+ * added to what dlogits holds (as mi_moe_gate_backward left it), else dlogits is overwritten,
+ * with 0 where a token is not valid. */
+int mi_moe_balance_backward(const void* logits, const unsigned char* valid, const int* counts,
+                            const float* dloss, void* dlogits, int tokens, int experts, int k,
+                            float coef, int accumulate, int type, void* stream);
+size_t mi_moe_balance_workspace(int tokens, int experts);
 
 /* Sorts `slots` expert ids, stably.  offsets [experts + 1]: expert e's rows are
  * offsets[e] .. offsets[e + 1] - 1; position [slots]: the row of each slot, -1
