@@ -20,10 +20,12 @@ namespace mi {
 
 namespace {
 
-constexpr int kFwdThreads = 512;
+constexpr int kFwdThreads = 1024;
 constexpr int kFwdBlocks = 256;
-constexpr int kOneTokens = 256;  // tokens of a call that one workgroup does alone
+constexpr int kOneTrips = 4;  // rows of a lane group in a call that one workgroup does alone
 constexpr int kFinThreads = 1024;
+constexpr int kFinExperts = 16;  // experts of a workgroup that adds partial rows
+constexpr int kFinSlices = kFinThreads / kFinExperts;
 constexpr int kBwdThreads = 256;
 constexpr int kMaxGrid = 1 << 20;
 
@@ -46,26 +48,24 @@ __device__ __forceinline__ float softmax_terms(float (&v)[P]) {
     return s == 0.0f ? 0.0f : 1.0f / s;
 }
 
-// The loss from all experts' counts and mean probabilities, by a whole workgroup of NT
-// threads, in 64 bits.  Thread 0 has it.
-template <int NT>
-__device__ __forceinline__ float loss_of(const int* count, const float* prob, int experts, int k,
-                                         float coef, double* red) {
-    double s = 0.0;
-    for (int e = threadIdx.x; e < experts; e += NT)
-        s += static_cast<double>(count[e]) * static_cast<double>(prob[e]);
-    red[threadIdx.x] = s;
-    __syncthreads();
-#pragma unroll
-    for (int h = NT / 2; h >= 1; h /= 2) {
-        if (static_cast<int>(threadIdx.x) < h) red[threadIdx.x] += red[threadIdx.x + h];
-        __syncthreads();
-    }
-    const int n = count[experts];
+// sum c_e P_e to the loss.
+__device__ __forceinline__ float loss_of(double sum, int experts, int k, int n, float coef) {
     return n == 0 ? 0.0f
-                  : static_cast<float>(red[0] * static_cast<double>(coef) * experts /
+                  : static_cast<float>(sum * static_cast<double>(coef) * experts /
                                        (static_cast<double>(k) * n));
 }
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) v += __shfl_xor(v, m);
+    return v;
+}
+
+// What the workgroups that add partial rows leave for the last of them.
+struct Finish {
+    double sum[kMaxExperts / kFinExperts];
+    unsigned done;
+};
 
 // Sums of the probabilities and counts over a workgroup's tokens: a lane adds its experts'
 // over its rows in registers, the waves' sums meet in LDS, in order.  ONE: the only
@@ -74,15 +74,17 @@ template <int T, int L, int P, bool ONE>
 __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids, int tokens, int experts, int k,
     const unsigned char* __restrict__ valid, float* __restrict__ part, int* __restrict__ part_n,
-    int* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss, float coef) {
+    Finish* __restrict__ finish, int* __restrict__ counts, float* __restrict__ probs,
+    float* __restrict__ loss, float coef) {
     constexpr int PER = kFwdThreads / L, WAVES = kFwdThreads / kWave;
     constexpr int N = kPiece<T, P>;
-    __shared__ __align__(16) float sums[WAVES][L * P];
+    constexpr int SLOTS = L * P > 512 ? WAVES / 2 : WAVES;  // 32 KB of sums at most
+    __shared__ __align__(16) float sums[SLOTS][L * P];
     __shared__ int count[kMaxExperts + 1];
-    [[maybe_unused]] __shared__ double red[ONE ? kFwdThreads : 1];
-    const int gl = threadIdx.x & (L - 1);
+    const int gl = threadIdx.x & (L - 1), lane = threadIdx.x & (kWave - 1);
     const int wave = threadIdx.x / kWave;
     for (int e = threadIdx.x; e <= experts; e += kFwdThreads) count[e] = 0;
+    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) finish->done = 0;
     __syncthreads();
     float acc[P];
 #pragma unroll
@@ -93,98 +95,155 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
         const size_t row = want < tokens ? static_cast<size_t>(want)
                                          : static_cast<size_t>(tokens) - 1;
         const bool live = want < tokens && (!valid || valid[row] != 0);
-        const int id = live && gl < k ? ids[row * k + gl] : -1;
+        const int id = want < tokens && gl < k ? ids[row * k + gl] : -1;
         float v[P];
         load_logits<T, L, P>(logits, row, tokens, gl, experts, v);
         const float inv = softmax_terms<L, P>(v);
 #pragma unroll
         for (int p = 0; p < P; ++p) acc[p] += live ? v[p] * inv : 0.0f;
-        if (id >= 0 && id < experts) atomicAdd(&count[id], 1);
-        if (live && gl == 0) atomicAdd(&count[experts], 1);
+        if (live && id >= 0 && id < experts) atomicAdd(&count[id], 1);
+        const unsigned long long rows = __ballot(live && gl == 0);
+        if (lane == 0 && rows) atomicAdd(&count[experts], __popcll(rows));
     }
     // the wave's rows, then the waves
+    if constexpr (L == 16) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        if constexpr (L == 16) {
+        for (int p = 0; p < P; ++p) {
             acc[p] += __shfl_xor(acc[p], 16);
             acc[p] += __shfl_xor(acc[p], 32);
         }
-        if ((threadIdx.x & (kWave - 1)) < L)
-            sums[wave][gl * N + step_expert<T, L, P>(p)] = acc[p];
+    }
+    auto put = [&](int slot) {
+        if (lane < L) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) sums[slot][gl * N + step_expert<T, L, P>(p)] = acc[p];
+        }
+    };
+    if constexpr (SLOTS < WAVES) {
+        if (wave >= SLOTS) put(wave - SLOTS);
+        __syncthreads();
+        if (wave < SLOTS) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                acc[p] += sums[wave][gl * N + step_expert<T, L, P>(p)];
+        }
+        if (wave < SLOTS) put(wave);
+    } else {
+        put(wave);
     }
     __syncthreads();
-    [[maybe_unused]] const float n = static_cast<float>(max(count[experts], 1));
-    for (int e = threadIdx.x; e < experts; e += kFwdThreads) {
-        float s = sums[0][e];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += sums[w][e];
-        if constexpr (ONE) {
-            sums[0][e] = s / n;
-            probs[e] = s / n;
-            counts[e] = count[e];
-        } else {
-            part[static_cast<size_t>(blockIdx.x) * experts + e] = s;
-            part_n[static_cast<size_t>(blockIdx.x) * (experts + 1) + e] = count[e];
-        }
-    }
     if constexpr (ONE) {
-        __syncthreads();
-        const float l = loss_of<kFwdThreads>(count, sums[0], experts, k, coef, red);
-        if (threadIdx.x == 0) {
-            *loss = l;
-            counts[experts] = count[experts];
+        __shared__ double red[WAVES];
+        const int n = count[experts];
+        double s = 0.0;
+        for (int e = threadIdx.x; e < experts; e += kFwdThreads) {
+            float p = sums[0][e];
+#pragma unroll
+            for (int w = 1; w < SLOTS; ++w) p += sums[w][e];
+            p /= static_cast<float>(max(n, 1));
+            probs[e] = p;
+            counts[e] = count[e];
+            s += static_cast<double>(count[e]) * static_cast<double>(p);
         }
-    } else if (threadIdx.x == 0) {
-        part_n[static_cast<size_t>(blockIdx.x) * (experts + 1) + experts] = count[experts];
+        s = wave_sum_d(s);
+        if (lane == 0) red[wave] = s;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) s += red[w];
+            *loss = loss_of(s, experts, k, n, coef);
+            counts[experts] = n;
+        }
+    } else {
+        for (int e = threadIdx.x; e < experts; e += kFwdThreads) {
+            float s = sums[0][e];
+#pragma unroll
+            for (int w = 1; w < SLOTS; ++w) s += sums[w][e];
+            part[static_cast<size_t>(blockIdx.x) * experts + e] = s;
+        }
+        for (int e = threadIdx.x; e <= experts; e += kFwdThreads)
+            part_n[static_cast<size_t>(blockIdx.x) * (experts + 1) + e] = count[e];
     }
 }
 
-// Adds the partial rows, in slices of them side by side, each in order.
+// Adds the partial rows: a workgroup has 16 experts, 64 slices of the rows side by side, each in
+// order, then added pairwise.  The workgroup that ends last adds all workgroups' sums of c_e P_e,
+// in order, whichever it is.
 __global__ __launch_bounds__(kFinThreads) void balance_finish_kernel(
     const float* __restrict__ part, const int* __restrict__ part_n, int blocks, int experts, int k,
-    float coef, int* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss) {
-    __shared__ float prob[kFinThreads];
-    __shared__ int count[kFinThreads + 1];
+    float coef, int* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss,
+    Finish* finish) {
+    constexpr int TRIPS = kFwdBlocks / kFinSlices;
+    __shared__ float sum[kFinSlices][kFinExperts];
+    __shared__ int count[kFinSlices][kFinExperts];
     __shared__ int total;
-    __shared__ double red[kFinThreads];
-    int width = 1;
-    while (width < experts) width *= 2;
-    const int slices = kFinThreads / width;
-    const int e = threadIdx.x & (width - 1), slice = threadIdx.x / width;
-    float s = 0.0f;
-    int c = 0;
+    const int col = threadIdx.x & (kFinExperts - 1), slice = threadIdx.x / kFinExperts;
+    const int e = blockIdx.x * kFinExperts + col;
     if (threadIdx.x == 0) total = 0;
-    if (e < experts) {
-        for (int b = slice; b < blocks; b += slices) {
-            s += part[static_cast<size_t>(b) * experts + e];
-            c += part_n[static_cast<size_t>(b) * (experts + 1) + e];
-        }
+    const int rows = static_cast<int>(threadIdx.x) < blocks
+                         ? part_n[static_cast<size_t>(threadIdx.x) * (experts + 1) + experts]
+                         : 0;
+    float p[TRIPS];
+    int c[TRIPS];
+#pragma unroll
+    for (int i = 0; i < TRIPS; ++i) {
+        const int b = slice + i * kFinSlices;
+        const bool there = b < blocks && e < experts;
+        p[i] = there ? part[static_cast<size_t>(b) * experts + e] : 0.0f;
+        c[i] = there ? part_n[static_cast<size_t>(b) * (experts + 1) + e] : 0;
     }
-    prob[threadIdx.x] = s;
-    count[threadIdx.x] = c;
-    __syncthreads();
-    int n = 0;
-    for (int b = threadIdx.x; b < blocks; b += kFinThreads)
-        n += part_n[static_cast<size_t>(b) * (experts + 1) + experts];
-    if (n) atomicAdd(&total, n);
-    if (slice == 0 && e < experts)
-        for (int i = 1; i < slices; ++i) {
-            s += prob[i * width + e];
-            c += count[i * width + e];
-        }
-    __syncthreads();
-    n = total;
-    if (slice == 0 && e < experts) {
-        prob[e] = s / static_cast<float>(max(n, 1));
-        count[e] = c;
-        probs[e] = prob[e];
-        counts[e] = c;
+#pragma unroll
+    for (int i = 1; i < TRIPS; ++i) {
+        p[0] += p[i];
+        c[0] += c[i];
     }
-    if (threadIdx.x == 0) count[experts] = counts[experts] = n;
+    sum[slice][col] = p[0];
+    count[slice][col] = c[0];
     __syncthreads();
-    const float l = loss_of<kFinThreads>(count, prob, experts, k, coef, red);
-    if (threadIdx.x == 0) *loss = l;
+    if (rows) atomicAdd(&total, rows);
+#pragma unroll
+    for (int h = kFinSlices / 2; h >= 1; h /= 2) {
+        if (slice < h) {
+            sum[slice][col] += sum[slice + h][col];
+            count[slice][col] += count[slice + h][col];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x >= kWave) return;
+    const int n = total;
+    double s = 0.0;
+    if (threadIdx.x < kFinExperts && e < experts) {
+        const float mean = sum[0][col] / static_cast<float>(max(n, 1));
+        probs[e] = mean;
+        counts[e] = count[0][col];
+        s = static_cast<double>(count[0][col]) * static_cast<double>(mean);
+    }
+    s = wave_sum_d(s);
+    if (gridDim.x > 1) {
+        unsigned before = 0;
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(&finish->sum[blockIdx.x], s, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+            before = __hip_atomic_fetch_add(&finish->done, 1u, __ATOMIC_ACQ_REL,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(before))) !=
+            gridDim.x - 1)
+            return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        s = threadIdx.x < gridDim.x
+                ? __hip_atomic_load(&finish->sum[threadIdx.x], __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT)
+                : 0.0;
+        s = wave_sum_d(s);
+    }
+    if (threadIdx.x == 0) {
+        *loss = loss_of(s, experts, k, n, coef);
+        counts[experts] = n;
+    }
 }
+static_assert(kMaxExperts / kFinExperts <= kWave && kFwdBlocks <= kFinThreads,
+              "a lane for each workgroup's sum, a thread for each partial row");
 
 // The counts enter less a whole number near their mean, which changes nothing (the p of a row
 // add up to 1) and keeps the bits of what is left.
@@ -256,10 +315,14 @@ __global__ __launch_bounds__(kBwdThreads) void balance_bwd_kernel(
 }
 
 int fwd_blocks(int tokens, int experts) {
-    if (tokens <= kOneTokens) return 1;
     const int per = kFwdThreads / (experts <= 256 ? 16 : 64);
+    if (tokens <= kOneTrips * per) return 1;
     return static_cast<int>(
         std::min<long long>((static_cast<long long>(tokens) + per - 1) / per, kFwdBlocks));
+}
+
+size_t partial_bytes(int blocks, int experts) {
+    return static_cast<size_t>(blocks) * (2 * static_cast<size_t>(experts) + 1) * sizeof(float);
 }
 
 }  // namespace
@@ -270,9 +333,11 @@ using namespace mi;
 extern "C" {
 
 size_t mi_moe_balance_workspace(int tokens, int experts) {
-    if (tokens <= kOneTokens || experts <= 0) return 0;
-    return colsum_part_offset() + static_cast<size_t>(fwd_blocks(tokens, experts)) *
-                                      (2 * static_cast<size_t>(experts) + 1) * sizeof(float);
+    if (tokens <= 0 || experts <= 0) return 0;
+    const int blocks = fwd_blocks(tokens, experts);
+    return blocks == 1 ? 0
+                       : colsum_part_offset() + round_up(sizeof(Finish), 256) +
+                             partial_bytes(blocks, experts);
 }
 
 int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned char* valid,
@@ -284,6 +349,7 @@ int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned ch
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     hipStream_t st = to_stream(stream);
     const int blocks = fwd_blocks(tokens, experts);
+    Finish* finish = nullptr;
     float* part = nullptr;
     int* part_n = nullptr;
     if (blocks > 1) {
@@ -291,7 +357,8 @@ int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned ch
         char* ws = static_cast<char*>(
             workspace_get(mi_moe_balance_workspace(tokens, experts), st, &err));
         if (!ws) return err;
-        part = reinterpret_cast<float*>(ws + colsum_part_offset());
+        finish = reinterpret_cast<Finish*>(ws + colsum_part_offset());
+        part = reinterpret_cast<float*>(ws + colsum_part_offset() + round_up(sizeof(Finish), 256));
         part_n = reinterpret_cast<int*>(part + static_cast<size_t>(blocks) * experts);
     }
     with_row_type(type, [&](auto t) {
@@ -300,14 +367,16 @@ int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned ch
             with_flag(blocks == 1, [&](auto one) {
                 hipLaunchKernelGGL((balance_fwd_kernel<T, L, P, decltype(one)::value>),
                                    dim3(blocks), dim3(kFwdThreads), 0, st, logits, ids, tokens,
-                                   experts, k, valid, part, part_n, counts, probs, loss, coef);
+                                   experts, k, valid, part, part_n, finish, counts, probs, loss,
+                                   coef);
             });
         });
     });
     if (int rc = check_launch(name)) return rc;
     if (blocks == 1) return MI_OK;
-    hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(kFinThreads), 0, st, part, part_n,
-                       blocks, experts, k, coef, counts, probs, loss);
+    hipLaunchKernelGGL(balance_finish_kernel, dim3((experts + kFinExperts - 1) / kFinExperts),
+                       dim3(kFinThreads), 0, st, part, part_n, blocks, experts, k, coef, counts,
+                       probs, loss, finish);
     return check_launch(name);
 }
 

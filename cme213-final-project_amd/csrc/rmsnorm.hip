@@ -1,600 +1,25 @@
-// Root-mean-square norm forward / backward for gfx950, with the residual's
-// addition and with an output in 8 bits.  Beside the LayerNorm of
-// FINAL_CLEAN_CODE/src/kernels/layernorm.cu:10-308 (its fused residual form and
-// its backward into the residual stream's gradient); the reference has no RMS
-// norm.  Rows are fp32, fp16 or bf16; gamma, statistics and sums fp32.
-//
-//   h = a + b (or x);  r = 1 / sqrt(mean(h^2) + eps);  y = h r gamma
-//   dx = r (g - n mean(g n)),  n = h r,  g = dy gamma;  dgamma += sum_rows dy n
-//
-// A group of GT threads (a part of a wave, a wave, or several) holds a row in
-// registers, in units of 16 bytes that its threads take in turn, so a row is
-// read once.  The last unit of a row that is no whole number of them begins
-// early, at the row's last 16 bytes: the elements that it shares with the unit
-// before it count once in the sums, and are written twice with the same bits.
-// Rows of less than one unit, and rows too long for registers, are walked twice.
-//
-// y is computed from the unrounded sum a + b; the rounded one is what is kept
-// for the backward pass, with r as it was.  An output is rounded to its type from
-// its fp32 value (`rounded`: or the compiler may join the last product with its
-// conversion to fp16 in one of two threads that write the same element).
-#include <algorithm>
-#include <climits>
-#include <type_traits>
-
-#include "mi_common.hpp"
+// Entry points of the RMS norm calls: their checks, the backward pass's workspace and the sum of
+// its partial rows.  The kernels are in mi_rmsnorm_kernels.hpp.
+#include "mi_rmsnorm.hpp"
 #include "mi_rowtype.hpp"
 
 namespace mi {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxGrid = 1 << 20;  // workgroups over the rows, which are taken in strides
 constexpr int kMaxCols = 1 << 24;
-constexpr int kFewRows = 1024;
-constexpr float kLeast = 0x1p-100f;  // a row or block counts as at least this large
 
-template <int GT>
-constexpr int kGroupThreads = GT > kThreads ? GT : kThreads;
-
-// The unit that thread t of a row's group has in step k: where it begins, and how many of its
-// first elements belong to another unit (all of them behind the row's end).
-template <int V>
-struct UnitAt {
-    int col, skip;
-};
-
-template <int V>
-__device__ __forceinline__ UnitAt<V> unit_at(int j, int units, int cols) {
-    const int shared = units * V - cols;
-    return {min(j * V, cols - V), j < units - 1 ? 0 : j == units - 1 ? shared : V};
+int check_rows(const char* name, int rows, int cols, int type) {
+    if (rows < 0 || cols < 1 || cols > kMaxCols)
+        return set_error(MI_ERR_INVALID_ARG, "%s: invalid shape rows=%d cols=%d (cols is 1 to %d)",
+                         name, rows, cols, kMaxCols);
+    if (!row_type_ok(type)) return set_error(MI_ERR_INVALID_ARG, "%s: type=%d", name, type);
+    return MI_OK;
 }
-
-template <int T>
-__device__ __forceinline__ const char* element_ptr(const void* p, size_t i) {
-    return static_cast<const char*>(p) + i * sizeof(row_elem<T>);
-}
-template <int T>
-__device__ __forceinline__ char* element_ptr(void* p, size_t i) {
-    return static_cast<char*>(p) + i * sizeof(row_elem<T>);
-}
-
-template <int V>
-__device__ __forceinline__ void load_gamma(const float* gamma, int col, float (&g)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-        const u32x4 w = load16b<false>(gamma + col + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) g[i + e] = __uint_as_float(w[e]);
-    }
-}
-
-__device__ __forceinline__ unsigned larger(unsigned v, unsigned w) { return v > w ? v : w; }
-
-// Largest of the L lanes (16, 32 or 64) around a lane, as unsigned integers:
-// the order of magnitudes, with infinities and NaN above all.
-template <int L>
-__device__ __forceinline__ unsigned lanes_max(unsigned v) {
-    auto step = [&](auto ctrl) {
-        v = larger(v, static_cast<unsigned>(dpp_move_i<decltype(ctrl)::value>(static_cast<int>(v))));
-    };
-    step(std::integral_constant<int, 0xB1>());
-    step(std::integral_constant<int, 0x4E>());
-    step(std::integral_constant<int, 0x141>());
-    step(std::integral_constant<int, 0x140>());
-    if constexpr (L >= 32) v = larger(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), 16)));
-    if constexpr (L >= 64) v = larger(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), 32)));
-    return v;
-}
-
-__device__ __forceinline__ unsigned magnitude(float v) {
-    return __float_as_uint(v) & 0x7fffffffu;
-}
-
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
-    if constexpr (L == 32) {
-        v = group_sum<16>(v);
-        return v + __shfl_xor(v, 16);
-    } else {
-        return group_sum<L>(v);
-    }
-}
-
-struct SumTop {
-    float sum;
-    unsigned top;
-};
-
-// Sum and largest over the GT threads of a row's group, in every one of them.  Groups of
-// several waves exchange through LDS; `turn` alternates between two places, so that the next
-// exchange's writes cannot meet this one's reads (a barrier lies between any two of the same
-// place).
-template <int GT>
-struct GroupRed {
-    static constexpr int kWavesOf = kGroupThreads<GT> / kWave;
-    SumTop (*red)[kWavesOf];
-    int turn = 0;
-
-    template <bool TOP>
-    __device__ __forceinline__ SumTop both(float sum, unsigned top) {
-        if constexpr (GT <= kWave) {
-            return {lanes_sum<GT>(sum), TOP ? lanes_max<GT>(top) : 0u};
-        } else {
-            sum = wave_sum(sum);
-            if constexpr (TOP) top = lanes_max<kWave>(top);
-            SumTop* r = red[turn];
-            turn ^= 1;
-            if ((threadIdx.x & (kWave - 1)) == 0) r[threadIdx.x / kWave] = {sum, top};
-            __syncthreads();
-            const int w0 = static_cast<int>(threadIdx.x) / GT * (GT / kWave);
-            SumTop t = r[w0];
-#pragma unroll
-            for (int i = 1; i < GT / kWave; ++i) {
-                t.sum += r[w0 + i].sum;
-                if constexpr (TOP) t.top = larger(t.top, r[w0 + i].top);
-            }
-            return t;
-        }
-    }
-    __device__ __forceinline__ float sum(float v) { return both<false>(v, 0u).sum; }
-    __device__ __forceinline__ unsigned max(unsigned v) { return both<true>(0.0f, v).top; }
-};
-
-// The scale of values v r (v = h gamma) whose largest magnitude of v has the bits `top`, and
-// what v is multiplied by (0 where one of them is no number: their codes are 0, the scale NaN).
-// r, the same for all of them, cancels in the codes and adds no rounding to them.
-struct Scale {
-    float scale, mul;
-};
-
-__device__ __forceinline__ Scale scale_of(unsigned top, float r, int format) {
-    const float largest = format == MI_ROW8_INT8 ? 127.0f : 448.0f;
-    const float v = __uint_as_float(top), m = v * r;
-    if (!(m < __builtin_inff())) return {__builtin_nanf(""), 0.0f};
-    if (m >= kLeast) return {m / largest, largest / v};
-    return {kLeast / largest, fminf(r * (largest / kLeast), 3.0e38f)};
-}
-
-// The codes of N values (4 or 8), the first in the lowest byte.  int8: adding 1.5 2^23
-// leaves rint(v mul) in the low bits of the sum, two's complement.
-template <int N>
-__device__ __forceinline__ uint64_t codes_of(const float (&v)[N], const Scale& s, int format) {
-    uint32_t q[2] = {0, 0};
-    if (s.mul != 0.0f) {
-#pragma unroll
-        for (int h = 0; h < N / 4; ++h) {
-            if (format == MI_ROW8_INT8) {
-                uint32_t b[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    b[e] = __float_as_uint(fmaf(v[4 * h + e], s.mul, 12582912.0f));
-                const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
-                const uint32_t hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
-                q[h] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-            } else {
-                int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h] * s.mul, v[4 * h + 1] * s.mul, 0,
-                                                        false);
-                w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * s.mul, v[4 * h + 3] * s.mul, w,
-                                                    true);
-                q[h] = static_cast<uint32_t>(w);
-            }
-        }
-    }
-    return static_cast<uint64_t>(q[1]) << 32 | q[0];
-}
-
-// A unit's codes without the `skip` first ones, to the place of the others.
-template <int V>
-__device__ __forceinline__ void store_codes(char* p, uint64_t q, int skip) {
-    if (skip == 0) {
-        if constexpr (V == 8)
-            store_piece(p, q);
-        else
-            store_piece(p, static_cast<uint32_t>(q));
-        return;
-    }
-    const int n = V - skip;
-    p += skip;
-    q >>= 8 * skip;
-    if (n & 4) {
-        store_piece(p, static_cast<uint32_t>(q));
-        p += 4;
-        q >>= 32;
-    }
-    if (n & 2) {
-        store_piece(p, static_cast<uint16_t>(q));
-        p += 2;
-        q >>= 16;
-    }
-    if (n & 1) store_piece(p, static_cast<uint8_t>(q));
-}
-
-// ---------------------------------------------------------------------------
-// Forward: one row a group at a time.  out may be a (without RESID), residual_out
-// a or b: a row's loads all end before its first store.
-// ---------------------------------------------------------------------------
-enum class Out { Rows, Row8, Block8 };  // rows; 8 bits with a scale a row, or 128 columns
-
-template <int T, int GT, int N, bool RESID, Out OUT>
-__global__ __launch_bounds__(kGroupThreads<GT>) void rms_fwd_kernel(
-    int rows, int cols, const void* a, const void* b, const float* __restrict__ gamma,
-    void* residual_out, void* out, float eps, float* __restrict__ inv_rms, char* __restrict__ q,
-    float* __restrict__ scales, int format, bool nt) {
-    constexpr bool Q8 = OUT != Out::Rows;
-    constexpr int V = row_vec<T>();
-    constexpr int PER = kGroupThreads<GT> / GT;
-    __shared__ SumTop red[2][GroupRed<GT>::kWavesOf];
-    GroupRed<GT> group{red};
-    const int t = threadIdx.x & (GT - 1);
-    const int units = (cols + V - 1) / V;
-    for (long long row0 = static_cast<long long>(blockIdx.x) * PER; row0 < rows;
-         row0 += static_cast<long long>(gridDim.x) * PER) {
-        const long long want = row0 + threadIdx.x / GT;
-        const bool valid = want < rows;  // the others repeat the last row and store nothing
-        const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(rows) - 1;
-        const size_t base = row * cols;
-        UnitAt<V> at[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) at[k] = unit_at<V>(t + k * GT, units, cols);
-
-        u32x4 x[N];
-        [[maybe_unused]] u32x4 y[N];
-        auto load = [&](auto stream) {
-            constexpr bool NT = decltype(stream)::value;
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                x[k] = load16b<NT>(element_ptr<T>(a, base + at[k].col));
-                if constexpr (RESID) y[k] = load16b<NT>(element_ptr<T>(b, base + at[k].col));
-            }
-        };
-        if (nt)
-            load(std::true_type());
-        else
-            load(std::false_type());
-        float v[N][V];  // gamma, then h gamma
-#pragma unroll
-        for (int k = 0; k < N; ++k) load_gamma<V>(gamma, at[k].col, v[k]);
-        // Only the last step's units can be partial or behind the row's end.
-        float s = 0.0f;
-        unsigned row_top = 0;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int skip = k == N - 1 ? at[k].skip : 0;
-            float h[V];
-            row_unpack<T>(x[k], h);
-            if constexpr (RESID) {
-                float other[V];
-                row_unpack<T>(y[k], other);
-#pragma unroll
-                for (int e = 0; e < V; ++e) h[e] += other[e];
-                x[k] = row_pack<T>(h);  // as it is kept
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                v[k][e] *= h[e];
-                s += e < skip ? 0.0f : h[e] * h[e];
-                if constexpr (OUT == Out::Row8)
-                    row_top = larger(row_top, e < skip ? 0u : magnitude(v[k][e]));
-            }
-        }
-        const SumTop all = group.template both<OUT == Out::Row8>(s, row_top);
-        const float r = 1.0f / sqrtf(all.sum / static_cast<float>(cols) + eps);
-        wave_order();
-        if (valid && t == 0 && inv_rms) inv_rms[row] = r;
-
-        [[maybe_unused]] Scale sc{};
-        if constexpr (OUT == Out::Row8) {
-            sc = scale_of(all.top, r, format);
-            if (valid && t == 0) scales[row] = sc.scale;
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const bool stored = valid && (k < N - 1 || at[k].skip < V);
-            if constexpr (RESID) {
-                if (stored) store16b(element_ptr<T>(residual_out, base + at[k].col), x[k]);
-            }
-            if (!Q8 || out) {
-                float o[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = rounded(v[k][e] * r);
-                if (stored) store16b(element_ptr<T>(out, base + at[k].col), row_pack<T>(o));
-            }
-            if constexpr (Q8) {
-                if constexpr (OUT == Out::Block8) {
-                    constexpr int L = MI_ROW8_BLOCK / V;  // lanes that hold a block
-                    const int skip = k == N - 1 ? at[k].skip : 0, j = t + k * GT;
-                    unsigned top = 0;
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        top = larger(top, e < skip ? 0u : magnitude(v[k][e]));
-                    sc = scale_of(lanes_max<(L < GT ? L : GT)>(top), r, format);
-                    const int blocks = (cols + MI_ROW8_BLOCK - 1) / MI_ROW8_BLOCK;
-                    if (stored && j % L == 0) scales[row * blocks + j / L] = sc.scale;
-                }
-                const uint64_t codes = codes_of<V>(v[k], sc, format);
-                if (stored) store_codes<V>(q + base + at[k].col, codes, at[k].skip);
-            }
-        }
-    }
-}
-
-// Forward, rows of less than a unit or more than the registers hold: a workgroup a row,
-// which it walks twice.  A wave takes 128 columns at a time, the columns of a scale.
-template <int T, bool RESID, Out OUT>
-__global__ __launch_bounds__(kThreads) void rms_fwd_walk_kernel(
-    int rows, int cols, const void* a, const void* b, const float* __restrict__ gamma,
-    void* residual_out, void* out, float eps, float* __restrict__ inv_rms, char* __restrict__ q,
-    float* __restrict__ scales, int format) {
-    constexpr bool Q8 = OUT != Out::Rows;
-    __shared__ SumTop red[2][kThreads / kWave];
-    GroupRed<kThreads> group{red};
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-    const int blocks = (cols + MI_ROW8_BLOCK - 1) / MI_ROW8_BLOCK;
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        const size_t base = static_cast<size_t>(row) * cols;
-        auto value = [&](int c) {
-            float h = row_get<T>(a, base + c);
-            if constexpr (RESID) h += row_get<T>(b, base + c);
-            return h;
-        };
-        float s = 0.0f;
-        for (int c = threadIdx.x; c < cols; c += kThreads) {
-            const float h = value(c);
-            s += h * h;
-        }
-        const float r = 1.0f / sqrtf(group.sum(s) / static_cast<float>(cols) + eps);
-        Scale sc{};
-        if constexpr (OUT == Out::Row8) {
-            unsigned top = 0;
-            for (int c = threadIdx.x; c < cols; c += kThreads)
-                top = larger(top, magnitude(value(c) * gamma[c]));
-            sc = scale_of(group.max(top), r, format);
-            if (threadIdx.x == 0) scales[row] = sc.scale;
-        }
-        for (int i = wave; i < blocks; i += kThreads / kWave) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the first two are the lane's columns
-            unsigned top = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = i * MI_ROW8_BLOCK + e * kWave + lane;
-                if (c >= cols) continue;
-                const float h = value(c);
-                v[e] = h * gamma[c];
-                top = larger(top, magnitude(v[e]));
-                if constexpr (RESID) row_put<T>(residual_out, base + c, h);
-                if (!Q8 || out) row_put<T>(out, base + c, rounded(v[e] * r));
-            }
-            if constexpr (Q8) {
-                if constexpr (OUT == Out::Block8) {
-                    sc = scale_of(lanes_max<kWave>(top), r, format);
-                    if (lane == 0) scales[static_cast<size_t>(row) * blocks + i] = sc.scale;
-                }
-                const uint64_t codes = codes_of<4>(v, sc, format);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int c = i * MI_ROW8_BLOCK + e * kWave + lane;
-                    if (c < cols) q[base + c] = static_cast<char>(codes >> (8 * e));
-                }
-            }
-        }
-        if (threadIdx.x == 0 && inv_rms) inv_rms[row] = r;
-    }
-}
-
-// ---------------------------------------------------------------------------
-// Backward.  A group walks its rows, holding gamma and its columns' sums of
-// dgamma in registers; a workgroup's groups add theirs through LDS, in order, into
-// one partial row, and colsum_finalize adds the partial rows.
-// ---------------------------------------------------------------------------
-constexpr int kBwdThreads = 512;
-constexpr int kBwdBlocks = 256;
-
-template <int GT>
-constexpr int kBwdGroupThreads = GT > kBwdThreads ? GT : kBwdThreads;
-
-template <int T, int GT, int N, bool ADD>
-__global__ __launch_bounds__(kBwdGroupThreads<GT>) void rms_bwd_kernel(
-    int rows, int cols, const void* dy, const void* __restrict__ x,
-    const float* __restrict__ inv_rms, const float* __restrict__ gamma, void* dx,
-    float* __restrict__ part, bool nt) {
-    constexpr int V = row_vec<T>();
-    constexpr int WG = kBwdGroupThreads<GT>;
-    constexpr int PER = WG / GT;
-    extern __shared__ __align__(16) float sums[];  // [PER][cols]
-    __shared__ float red[2][WG / kWave];
-    const int t = threadIdx.x & (GT - 1), grp = threadIdx.x / GT;
-    const int units = (cols + V - 1) / V;
-    UnitAt<V> at[N];
-    float gm[N][V], acc[N][V];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        at[k] = unit_at<V>(t + k * GT, units, cols);
-        load_gamma<V>(gamma, at[k].col, gm[k]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[k][e] = 0.0f;
-    }
-    int turn = 0;
-    for (long long row0 = static_cast<long long>(blockIdx.x) * PER; row0 < rows;
-         row0 += static_cast<long long>(gridDim.x) * PER) {
-        const long long want = row0 + grp;
-        const bool valid = want < rows;
-        const size_t row = valid ? static_cast<size_t>(want) : static_cast<size_t>(rows) - 1;
-        const size_t base = row * cols;
-        u32x4 rd[N], rx[N];
-        [[maybe_unused]] u32x4 ro[N];
-        auto load = [&](auto stream) {
-            constexpr bool NT = decltype(stream)::value;
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                rd[k] = load16b<NT>(element_ptr<T>(dy, base + at[k].col));
-                rx[k] = load16b<NT>(element_ptr<T>(x, base + at[k].col));
-                if constexpr (ADD) ro[k] = load16b<NT>(element_ptr<T>(static_cast<const void*>(dx), base + at[k].col));
-            }
-        };
-        if (nt)
-            load(std::true_type());
-        else
-            load(std::false_type());
-        const float r = inv_rms[row];
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            float d[V], n[V];
-            row_unpack<T>(rd[k], d);
-            row_unpack<T>(rx[k], n);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const bool counts = valid && !(k == N - 1 && e < at[k].skip);
-                const float dn = counts ? d[e] * (n[e] * r) : 0.0f;
-                acc[k][e] += dn;
-                s += dn * gm[k][e];
-            }
-        }
-        float total;
-        if constexpr (GT <= kWave) {
-            total = lanes_sum<GT>(s);
-        } else {
-            s = wave_sum(s);
-            if ((threadIdx.x & (kWave - 1)) == 0) red[turn][threadIdx.x / kWave] = s;
-            __syncthreads();
-            const int w0 = grp * (GT / kWave);
-            total = red[turn][w0];
-#pragma unroll
-            for (int i = 1; i < GT / kWave; ++i) total += red[turn][w0 + i];
-            turn ^= 1;
-        }
-        wave_order();
-        const float m = total / static_cast<float>(cols);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            float d[V], n[V], o[V];
-            row_unpack<T>(rd[k], d);
-            row_unpack<T>(rx[k], n);
-            if constexpr (ADD) row_unpack<T>(ro[k], o);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float v = r * (d[e] * gm[k][e] - n[e] * r * m);
-                o[e] = rounded(ADD ? o[e] + v : v);
-            }
-            if (valid && (k < N - 1 || at[k].skip < V))
-                store16b(element_ptr<T>(dx, base + at[k].col), row_pack<T>(o));
-        }
-    }
-    float* prow = part + static_cast<size_t>(blockIdx.x) * cols;
-    float* own = PER > 1 ? sums + static_cast<size_t>(grp) * cols : prow;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e >= at[k].skip) own[at[k].col + e] = acc[k][e];
-    if constexpr (PER > 1) {
-        __syncthreads();
-        for (int c = threadIdx.x; c < cols; c += WG) {
-            float v = sums[c];
-            for (int g = 1; g < PER; ++g) v += sums[static_cast<size_t>(g) * cols + c];
-            prow[c] = v;
-        }
-    }
-}
-
-// Backward, rows of less than a unit or too long for registers: a workgroup walks a row twice
-// and keeps its columns' sums in its partial row, each column with one thread.
-template <int T, bool ADD>
-__global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
-    int rows, int cols, const void* dy, const void* __restrict__ x,
-    const float* __restrict__ inv_rms, const float* __restrict__ gamma, void* dx,
-    float* __restrict__ part) {
-    __shared__ SumTop red[2][kThreads / kWave];
-    GroupRed<kThreads> group{red};
-    float* prow = part + static_cast<size_t>(blockIdx.x) * cols;
-    for (int c = threadIdx.x; c < cols; c += kThreads) prow[c] = 0.0f;
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        const size_t base = static_cast<size_t>(row) * cols;
-        const float r = inv_rms[row];
-        float s = 0.0f;
-        for (int c = threadIdx.x; c < cols; c += kThreads)
-            s += row_get<T>(dy, base + c) * (row_get<T>(x, base + c) * r) * gamma[c];
-        const float m = group.sum(s) / static_cast<float>(cols);
-        for (int c = threadIdx.x; c < cols; c += kThreads) {
-            const float d = row_get<T>(dy, base + c), n = row_get<T>(x, base + c) * r;
-            float v = r * (d * gamma[c] - n * m);
-            if constexpr (ADD) v += row_get<T>(dx, base + c);
-            row_put<T>(dx, base + c, rounded(v));
-            prow[c] += d * n;
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------
-// Host dispatch.
-// ---------------------------------------------------------------------------
-
-int units_of(int cols, int type) {
-    const int v = 16 / row_type_size(type);
-    return (cols + v - 1) / v;
-}
-
-bool walked(int cols, int type, int most_units) {
-    return cols < 16 / row_type_size(type) || units_of(cols, type) > most_units;
-}
-
-// Calls f(GT, N): threads of a row's group and units of a thread.
-template <int GT, int FROM, int TO, class F>
-void with_steps(int units, F f) {
-    if constexpr (FROM < TO) {
-        if (units > GT * FROM) return with_steps<GT, FROM + 1, TO>(units, f);
-    }
-    f(std::integral_constant<int, GT>(), std::integral_constant<int, FROM>());
-}
-
-// Units of a thread, at most: 32 elements in the forward kernel, 24 in the backward kernel,
-// whose registers hold gamma and the sums beside the row's inputs; fewer in a workgroup of 1024
-// threads, which has half as many registers a thread.
-constexpr int fwd_steps(int type) { return type == MI_TYPE_F32 ? 8 : 4; }
-constexpr int bwd_steps(int type) { return type == MI_TYPE_F32 ? 6 : 3; }
-constexpr int wide_steps(int type) { return type == MI_TYPE_F32 ? 3 : 2; }
-
-// A wave holds a row of up to 2048 columns; a few rows, and longer ones, take more waves each.
-template <int T, class F>
-void with_fwd_shape(int rows, int units, F f) {
-    constexpr int STEPS = fwd_steps(T);
-    if (units <= 16)
-        with_steps<16, 1, 1>(units, f);
-    else if (units <= 32)
-        with_steps<32, 1, 1>(units, f);
-    else if (units <= 64 || (units <= 64 * STEPS && rows > kFewRows))
-        with_steps<64, 1, STEPS>(units, f);
-    else if (units <= 256 * STEPS)
-        with_steps<256, 1, STEPS>(units, f);
-    else
-        with_steps<1024, STEPS / 4 + 1, wide_steps(T)>(units, f);
-}
-
-unsigned row_grid(int rows, int per) {
-    return static_cast<unsigned>(
-        std::min<long long>((static_cast<long long>(rows) + per - 1) / per, kMaxGrid));
-}
-
-struct FwdCall {
-    const void *a, *b;
-    const float* gamma;
-    void *residual_out, *out;
-    float* inv_rms;
-    void* q;
-    float* scales;
-    int rows, cols;
-    float eps;
-    int block, format, type;
-};
 
 template <bool RESID, bool Q8>
-int rms_forward(const char* name, const FwdCall& c, void* stream) {
-    if (c.rows < 0 || c.cols < 1 || c.cols > kMaxCols)
-        return set_error(MI_ERR_INVALID_ARG, "%s: invalid shape rows=%d cols=%d (cols is 1 to %d)",
-                         name, c.rows, c.cols, kMaxCols);
-    if (!row_type_ok(c.type)) return set_error(MI_ERR_INVALID_ARG, "%s: type=%d", name, c.type);
+int rms_forward(const char* name, const rms::Forward& c, void* stream) {
+    if (int rc = check_rows(name, c.rows, c.cols, c.type)) return rc;
     if (!(c.eps >= 0.0f && c.eps <= 3.0e38f))
         return set_error(MI_ERR_INVALID_ARG, "%s: eps=%g", name, static_cast<double>(c.eps));
     if (Q8 && c.format != MI_ROW8_INT8 && c.format != MI_ROW8_E4M3)
@@ -606,103 +31,26 @@ int rms_forward(const char* name, const FwdCall& c, void* stream) {
     if (!c.a || !c.gamma || (RESID && (!c.b || !c.residual_out)) ||
         (Q8 ? !c.q || !c.scales : !c.out))
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
-    hipStream_t st = to_stream(stream);
-    char* q = static_cast<char*>(c.q);
-    const bool nt = stream_loads(static_cast<double>(c.rows) * c.cols * row_type_size(c.type) *
-                                 (RESID ? 2 : 1));
-    with_row_type(c.type, [&](auto type) {
-        constexpr int T = decltype(type)::value;
-        auto launch = [&](auto kind) {
-            constexpr Out OUT = decltype(kind)::value;
-            if (walked(c.cols, c.type, 1024 * wide_steps(c.type))) {
-                hipLaunchKernelGGL((rms_fwd_walk_kernel<T, RESID, OUT>),
-                                   dim3(row_grid(c.rows, 1)), dim3(kThreads), 0, st, c.rows,
-                                   c.cols, c.a, c.b, c.gamma, c.residual_out, c.out, c.eps,
-                                   c.inv_rms, q, c.scales, c.format);
-                return;
-            }
-            with_fwd_shape<T>(c.rows, units_of(c.cols, c.type), [&](auto gt, auto n) {
-                constexpr int GT = decltype(gt)::value, N = decltype(n)::value;
-                hipLaunchKernelGGL((rms_fwd_kernel<T, GT, N, RESID, OUT>),
-                                   dim3(row_grid(c.rows, kGroupThreads<GT> / GT)),
-                                   dim3(kGroupThreads<GT>), 0, st, c.rows, c.cols, c.a, c.b,
-                                   c.gamma, c.residual_out, c.out, c.eps, c.inv_rms, q, c.scales,
-                                   c.format, nt);
-            });
-        };
-        if constexpr (!Q8)
-            launch(std::integral_constant<Out, Out::Rows>());
-        else if (c.block)
-            launch(std::integral_constant<Out, Out::Block8>());
-        else
-            launch(std::integral_constant<Out, Out::Row8>());
-    });
+    with_row_type(c.type,
+                  [&](auto t) { rms::forward<decltype(t)::value>(c, to_stream(stream)); });
     return check_launch(name);
 }
 
-int bwd_threads(int units, int steps) {
-    return units <= 16 ? 16 : units <= 32 ? 32 : units <= 64 * steps ? 64
-           : units <= 256 * steps ? 256 : 1024;
-}
-
-template <int T, class F>
-void with_bwd_shape(int units, F f) {
-    constexpr int STEPS = bwd_steps(T);
-    switch (bwd_threads(units, STEPS)) {
-        case 16: return with_steps<16, 1, 1>(units, f);
-        case 32: return with_steps<32, 1, 1>(units, f);
-        case 64: return with_steps<64, 1, STEPS>(units, f);
-        case 256: return with_steps<256, 1, STEPS>(units, f);
-        default: return with_steps<1024, STEPS / 4 + 1, wide_steps(T)>(units, f);
-    }
-}
-
-// Partial rows: workgroups of the backward kernel.
-int bwd_blocks(int rows, int cols, int type) {
-    int per = 1;
-    if (!walked(cols, type, 1024 * wide_steps(type)))
-        per = std::max(1, kBwdThreads / bwd_threads(units_of(cols, type), bwd_steps(type)));
-    return static_cast<int>(
-        std::min<long long>((static_cast<long long>(rows) + per - 1) / per, kBwdBlocks));
-}
-
-template <bool ADD>
-int rms_backward(const char* name, const void* dy, const void* x, const float* inv_rms,
-                 const float* gamma, void* dx, float* dgamma, int rows, int cols, int type,
-                 void* stream) {
-    if (rows < 0 || cols < 1 || cols > kMaxCols)
-        return set_error(MI_ERR_INVALID_ARG, "%s: invalid shape rows=%d cols=%d (cols is 1 to %d)",
-                         name, rows, cols, kMaxCols);
-    if (!row_type_ok(type)) return set_error(MI_ERR_INVALID_ARG, "%s: type=%d", name, type);
-    if (rows == 0) return MI_OK;
-    if (!dy || !x || !inv_rms || !gamma || !dx || !dgamma)
+int rms_backward(const char* name, rms::Backward c, float* dgamma, void* stream) {
+    if (int rc = check_rows(name, c.rows, c.cols, c.type)) return rc;
+    if (c.rows == 0) return MI_OK;
+    if (!c.grad_out || !c.x || !c.inv_rms || !c.gamma || !c.dx || !dgamma)
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     hipStream_t st = to_stream(stream);
     int err = MI_OK;
     char* ws = static_cast<char*>(
-        workspace_get(mi_rmsnorm_backward_workspace(rows, cols, type), st, &err));
+        workspace_get(mi_rmsnorm_backward_workspace(c.rows, c.cols, c.type), st, &err));
     if (!ws) return err;
-    float* part = reinterpret_cast<float*>(ws + colsum_part_offset());
-    const int blocks = bwd_blocks(rows, cols, type);
-    const bool nt = stream_loads(static_cast<double>(rows) * cols * row_type_size(type) *
-                                 (ADD ? 3 : 2));
-    with_row_type(type, [&](auto tc) {
-        constexpr int T = decltype(tc)::value;
-        if (walked(cols, type, 1024 * wide_steps(type))) {
-            hipLaunchKernelGGL((rms_bwd_walk_kernel<T, ADD>), dim3(blocks), dim3(kThreads), 0, st,
-                               rows, cols, dy, x, inv_rms, gamma, dx, part);
-            return;
-        }
-        with_bwd_shape<T>(units_of(cols, type), [&](auto gt, auto n) {
-            constexpr int GT = decltype(gt)::value, N = decltype(n)::value;
-            constexpr int WG = kBwdGroupThreads<GT>, PER = WG / GT;
-            hipLaunchKernelGGL((rms_bwd_kernel<T, GT, N, ADD>), dim3(blocks), dim3(WG),
-                               PER > 1 ? static_cast<size_t>(PER) * cols * sizeof(float) : 0, st,
-                               rows, cols, dy, x, inv_rms, gamma, dx, part, nt);
-        });
-    });
+    c.part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    with_row_type(c.type, [&](auto t) { rms::backward<decltype(t)::value>(c, st); });
     if (int rc = check_launch(name)) return rc;
-    return launch_colsum_finalize(part, blocks, cols, dgamma, cols, nullptr, st);
+    return launch_colsum_finalize(c.part, rms::backward_blocks(c.rows, c.cols, c.type), c.cols,
+                                  dgamma, c.cols, nullptr, st);
 }
 
 }  // namespace
@@ -716,7 +64,7 @@ int mi_rmsnorm_forward(const void* x, const float* gamma, void* out, float* inv_
                        int cols, float eps, int type, void* stream) {
     return rms_forward<false, false>(
         "mi_rmsnorm_forward",
-        FwdCall{x, nullptr, gamma, nullptr, out, inv_rms, nullptr, nullptr, rows, cols, eps, 0, 0,
+        rms::Forward{x, nullptr, gamma, nullptr, out, inv_rms, nullptr, nullptr, rows, cols, eps, 0, 0,
                 type},
         stream);
 }
@@ -726,7 +74,7 @@ int mi_residual_rmsnorm_forward(const void* a, const void* b, const float* gamma
                                 float eps, int type, void* stream) {
     return rms_forward<true, false>(
         "mi_residual_rmsnorm_forward",
-        FwdCall{a, b, gamma, residual_out, out, inv_rms, nullptr, nullptr, rows, cols, eps, 0, 0,
+        rms::Forward{a, b, gamma, residual_out, out, inv_rms, nullptr, nullptr, rows, cols, eps, 0, 0,
                 type},
         stream);
 }
@@ -736,7 +84,7 @@ int mi_rmsnorm_forward_row8(const void* x, const float* gamma, void* q, float* s
                             int type, void* stream) {
     return rms_forward<false, true>(
         "mi_rmsnorm_forward_row8",
-        FwdCall{x, nullptr, gamma, nullptr, out, inv_rms, q, scales, rows, cols, eps, block,
+        rms::Forward{x, nullptr, gamma, nullptr, out, inv_rms, q, scales, rows, cols, eps, block,
                 format, type},
         stream);
 }
@@ -747,7 +95,7 @@ int mi_residual_rmsnorm_forward_row8(const void* a, const void* b, const float* 
                                      int format, int type, void* stream) {
     return rms_forward<true, true>(
         "mi_residual_rmsnorm_forward_row8",
-        FwdCall{a, b, gamma, residual_out, out, inv_rms, q, scales, rows, cols, eps, block, format,
+        rms::Forward{a, b, gamma, residual_out, out, inv_rms, q, scales, rows, cols, eps, block, format,
                 type},
         stream);
 }
@@ -755,20 +103,24 @@ int mi_residual_rmsnorm_forward_row8(const void* a, const void* b, const float* 
 int mi_rmsnorm_backward(const void* grad_out, const void* x, const float* inv_rms,
                         const float* gamma, void* grad_x, float* dgamma, int rows, int cols,
                         int type, void* stream) {
-    return rms_backward<false>("mi_rmsnorm_backward", grad_out, x, inv_rms, gamma, grad_x, dgamma,
-                               rows, cols, type, stream);
+    return rms_backward("mi_rmsnorm_backward",
+                        rms::Backward{grad_out, x, inv_rms, gamma, grad_x, false, rows, cols, type,
+                                      nullptr},
+                        dgamma, stream);
 }
 
 int mi_rmsnorm_backward_residual(const void* grad_out, const void* x, const float* inv_rms,
                                  const float* gamma, void* grad_residual, float* dgamma, int rows,
                                  int cols, int type, void* stream) {
-    return rms_backward<true>("mi_rmsnorm_backward_residual", grad_out, x, inv_rms, gamma,
-                              grad_residual, dgamma, rows, cols, type, stream);
+    return rms_backward("mi_rmsnorm_backward_residual",
+                        rms::Backward{grad_out, x, inv_rms, gamma, grad_residual, true, rows, cols,
+                                      type, nullptr},
+                        dgamma, stream);
 }
 
 size_t mi_rmsnorm_backward_workspace(int rows, int cols, int type) {
     if (rows <= 0 || cols <= 0 || !row_type_ok(type)) return 0;
-    return colsum_bytes(bwd_blocks(rows, cols, type), cols);
+    return colsum_bytes(rms::backward_blocks(rows, cols, type), cols);
 }
 
 }  // extern "C"

@@ -19,43 +19,49 @@ namespace mi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 112;           // tensors of a launch: 3.3 KB of arguments
-constexpr long long kUnit = 8192;     // elements
+constexpr int kBatch = 96;            // tensors of a launch: 3.4 KB of arguments
+constexpr int kShift = 13;            // a unit has 2^kShift elements,
+constexpr int kFewShift = 11;         // or 2^kFewShift where all tensors have less than
+constexpr long long kFew = 1ll << 23; // so many together
 constexpr int kNormBlocks = 2048;     // workgroups of the norm's launches, about
 constexpr int kScaleBlocks = 131072;
+constexpr int kFewParts = 512;        // partial sums that every workgroup may add for itself
 constexpr int kFinThreads = 1024;
 constexpr long long kMaxUnits = 1ll << 30;
 
-struct Batch {
-    const void* data[kBatch];
-    void* out[kBatch];
-    long long size[kBatch];
-    unsigned end[kBatch];  // units up to the tensor's last
-    unsigned char type[kBatch];
-    int count;
+struct Tensor {
+    const void* data;
+    void* out;
+    long long size;
+    int type, unused;
 };
 
-// The first tensor that ends behind unit u.
+struct Batch {
+    Tensor tensor[kBatch];
+    unsigned end[kBatch];  // units up to the tensor's last; the largest number behind the last one
+    int count;
+    int shift;
+};
+
+// The first tensor that ends behind unit u: the number of ends up to u, which the lanes count
+// in one round trip (the arguments may lie in host memory).
 __device__ __forceinline__ int tensor_of(const Batch& b, unsigned u) {
-    int lo = 0, hi = b.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (b.end[mid] > u)
-            hi = mid;
-        else
-            lo = mid + 1;
-    }
-    return lo;
+    const int lane = threadIdx.x & (kWave - 1);
+    static_assert(kBatch > kWave && kBatch <= 2 * kWave, "two ends a lane");
+    const unsigned e0 = b.end[lane], e1 = b.end[min(lane + kWave, kBatch - 1)];
+    return __popcll(__ballot(e0 <= u)) + __popcll(__ballot(lane < kBatch - kWave && e1 <= u));
 }
 
 // Calls f(tensor, first element, end element) for the pieces of units [u, end).
 template <class F>
 __device__ __forceinline__ void for_pieces(const Batch& b, unsigned u, unsigned end, F f) {
-    for (int i = tensor_of(b, u); u < end; ++i) {
+    if (u >= end) return;
+    const int shift = b.shift;
+    for (int i = __builtin_amdgcn_readfirstlane(tensor_of(b, u)); u < end; ++i) {
         const unsigned from = i ? b.end[i - 1] : 0u, to = min(end, b.end[i]);
-        if (u >= to) continue;
-        f(i, static_cast<long long>(u - from) * kUnit,
-          min(b.size[i], static_cast<long long>(to - from) * kUnit));
+        const Tensor t = b.tensor[i];
+        f(t, static_cast<long long>(u - from) << shift,
+          min(t.size, static_cast<long long>(to - from) << shift));
         u = to;
     }
 }
@@ -89,9 +95,9 @@ __device__ __forceinline__ void add_squares(const void* data, long long first, l
     }
 }
 
-__global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(const Batch b,
-                                                                 float* __restrict__ part,
-                                                                 unsigned units, bool nt) {
+__global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(float* __restrict__ part,
+                                                                 unsigned units, bool nt,
+                                                                 const Batch b) {
     __shared__ float red[kThreads / kWave];
     const unsigned u0 = static_cast<unsigned>(static_cast<unsigned long long>(units) * blockIdx.x /
                                               gridDim.x);
@@ -100,15 +106,15 @@ __global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(const Batch b,
     float acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-    for_pieces(b, u0, u1, [&](int i, long long first, long long end) {
+    for_pieces(b, u0, u1, [&](const Tensor& t, long long first, long long end) {
         auto add = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
-            if (b.type[i] == MI_TYPE_F32)
-                add_squares<MI_TYPE_F32, NT>(b.data[i], first, end, acc);
-            else if (b.type[i] == MI_TYPE_F16)
-                add_squares<MI_TYPE_F16, NT>(b.data[i], first, end, acc);
+            if (t.type == MI_TYPE_F32)
+                add_squares<MI_TYPE_F32, NT>(t.data, first, end, acc);
+            else if (t.type == MI_TYPE_F16)
+                add_squares<MI_TYPE_F16, NT>(t.data, first, end, acc);
             else
-                add_squares<MI_TYPE_BF16, NT>(b.data[i], first, end, acc);
+                add_squares<MI_TYPE_BF16, NT>(t.data, first, end, acc);
         };
         if (nt)
             add(std::true_type());
@@ -129,89 +135,139 @@ __global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(const Batch b,
     }
 }
 
-// The partial sums in 64 bits, in a fixed order.
+// The partial sums in 64 bits, in a fixed order; every thread gets the total.
+template <int NT>
+__device__ __forceinline__ double add_parts(const float* part, int parts, double* red) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += NT) s += static_cast<double>(part[i]);
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) s += __shfl_xor(s, m);
+    if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = s;
+    __syncthreads();
+    s = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / kWave; ++w) s += red[w];
+    return s;
+}
+
+__device__ __forceinline__ float clip_scale(float norm_sq, float max_norm) {
+    const float norm = sqrtf(norm_sq);
+    return norm > max_norm ? max_norm / norm : 1.0f;
+}
+
 __global__ __launch_bounds__(kFinThreads) void tensors_finish_kernel(
     const float* __restrict__ part, int parts, float* __restrict__ result, bool accumulate,
     float* __restrict__ clip, float max_norm) {
-    __shared__ double red[kFinThreads];
-    double s = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kFinThreads) s += static_cast<double>(part[i]);
-    red[threadIdx.x] = s;
-    __syncthreads();
-#pragma unroll
-    for (int h = kFinThreads / 2; h >= 1; h /= 2) {
-        if (static_cast<int>(threadIdx.x) < h) red[threadIdx.x] += red[threadIdx.x + h];
-        __syncthreads();
-    }
+    __shared__ double red[kFinThreads / kWave];
+    const double s = add_parts<kFinThreads>(part, parts, red);
     if (threadIdx.x == 0) {
-        const float total = static_cast<float>(accumulate ? *result + red[0] : red[0]);
+        const float total = static_cast<float>(accumulate ? *result + s : s);
         *result = total;
-        if (clip) {
-            const float norm = sqrtf(total);
-            *clip = norm > max_norm ? max_norm / norm : 1.0f;
-        }
+        if (clip) *clip = clip_scale(total, max_norm);
+    }
+}
+
+// The elements of a load: 16 bytes, or as many as make 16 bytes of fp32, so that the lanes' stores
+// are side by side too.
+template <int T, bool WIDE>
+constexpr int kScaleVec = WIDE ? 4 : row_vec<T>();
+
+template <int T, int V, bool NT>
+__device__ __forceinline__ void load_values(const char* p, float (&v)[V]) {
+    if constexpr (V == row_vec<T>()) {
+        row_unpack<T>(load16b<NT>(p), v);
+    } else {
+        typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
+        u32x2 half;
+        if constexpr (NT)
+            half = __builtin_nontemporal_load(reinterpret_cast<const u32x2_at2*>(p));
+        else
+            half = *reinterpret_cast<const u32x2_at2*>(p);
+        float w[2 * V];
+        row_unpack<T>(u32x4{half.x, half.y, 0u, 0u}, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = w[e];
     }
 }
 
 // A product is rounded to fp32 and then to the type, wherever it stands (rounded: a multiplication
 // may otherwise be joined with its conversion to fp16, or not).
 template <int T, bool WIDE, bool NT>
-__device__ __forceinline__ void scale_piece(const void* data, void* out, long long first,
-                                            long long end, float c) {
-    constexpr int V = row_vec<T>(), U = 4;
+__device__ __forceinline__ void scale_piece(const Tensor& t, long long first, long long end,
+                                            float c) {
+    constexpr int V = kScaleVec<T, WIDE>, O = WIDE ? MI_TYPE_F32 : T;
+    constexpr int U = 64 / (V * static_cast<int>(sizeof(row_elem<T>)));
     constexpr long long kStep = static_cast<long long>(kThreads) * V;
-    const char* p = static_cast<const char*>(data);
+    const char* p = static_cast<const char*>(t.data);
+    char* o = static_cast<char*>(t.out);
     const long long whole = first + (end - first) / V * V;
     long long at = first + static_cast<long long>(threadIdx.x) * V;
-    auto put = [&](long long i, const u32x4& raw) {
-        float v[V];
-        row_unpack<T>(raw, v);
+    auto put = [&](long long i, float (&v)[V]) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = rounded(v[e] * c);
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int e = 0; e < V; e += 4)
-                store16b(static_cast<float*>(out) + i + e,
-                         u32x4{__float_as_uint(v[e]), __float_as_uint(v[e + 1]),
-                               __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3])});
-        } else {
-            store16b(static_cast<char*>(out) + i * sizeof(row_elem<T>), row_pack<T>(v));
-        }
+        store16b(o + i * sizeof(row_elem<O>), row_pack<O>(v));
     };
     for (; at + (U - 1) * kStep < whole; at += U * kStep) {
-        u32x4 raw[U];
+        float v[U][V];
 #pragma unroll
         for (int i = 0; i < U; ++i)
-            raw[i] = load16b<NT>(p + (at + i * kStep) * sizeof(row_elem<T>));
+            load_values<T, V, NT>(p + (at + i * kStep) * sizeof(row_elem<T>), v[i]);
 #pragma unroll
-        for (int i = 0; i < U; ++i) put(at + i * kStep, raw[i]);
+        for (int i = 0; i < U; ++i) put(at + i * kStep, v[i]);
     }
-    for (; at < whole; at += kStep) put(at, load16b<NT>(p + at * sizeof(row_elem<T>)));
+    for (; at < whole; at += kStep) {
+        float v[V];
+        load_values<T, V, NT>(p + at * sizeof(row_elem<T>), v);
+        put(at, v);
+    }
     if (whole + threadIdx.x < end) {
         const size_t i = static_cast<size_t>(whole) + threadIdx.x;
-        row_put<WIDE ? MI_TYPE_F32 : T>(out, i, rounded(row_get<T>(data, i) * c));
+        row_put<O>(t.out, i, rounded(row_get<T>(t.data, i) * c));
     }
 }
 
-template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void tensors_scale_kernel(const Batch b,
-                                                                 const float* __restrict__ scale,
-                                                                 unsigned units, bool nt) {
-    const float c = *scale;
+// The norm's partial sums, which every workgroup adds (the same way) instead of a launch of its
+// own: part NULL where the scale is there.
+struct Parts {
+    const float* part;
+    int parts;
+    float max_norm;
+    float* norm_sq;
+    float* clip;
+};
+
+template <bool WIDE, bool PARTS>
+__global__ __launch_bounds__(kThreads) void tensors_scale_kernel(const float* __restrict__ scale,
+                                                                 unsigned units, bool nt,
+                                                                 const Parts parts,
+                                                                 const Batch b) {
+    float c;
+    if constexpr (PARTS) {
+        __shared__ double red[kThreads / kWave];
+        const float total =
+            static_cast<float>(add_parts<kThreads>(parts.part, parts.parts, red));
+        c = clip_scale(total, parts.max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            *parts.norm_sq = total;
+            *parts.clip = c;
+        }
+    } else {
+        c = *scale;
+    }
     if (!WIDE && c == 1.0f) return;
     const unsigned u0 = static_cast<unsigned>(static_cast<unsigned long long>(units) * blockIdx.x /
                                               gridDim.x);
     const unsigned u1 = static_cast<unsigned>(static_cast<unsigned long long>(units) *
                                               (blockIdx.x + 1ull) / gridDim.x);
-    for_pieces(b, u0, u1, [&](int i, long long first, long long end) {
+    for_pieces(b, u0, u1, [&](const Tensor& t, long long first, long long end) {
         auto put = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
-            if (b.type[i] == MI_TYPE_F32)
-                scale_piece<MI_TYPE_F32, WIDE, NT>(b.data[i], b.out[i], first, end, c);
-            else if (b.type[i] == MI_TYPE_F16)
-                scale_piece<MI_TYPE_F16, WIDE, NT>(b.data[i], b.out[i], first, end, c);
+            if (t.type == MI_TYPE_F32)
+                scale_piece<MI_TYPE_F32, WIDE, NT>(t, first, end, c);
+            else if (t.type == MI_TYPE_F16)
+                scale_piece<MI_TYPE_F16, WIDE, NT>(t, first, end, c);
             else
-                scale_piece<MI_TYPE_BF16, WIDE, NT>(b.data[i], b.out[i], first, end, c);
+                scale_piece<MI_TYPE_BF16, WIDE, NT>(t, first, end, c);
         };
         if (nt)
             put(std::true_type());
@@ -227,53 +283,67 @@ struct List {
     const int* types;
     int count;
     int type(int i) const { return types ? types[i] : MI_TYPE_F32; }
-    long long units(int i) const { return (sizes[i] + kUnit - 1) / kUnit; }
 };
 
+long long units_of(long long elements, int shift) {
+    return (elements + (1ll << shift) - 1) >> shift;
+}
+
 struct Totals {
-    long long units = 0;
+    long long elements = 0, units = 0;
     double bytes = 0.0;
+    int shift = kShift, batches = 0;
 };
 
 int check_list(const char* name, const List& l, Totals* total) {
     if (l.count < 0) return set_error(MI_ERR_INVALID_ARG, "%s: count=%d", name, l.count);
     if (l.count > 0 && (!l.tensors || !l.sizes))
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    int some = 0;
     for (int i = 0; i < l.count; ++i) {
-        if (l.sizes[i] < 0 || l.sizes[i] > kMaxUnits * kUnit)
+        if (l.sizes[i] < 0 || l.sizes[i] > kMaxUnits << kShift)
             return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d has size %lld", name, i,
                              l.sizes[i]);
         if (!row_type_ok(l.type(i)))
             return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d has unknown type %d", name, i,
                              l.type(i));
-        if (l.sizes[i] > 0 && (!l.tensors[i] || (l.outs && !l.outs[i])))
+        if (l.sizes[i] == 0) continue;
+        if (!l.tensors[i] || (l.outs && !l.outs[i]))
             return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d: NULL pointer", name, i);
-        total->units += l.units(i);
+        ++some;
+        total->elements += l.sizes[i];
+        total->units += units_of(l.sizes[i], kShift);
         total->bytes += static_cast<double>(l.sizes[i]) * row_type_size(l.type(i));
         if (total->units > kMaxUnits)
             return set_error(MI_ERR_INVALID_ARG, "%s: more than %lld elements", name,
-                             kMaxUnits * kUnit);
+                             kMaxUnits << kShift);
+    }
+    total->batches = (some + kBatch - 1) / kBatch;
+    if (total->elements < kFew) {
+        total->shift = kFewShift;
+        total->units = 0;
+        for (int i = 0; i < l.count; ++i) total->units += units_of(l.sizes[i], kFewShift);
     }
     return MI_OK;
 }
 
 // Calls f(batch, its units) for every kBatch tensors that have elements.
 template <class F>
-int for_batches(const List& l, F f) {
+int for_batches(const List& l, int shift, F f) {
     Batch b;
     b.count = 0;
+    b.shift = shift;
     unsigned units = 0;
     for (int i = 0; i < l.count; ++i) {
         if (l.sizes[i] > 0) {
             const int n = b.count++;
-            units += static_cast<unsigned>(l.units(i));
-            b.data[n] = l.tensors[i];
-            b.out[n] = l.outs ? l.outs[i] : const_cast<void*>(l.tensors[i]);
-            b.size[n] = l.sizes[i];
+            units += static_cast<unsigned>(units_of(l.sizes[i], shift));
+            b.tensor[n] = {l.tensors[i], l.outs ? l.outs[i] : const_cast<void*>(l.tensors[i]),
+                           l.sizes[i], l.type(i), 0};
             b.end[n] = units;
-            b.type[n] = static_cast<unsigned char>(l.type(i));
         }
         if (b.count > 0 && (b.count == kBatch || i == l.count - 1)) {
+            for (int n = b.count; n < kBatch; ++n) b.end[n] = UINT_MAX;
             if (int rc = f(b, units)) return rc;
             b.count = 0;
             units = 0;
@@ -288,35 +358,42 @@ int norm_blocks(unsigned units, long long all) {
     return static_cast<int>(std::min<long long>(share, units));
 }
 
-int norm_sq(const char* name, const List& l, const Totals& total, float* result, bool accumulate,
-            float* clip, float max_norm, hipStream_t st) {
+// The partial sums of all squares, in *part.
+int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t st, float** part,
+               int* parts) {
     int err = MI_OK;
     char* ws = static_cast<char*>(workspace_get(mi_tensors_workspace(l.count), st, &err));
     if (!ws) return err;
-    float* part = reinterpret_cast<float*>(ws + colsum_part_offset());
-    int parts = 0;
+    *part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    *parts = 0;
     const bool nt = stream_loads(total.bytes);
-    const int rc = for_batches(l, [&](const Batch& b, unsigned units) {
+    return for_batches(l, total.shift, [&](const Batch& b, unsigned units) {
         const int blocks = norm_blocks(units, total.units);
-        hipLaunchKernelGGL(tensors_sumsq_kernel, dim3(blocks), dim3(kThreads), 0, st, b,
-                           part + parts, units, nt);
-        parts += blocks;
+        hipLaunchKernelGGL(tensors_sumsq_kernel, dim3(blocks), dim3(kThreads), 0, st,
+                           *part + *parts, units, nt, b);
+        *parts += blocks;
         return check_launch(name);
     });
-    if (rc) return rc;
+}
+
+int finish_norm(const char* name, const float* part, int parts, float* result, bool accumulate,
+                float* clip, float max_norm, hipStream_t st) {
     hipLaunchKernelGGL(tensors_finish_kernel, dim3(1), dim3(kFinThreads), 0, st, part, parts,
                        result, accumulate, clip, max_norm);
     return check_launch(name);
 }
 
 int scale_all(const char* name, const List& l, const Totals& total, const float* scale,
-              hipStream_t st) {
+              const Parts* parts, hipStream_t st) {
     const bool nt = stream_loads(total.bytes);
-    return for_batches(l, [&](const Batch& b, unsigned units) {
+    return for_batches(l, total.shift, [&](const Batch& b, unsigned units) {
         const dim3 grid(std::min<unsigned>(units, kScaleBlocks));
         with_flag(l.outs != nullptr, [&](auto wide) {
-            hipLaunchKernelGGL((tensors_scale_kernel<decltype(wide)::value>), grid,
-                               dim3(kThreads), 0, st, b, scale, units, nt);
+            with_flag(parts != nullptr, [&](auto add) {
+                hipLaunchKernelGGL(
+                    (tensors_scale_kernel<decltype(wide)::value, decltype(add)::value>), grid,
+                    dim3(kThreads), 0, st, scale, units, nt, parts ? *parts : Parts{}, b);
+            });
         });
         return check_launch(name);
     });
@@ -344,7 +421,11 @@ int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, c
     if (int rc = check_list(name, l, &total)) return rc;
     if (!d_result) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     if (total.units == 0) return MI_OK;
-    return norm_sq(name, l, total, d_result, true, nullptr, 0.0f, to_stream(stream));
+    hipStream_t st = to_stream(stream);
+    float* part = nullptr;
+    int parts = 0;
+    if (int rc = norm_parts(name, l, total, st, &part, &parts)) return rc;
+    return finish_norm(name, part, parts, d_result, true, nullptr, 0.0f, st);
 }
 
 int mi_tensors_scale(const void* const* tensors, void* const* outs, const long long* sizes,
@@ -354,7 +435,7 @@ int mi_tensors_scale(const void* const* tensors, void* const* outs, const long l
     Totals total;
     if (int rc = check_list(name, l, &total)) return rc;
     if (!d_scale) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
-    return scale_all(name, l, total, d_scale, to_stream(stream));
+    return scale_all(name, l, total, d_scale, nullptr, to_stream(stream));
 }
 
 int mi_tensors_clip(const void* const* tensors, void* const* outs, const long long* sizes,
@@ -369,8 +450,16 @@ int mi_tensors_clip(const void* const* tensors, void* const* outs, const long lo
         return set_error(MI_ERR_INVALID_ARG, "%s: max_norm=%g", name,
                          static_cast<double>(max_norm));
     hipStream_t st = to_stream(stream);
-    if (int rc = norm_sq(name, l, total, d_norm_sq, false, d_clip_scale, max_norm, st)) return rc;
-    return scale_all(name, l, total, d_clip_scale, st);
+    float* part = nullptr;
+    int parts = 0;
+    if (int rc = norm_parts(name, l, total, st, &part, &parts)) return rc;
+    if (total.batches == 1 && parts <= kFewParts) {
+        const Parts p{part, parts, max_norm, d_norm_sq, d_clip_scale};
+        return scale_all(name, l, total, nullptr, &p, st);
+    }
+    if (int rc = finish_norm(name, part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
+        return rc;
+    return scale_all(name, l, total, d_clip_scale, nullptr, st);
 }
 
 }  // extern "C"
