@@ -23,11 +23,51 @@ namespace {
 constexpr int kFwdThreads = 1024;
 constexpr int kFwdBlocks = 256;
 constexpr int kOneTrips = 4;  // rows of a lane group in a call that one workgroup does alone
-constexpr int kFinThreads = 1024;
+constexpr int kFinThreads = 256;
 constexpr int kFinExperts = 16;  // experts of a workgroup that adds partial rows
 constexpr int kFinSlices = kFinThreads / kFinExperts;
 constexpr int kBwdThreads = 256;
 constexpr int kMaxGrid = 1 << 20;
+
+// A lane's pieces of a row: where piece p begins, and how many of its first elements another
+// lane has.  A row that is no whole number of pieces ends with one that begins early (there are
+// no fewer experts than a piece has, for the number of experts decides P); what is shared counts
+// once in sums, and is written twice with the same bits.  So every load is whole and inside the
+// row, and a row's loads go out together: with the cut ones behind branches, each waited for the
+// one before (FIXME).
+template <int T, int L, int P>
+struct Pieces {
+    static constexpr int N = kPiece<T, P>;
+    int begin[P / N], skip[P / N];
+    __device__ __forceinline__ Pieces(int gl, int experts) {
+#pragma unroll
+        for (int i = 0; i < P / N; ++i) {
+            const int e0 = gl * N + i * N * L, last = experts - N;
+            begin[i] = min(e0, last);
+            skip[i] = min(max(e0 - last, 0), N);
+        }
+    }
+    // More than half of the lanes' places have an expert.
+    static constexpr bool whole(int i) { return L * P > 16 && (i + 1) * N * L <= L * P / 2; }
+    __device__ __forceinline__ bool own(int i, int e) const { return whole(i) || e >= skip[i]; }
+};
+
+template <int T, int L, int P, bool NT>
+__device__ __forceinline__ void load_pieces(const void* logits, size_t row, int experts,
+                                            const Pieces<T, L, P>& at, float (&v)[P]) {
+    constexpr int N = Pieces<T, L, P>::N;
+    const row_elem<T>* p = static_cast<const row_elem<T>*>(logits) + row * experts;
+#pragma unroll
+    for (int i = 0; i < P / N; ++i) {
+        float part[N];
+        if constexpr (N == row_vec<T>())
+            row_unpack<T>(load16b<NT>(p + at.begin[i]), part);
+        else
+            row_get_n<T, N>(p, at.begin[i], part);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i * N + e] = part[e];
+    }
+}
 
 // e^(v - max) of a row's logits, and 1 over their sum: 0 for a row of -inf alone; a
 // NaN or +inf makes all of them NaN.
@@ -48,6 +88,16 @@ __device__ __forceinline__ float softmax_terms(float (&v)[P]) {
     return s == 0.0f ? 0.0f : 1.0f / s;
 }
 
+// The sum of lanes l, l + 16, l + 32 and l + 48, in all four.  (Through LDS, 32 permutes a wave:
+// the loss of [32768, 256] FIXME.)
+__device__ __forceinline__ float add_rows_of_16(float v) {
+    auto both = [](auto pair) { return __uint_as_float(pair[0]) + __uint_as_float(pair[1]); };
+    unsigned u = __float_as_uint(v);
+    v = both(__builtin_amdgcn_permlane16_swap(u, u, false, false));
+    u = __float_as_uint(v);
+    return both(__builtin_amdgcn_permlane32_swap(u, u, false, false));
+}
+
 // sum c_e P_e to the loss.
 __device__ __forceinline__ float loss_of(double sum, int experts, int k, int n, float coef) {
     return n == 0 ? 0.0f
@@ -61,16 +111,19 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 
-// What the workgroups that add partial rows leave for the last of them.
+// sum c_e P_e over the workgroups that add partial rows, as whole numbers, which come out the same
+// in any order: each adds its share of n k, the largest such sum, in units of 2^-49 of it, to bits 7
+// to 56 of one word, 1 to the bits below, so that the last one knows that it is, and 1 to those
+// above where its share is no number.  The word says all, so nothing has to be ordered by it.
 struct Finish {
-    double sum[kMaxExperts / kFinExperts];
-    unsigned done;
+    unsigned long long word;
 };
+constexpr double kShare = 0x1p49;
 
 // Sums of the probabilities and counts over a workgroup's tokens: a lane adds its experts'
 // over its rows in registers, the waves' sums meet in LDS, in order.  ONE: the only
 // workgroup, which writes the results; else a partial row of both.
-template <int T, int L, int P, bool ONE>
+template <int T, int L, int P, bool ONE, bool NT>
 __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
     const void* __restrict__ logits, const int* __restrict__ ids, int tokens, int experts, int k,
     const unsigned char* __restrict__ valid, float* __restrict__ part, int* __restrict__ part_n,
@@ -83,40 +136,61 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
     __shared__ int count[kMaxExperts + 1];
     const int gl = threadIdx.x & (L - 1), lane = threadIdx.x & (kWave - 1);
     const int wave = threadIdx.x / kWave;
+    const Pieces<T, L, P> at(gl, experts);
+    const unsigned char* flags = valid ? valid : reinterpret_cast<const unsigned char*>(ids);
+    struct Row {
+        float v[P];
+        int id;
+        bool live;
+    };
+    auto load = [&](long long base, Row& r) {
+        const long long want = base + threadIdx.x / L;
+        const bool inside = want < tokens;
+        const size_t row = inside ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
+        load_pieces<T, L, P, NT>(logits, row, experts, at, r.v);
+        r.id = ids[row * k + min(gl, k - 1)];
+        r.live = inside && (flags[row] != 0 || !valid);
+    };
+    const long long stride = static_cast<long long>(gridDim.x) * PER;
+    long long base = static_cast<long long>(blockIdx.x) * PER;
+    Row r;
+    if (base < tokens) load(base, r);
     for (int e = threadIdx.x; e <= experts; e += kFwdThreads) count[e] = 0;
-    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) finish->done = 0;
+    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) finish->word = 0;
     __syncthreads();
     float acc[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) acc[p] = 0.0f;
-    for (long long base = static_cast<long long>(blockIdx.x) * PER; base < tokens;
-         base += static_cast<long long>(gridDim.x) * PER) {
-        const long long want = base + threadIdx.x / L;
-        const size_t row = want < tokens ? static_cast<size_t>(want)
-                                         : static_cast<size_t>(tokens) - 1;
-        const bool live = want < tokens && (!valid || valid[row] != 0);
-        const int id = want < tokens && gl < k ? ids[row * k + gl] : -1;
-        float v[P];
-        load_logits<T, L, P>(logits, row, tokens, gl, experts, v);
-        const float inv = softmax_terms<L, P>(v);
+    while (base < tokens) {
+        base += stride;
+        Row next;
+        if (base < tokens) load(base, next);
 #pragma unroll
-        for (int p = 0; p < P; ++p) acc[p] += live ? v[p] * inv : 0.0f;
-        if (live && id >= 0 && id < experts) atomicAdd(&count[id], 1);
-        const unsigned long long rows = __ballot(live && gl == 0);
-        if (lane == 0 && rows) atomicAdd(&count[experts], __popcll(rows));
+        for (int p = 0; p < P; ++p)
+            if (!at.own(p / N, p % N)) r.v[p] = -__builtin_inff();
+        const float inv = softmax_terms<L, P>(r.v);
+        const unsigned long long live = __ballot(r.live);
+        if (live == ~0ull) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) acc[p] += r.v[p] * inv;
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) acc[p] += r.live ? r.v[p] * inv : 0.0f;
+        }
+        if (r.live && gl < k && r.id >= 0 && r.id < experts) atomicAdd(&count[r.id], 1);
+        if (lane == 0 && live) atomicAdd(&count[experts], __popcll(live) / L);
+        r = next;
     }
     // the wave's rows, then the waves
     if constexpr (L == 16) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            acc[p] += __shfl_xor(acc[p], 16);
-            acc[p] += __shfl_xor(acc[p], 32);
-        }
+        for (int p = 0; p < P; ++p) acc[p] = add_rows_of_16(acc[p]);
     }
     auto put = [&](int slot) {
         if (lane < L) {
 #pragma unroll
-            for (int p = 0; p < P; ++p) sums[slot][gl * N + step_expert<T, L, P>(p)] = acc[p];
+            for (int p = 0; p < P; ++p)
+                if (at.own(p / N, p % N)) sums[slot][at.begin[p / N] + p % N] = acc[p];
         }
     };
     if constexpr (SLOTS < WAVES) {
@@ -125,9 +199,9 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
         if (wave < SLOTS) {
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                acc[p] += sums[wave][gl * N + step_expert<T, L, P>(p)];
+                if (at.own(p / N, p % N)) acc[p] += sums[wave][at.begin[p / N] + p % N];
+            put(wave);
         }
-        if (wave < SLOTS) put(wave);
     } else {
         put(wave);
     }
@@ -166,111 +240,108 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
     }
 }
 
-// Adds the partial rows: a workgroup has 16 experts, 64 slices of the rows side by side, each in
-// order, then added pairwise.  The workgroup that ends last adds all workgroups' sums of c_e P_e,
-// in order, whichever it is.
+// Adds the partial rows: a workgroup has 16 experts, and 16 slices of the rows side by side, each
+// in order, which are then added pairwise.
 __global__ __launch_bounds__(kFinThreads) void balance_finish_kernel(
     const float* __restrict__ part, const int* __restrict__ part_n, int blocks, int experts, int k,
     float coef, int* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss,
     Finish* finish) {
     constexpr int TRIPS = kFwdBlocks / kFinSlices;
     __shared__ float sum[kFinSlices][kFinExperts];
-    __shared__ int count[kFinSlices][kFinExperts];
-    __shared__ int total;
+    __shared__ int count[kFinSlices][kFinExperts], tokens[kFinThreads / kWave];
     const int col = threadIdx.x & (kFinExperts - 1), slice = threadIdx.x / kFinExperts;
-    const int e = blockIdx.x * kFinExperts + col;
-    if (threadIdx.x == 0) total = 0;
-    const int rows = static_cast<int>(threadIdx.x) < blocks
-                         ? part_n[static_cast<size_t>(threadIdx.x) * (experts + 1) + experts]
-                         : 0;
+    const int e = blockIdx.x * kFinExperts + col, at = min(e, experts - 1);
+    // every load goes out, from a place that is there, and counts where its place is
+    const int mine = min(static_cast<int>(threadIdx.x), blocks - 1);
+    int rows = part_n[static_cast<size_t>(mine) * (experts + 1) + experts];
     float p[TRIPS];
     int c[TRIPS];
 #pragma unroll
     for (int i = 0; i < TRIPS; ++i) {
-        const int b = slice + i * kFinSlices;
-        const bool there = b < blocks && e < experts;
-        p[i] = there ? part[static_cast<size_t>(b) * experts + e] : 0.0f;
-        c[i] = there ? part_n[static_cast<size_t>(b) * (experts + 1) + e] : 0;
+        const int b = min(slice + i * kFinSlices, blocks - 1);
+        p[i] = part[static_cast<size_t>(b) * experts + at];
+        c[i] = part_n[static_cast<size_t>(b) * (experts + 1) + at];
     }
+    rows = static_cast<int>(threadIdx.x) < blocks ? rows : 0;
 #pragma unroll
-    for (int i = 1; i < TRIPS; ++i) {
-        p[0] += p[i];
-        c[0] += c[i];
+    for (int m = 1; m < kWave; m *= 2) rows += __shfl_xor(rows, m);
+    if ((threadIdx.x & (kWave - 1)) == 0) tokens[threadIdx.x / kWave] = rows;
+#pragma unroll
+    for (int i = 0; i < TRIPS; ++i) {
+        const bool there = slice + i * kFinSlices < blocks;
+        p[i] = there ? p[i] : 0.0f;
+        c[i] = there ? c[i] : 0;
+        if (i > 0) {
+            p[0] += p[i];
+            c[0] += c[i];
+        }
     }
     sum[slice][col] = p[0];
     count[slice][col] = c[0];
     __syncthreads();
-    if (rows) atomicAdd(&total, rows);
-#pragma unroll
-    for (int h = kFinSlices / 2; h >= 1; h /= 2) {
-        if (slice < h) {
-            sum[slice][col] += sum[slice + h][col];
-            count[slice][col] += count[slice + h][col];
-        }
-        __syncthreads();
-    }
     if (threadIdx.x >= kWave) return;
-    const int n = total;
-    double s = 0.0;
+    // the first wave: lanes of the same expert 16 apart
+    float s = 0.0f;
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < kFinSlices / 4; ++i) {
+        s += sum[slice * (kFinSlices / 4) + i][col];
+        m += count[slice * (kFinSlices / 4) + i][col];
+    }
+    s = add_rows_of_16(s);
+    m += __shfl_xor(m, 16);
+    m += __shfl_xor(m, 32);
+    int n = tokens[0];
+#pragma unroll
+    for (int w = 1; w < kFinThreads / kWave; ++w) n += tokens[w];
+    const float mean = s / static_cast<float>(max(n, 1));
+    double share = 0.0;
     if (threadIdx.x < kFinExperts && e < experts) {
-        const float mean = sum[0][col] / static_cast<float>(max(n, 1));
         probs[e] = mean;
-        counts[e] = count[0][col];
-        s = static_cast<double>(count[0][col]) * static_cast<double>(mean);
+        counts[e] = m;
+        share = static_cast<double>(m) * static_cast<double>(mean);
     }
-    s = wave_sum_d(s);
-    if (gridDim.x > 1) {
-        unsigned before = 0;
-        if (threadIdx.x == 0) {
-            __hip_atomic_store(&finish->sum[blockIdx.x], s, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-            before = __hip_atomic_fetch_add(&finish->done, 1u, __ATOMIC_ACQ_REL,
-                                            __HIP_MEMORY_SCOPE_AGENT);
-        }
-        if (static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(before))) !=
-            gridDim.x - 1)
-            return;
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        s = threadIdx.x < gridDim.x
-                ? __hip_atomic_load(&finish->sum[threadIdx.x], __ATOMIC_RELAXED,
-                                    __HIP_MEMORY_SCOPE_AGENT)
-                : 0.0;
-        s = wave_sum_d(s);
-    }
-    if (threadIdx.x == 0) {
-        *loss = loss_of(s, experts, k, n, coef);
-        counts[experts] = n;
-    }
+    share = wave_sum_d(share);
+    if (threadIdx.x != 0) return;
+    const double most = static_cast<double>(k) * max(n, 1);
+    const bool number = share - share == 0.0;
+    const unsigned long long own =
+        (number ? static_cast<unsigned long long>(share / most * kShare) << 7 : 1ull << 57) + 1;
+    const unsigned long long word =
+        own + __hip_atomic_fetch_add(&finish->word, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if ((word & 127) != gridDim.x) return;
+    const double all = static_cast<double>(word >> 7 & ((1ull << 50) - 1)) / kShare * most;
+    *loss = word >> 57 ? __builtin_nanf("") : loss_of(all, experts, k, n, coef);
+    counts[experts] = n;
 }
-static_assert(kMaxExperts / kFinExperts <= kWave && kFwdBlocks <= kFinThreads,
-              "a lane for each workgroup's sum, a thread for each partial row");
+static_assert(kMaxExperts / kFinExperts < 128 && kFwdBlocks <= kFinThreads,
+              "7 bits count the workgroups; a thread for each partial row");
 
 // The counts enter less a whole number near their mean, which changes nothing (the p of a row
 // add up to 1) and keeps the bits of what is left.
-template <int T, int L, int P, bool ADD>
+template <int T, int L, int P, bool ADD, bool NT>
 __global__ __launch_bounds__(kBwdThreads) void balance_bwd_kernel(
-    const void* __restrict__ logits, void* __restrict__ dlogits, int tokens, int experts, int k,
+    const void* __restrict__ logits, void* dlogits, int tokens, int experts, int k,
     float coef, const int* __restrict__ counts, const float* __restrict__ dloss,
     const unsigned char* __restrict__ valid) {
     constexpr int PER = kBwdThreads / L;
     constexpr int N = kPiece<T, P>;
     const int gl = threadIdx.x & (L - 1);
+    const Pieces<T, L, P> at(gl, experts);
+    // read in any case: a branch would wait for what is on its way
+    const unsigned char* flags = valid ? valid : static_cast<const unsigned char*>(logits);
     int c[P];
     float sum = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const int e = gl * N + step_expert<T, L, P>(p);
-        c[p] = e < experts ? counts[e] : 0;
-        sum += static_cast<float>(c[p]);
+        c[p] = counts[at.begin[p / N] + p % N];
+        sum += at.own(p / N, p % N) ? static_cast<float>(c[p]) : 0.0f;
     }
     const int mean = static_cast<int>(
         fminf(group_sum<L>(sum) / static_cast<float>(experts), 2147483520.0f));
     float left[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int e = gl * N + step_expert<T, L, P>(p);
-        left[p] = e < experts ? static_cast<float>(c[p] - mean) : 0.0f;
-    }
+    for (int p = 0; p < P; ++p) left[p] = static_cast<float>(c[p] - mean);
     const int n = counts[experts];
     const float per = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
     const float scale = (dloss ? *dloss : 1.0f) * coef * static_cast<float>(experts) /
@@ -280,36 +351,47 @@ __global__ __launch_bounds__(kBwdThreads) void balance_bwd_kernel(
         const long long want = base + threadIdx.x / L;
         const bool inside = want < tokens;
         const size_t row = inside ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
-        const bool live = !valid || valid[row] != 0;
+        const bool live = flags[row] != 0 || !valid;
         float v[P];
         [[maybe_unused]] float old[P];
-        load_logits<T, L, P>(logits, row, tokens, gl, experts, v);
-        if constexpr (ADD) load_logits<T, L, P>(dlogits, row, tokens, gl, experts, old);
-        const float inv = softmax_terms<L, P>(v);
-        float d = 0.0f;
+        load_pieces<T, L, P, NT>(logits, row, experts, at, v);
+        if constexpr (ADD) load_pieces<T, L, P, NT>(dlogits, row, experts, at, old);
+        // e^(v - max) of shared elements is needed for what is written, not for the sum
+        float top = -__builtin_inff();
 #pragma unroll
-        for (int p = 0; p < P; ++p) d += v[p] * left[p];
+        for (int p = 0; p < P; ++p) top = at.own(p / N, p % N) ? fmaxf(top, v[p]) : top;
+        top = group_max<L>(top);
+        if (top == -__builtin_inff()) top = 0.0f;
+        float s = 0.0f, d = 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            v[p] = __builtin_amdgcn_exp2f((v[p] - top) * kLog2e);
+            const float own = at.own(p / N, p % N) ? v[p] : 0.0f;
+            s += own;
+            d += own * left[p];
+        }
+        s = group_sum<L>(s);
+        const float inv = s == 0.0f ? 0.0f : 1.0f / s;
         d = group_sum<L>(d) * inv;
         const float factor = inv * scale;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const float g = live ? v[p] * factor * (left[p] - d) : 0.0f;
-            v[p] = ADD ? old[p] + g : g;
+            v[p] = rounded(ADD ? old[p] + g : g);
         }
+        wave_order();  // the loads of what is written twice come before the stores
         if (!inside || (ADD && !live)) continue;
+        row_elem<T>* out = static_cast<row_elem<T>*>(dlogits) + row * experts;
 #pragma unroll
-        for (int p0 = 0; p0 < P; p0 += N) {
-            const int e0 = gl * N + step_expert<T, L, P>(p0);
+        for (int i = 0; i < P / N; ++i) {
+            if (!Pieces<T, L, P>::whole(i) && at.skip[i] == N) continue;
             float part[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) part[e] = v[p0 + e];
-            if (e0 + N <= experts) {
-                row_put_n<T, N>(dlogits, row * experts + e0, part);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e0 + e < experts) row_put<T>(dlogits, row * experts + e0 + e, part[e]);
-            }
+            for (int e = 0; e < N; ++e) part[e] = v[i * N + e];
+            if constexpr (N == row_vec<T>())
+                store16b(out + at.begin[i], row_pack<T>(part));
+            else
+                row_put_n<T, N>(out, at.begin[i], part);
         }
     }
 }
@@ -364,12 +446,17 @@ int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned ch
     with_row_type(type, [&](auto t) {
         with_gate_shape<false>(experts, false, [&](auto l, auto p) {
             constexpr int T = decltype(t)::value, L = decltype(l)::value, P = decltype(p)::value;
-            with_flag(blocks == 1, [&](auto one) {
-                hipLaunchKernelGGL((balance_fwd_kernel<T, L, P, decltype(one)::value>),
-                                   dim3(blocks), dim3(kFwdThreads), 0, st, logits, ids, tokens,
-                                   experts, k, valid, part, part_n, finish, counts, probs, loss,
-                                   coef);
-            });
+            auto launch = [&](auto one, auto nt) {
+                hipLaunchKernelGGL(
+                    (balance_fwd_kernel<T, L, P, decltype(one)::value, decltype(nt)::value>),
+                    dim3(blocks), dim3(kFwdThreads), 0, st, logits, ids, tokens, experts, k, valid,
+                    part, part_n, finish, counts, probs, loss, coef);
+            };
+            if (blocks == 1)
+                launch(std::true_type(), std::false_type());
+            else
+                with_flag(stream_loads(static_cast<double>(tokens) * experts * row_type_size(type)),
+                          [&](auto nt) { launch(std::false_type(), nt); });
         });
     });
     if (int rc = check_launch(name)) return rc;
@@ -388,16 +475,22 @@ int mi_moe_balance_backward(const void* logits, const unsigned char* valid, cons
     if (tokens == 0) return MI_OK;
     if (!logits || !counts || !dlogits)
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
+    hipStream_t st = to_stream(stream);
     with_row_type(type, [&](auto t) {
         with_gate_shape<false>(experts, false, [&](auto l, auto p) {
             constexpr int T = decltype(t)::value, L = decltype(l)::value, P = decltype(p)::value;
             constexpr int PER = kBwdThreads / L;
             const unsigned grid = static_cast<unsigned>(
                 std::min<long long>((static_cast<long long>(tokens) + PER - 1) / PER, kMaxGrid));
+            const bool nt = stream_loads(static_cast<double>(tokens) * experts *
+                                         row_type_size(type) * (accumulate ? 2 : 1));
             with_flag(accumulate != 0, [&](auto add) {
-                hipLaunchKernelGGL((balance_bwd_kernel<T, L, P, decltype(add)::value>), dim3(grid),
-                                   dim3(kBwdThreads), 0, to_stream(stream), logits, dlogits,
-                                   tokens, experts, k, coef, counts, dloss, valid);
+                with_flag(nt, [&](auto stream) {
+                    hipLaunchKernelGGL(
+                        (balance_bwd_kernel<T, L, P, decltype(add)::value, decltype(stream)::value>),
+                        dim3(grid), dim3(kBwdThreads), 0, st, logits, dlogits, tokens, experts, k,
+                        coef, counts, dloss, valid);
+                });
             });
         });
     });

@@ -24,33 +24,6 @@ constexpr int step_expert(int p) {
     return p / N * (N * L) + p % N;
 }
 
-// Loads them, -inf behind the last expert.  Accesses may run into the next row, and are
-// cut to single elements only at the tensor's end.
-template <int T, int L, int P>
-__device__ __forceinline__ void load_logits(const void* logits, size_t row, size_t rows, int gl,
-                                            int experts, float (&v)[P]) {
-    constexpr int N = kPiece<T, P>;
-    const size_t base = row * experts, total = rows * experts;
-#pragma unroll
-    for (int c = 0; c < P; c += N) {
-        const int e0 = gl * N + step_expert<T, L, P>(c);
-        float part[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) part[e] = 0.0f;
-        if (e0 < experts) {
-            if (base + e0 + N <= total) {
-                row_get_n<T, N>(logits, base + e0, part);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e0 + e < experts) part[e] = row_get<T>(logits, base + e0 + e);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[c + e] = e0 + e < experts ? part[e] : -__builtin_inff();
-    }
-}
-
 // f(L, P): 16 lanes a row up to 256 experts, 64 lanes above; where `wide`, 16 up to 512.
 template <bool MAY_BE_WIDE, class F>
 void with_gate_shape(int experts, bool wide, F f) {

@@ -56,6 +56,33 @@ __device__ __forceinline__ float key_value(int key) {
     return __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
 }
 
+// Loads a lane's logits of a row, -inf behind the last expert.  Accesses may run into the next row, and are
+// cut to single elements only at the tensor's end.
+template <int T, int L, int P>
+__device__ __forceinline__ void load_logits(const void* logits, size_t row, size_t rows, int gl,
+                                            int experts, float (&v)[P]) {
+    constexpr int N = kPiece<T, P>;
+    const size_t base = row * experts, total = rows * experts;
+#pragma unroll
+    for (int c = 0; c < P; c += N) {
+        const int e0 = gl * N + step_expert<T, L, P>(c);
+        float part[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) part[e] = 0.0f;
+        if (e0 < experts) {
+            if (base + e0 + N <= total) {
+                row_get_n<T, N>(logits, base + e0, part);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e0 + e < experts) part[e] = row_get<T>(logits, base + e0 + e);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[c + e] = e0 + e < experts ? part[e] : -__builtin_inff();
+    }
+}
+
 template <int CTRL>
 __device__ __forceinline__ double dpp_move_d(double v) {
     const u32x2 b = __builtin_bit_cast(u32x2, v);

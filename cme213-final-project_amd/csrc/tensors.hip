@@ -5,8 +5,10 @@
 // they are, fp32, fp16 and bf16 mixed.
 //
 // A launch takes up to kBatch tensors, described in its arguments: no table in device
-// memory has to be kept or copied, and a captured graph holds what it needs.  Tensors are
-// cut into units; a workgroup takes consecutive units, whichever tensors they are in.
+// memory has to be kept or copied, and a captured graph holds what it needs.  Where there are
+// more, the norm's launches leave their descriptions in the workspace, and one launch scales all.
+// Tensors are cut into units, numbered through the whole list; a workgroup takes consecutive
+// units, whichever tensors they are in.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -23,8 +25,9 @@ constexpr int kBatch = 96;            // tensors of a launch: 3.4 KB of argument
 constexpr int kShift = 13;            // a unit has 2^kShift elements,
 constexpr int kFewShift = 11;         // or 2^kFewShift where all tensors have less than
 constexpr long long kFew = 1ll << 23; // so many together
-constexpr int kNormBlocks = 2048;     // workgroups of the norm's launches, about
+constexpr int kNormBlocks = 2048;     // workgroups of a norm launch
 constexpr int kScaleBlocks = 131072;
+constexpr int kInPlaceBlocks = 32768;
 constexpr int kFewParts = 512;        // partial sums that every workgroup may add for itself
 constexpr int kFinThreads = 1024;
 constexpr long long kMaxUnits = 1ll << 30;
@@ -36,15 +39,25 @@ struct Tensor {
     int type, unused;
 };
 
+// The tensors of a launch, in its arguments.
 struct Batch {
     Tensor tensor[kBatch];
     unsigned end[kBatch];  // units up to the tensor's last; the largest number behind the last one
+    unsigned first;        // units before the first tensor
     int count;
     int shift;
 };
 
-// The first tensor that ends behind unit u: the number of ends up to u, which the lanes count
-// in one round trip (the arguments may lie in host memory).
+// All of a list's tensors, in device memory.
+struct Table {
+    const Tensor* tensor;
+    const unsigned* end;
+    int count;
+    int shift;
+};
+
+// The first tensor that ends behind unit u: the number of ends up to u, which the lanes count.
+// One round trip: the arguments may lie in host memory.
 __device__ __forceinline__ int tensor_of(const Batch& b, unsigned u) {
     const int lane = threadIdx.x & (kWave - 1);
     static_assert(kBatch > kWave && kBatch <= 2 * kWave, "two ends a lane");
@@ -52,18 +65,50 @@ __device__ __forceinline__ int tensor_of(const Batch& b, unsigned u) {
     return __popcll(__ballot(e0 <= u)) + __popcll(__ballot(lane < kBatch - kWave && e1 <= u));
 }
 
+// A 64th of the range at a time.
+__device__ __forceinline__ int tensor_of(const Table& b, unsigned u) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int from = 0, n = b.count;
+    while (n > 0) {
+        const int step = (n + kWave - 1) / kWave;
+        const int last = (lane + 1) * step - 1;  // of the lane's part
+        const bool before = last < n && b.end[from + last] <= u;
+        from += __popcll(__ballot(before)) * step;
+        n = step > 1 ? min(step, b.count - from) : 0;
+    }
+    return from;
+}
+
+__device__ __forceinline__ unsigned first_unit(const Batch& b, int i) {
+    return i ? b.end[i - 1] : b.first;
+}
+__device__ __forceinline__ unsigned first_unit(const Table& b, int i) {
+    return i ? b.end[i - 1] : 0u;
+}
+
 // Calls f(tensor, first element, end element) for the pieces of units [u, end).
-template <class F>
-__device__ __forceinline__ void for_pieces(const Batch& b, unsigned u, unsigned end, F f) {
+template <class List, class F>
+__device__ __forceinline__ void for_pieces(const List& b, unsigned u, unsigned end, F f) {
     if (u >= end) return;
     const int shift = b.shift;
     for (int i = __builtin_amdgcn_readfirstlane(tensor_of(b, u)); u < end; ++i) {
-        const unsigned from = i ? b.end[i - 1] : 0u, to = min(end, b.end[i]);
+        const unsigned from = first_unit(b, i), to = min(end, b.end[i]);
         const Tensor t = b.tensor[i];
         f(t, static_cast<long long>(u - from) << shift,
           min(t.size, static_cast<long long>(to - from) << shift));
         u = to;
     }
+}
+
+// A workgroup's share of `units` units from `first` on.
+struct Share {
+    unsigned begin, end;
+};
+
+__device__ __forceinline__ Share share_of(unsigned first, unsigned units) {
+    const unsigned long long n = units;
+    return {first + static_cast<unsigned>(n * blockIdx.x / gridDim.x),
+            first + static_cast<unsigned>(n * (blockIdx.x + 1ull) / gridDim.x)};
 }
 
 template <int T, bool NT>
@@ -95,18 +140,22 @@ __device__ __forceinline__ void add_squares(const void* data, long long first, l
     }
 }
 
+// tensor, end: where the descriptions go (NULL: nowhere).
 __global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(float* __restrict__ part,
                                                                  unsigned units, bool nt,
+                                                                 Tensor* __restrict__ tensor,
+                                                                 unsigned* __restrict__ end,
                                                                  const Batch b) {
     __shared__ float red[kThreads / kWave];
-    const unsigned u0 = static_cast<unsigned>(static_cast<unsigned long long>(units) * blockIdx.x /
-                                              gridDim.x);
-    const unsigned u1 = static_cast<unsigned>(static_cast<unsigned long long>(units) *
-                                              (blockIdx.x + 1ull) / gridDim.x);
+    if (tensor && blockIdx.x == 0 && static_cast<int>(threadIdx.x) < b.count) {
+        tensor[threadIdx.x] = b.tensor[threadIdx.x];
+        end[threadIdx.x] = b.end[threadIdx.x];
+    }
+    const Share u = share_of(b.first, units);
     float acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-    for_pieces(b, u0, u1, [&](const Tensor& t, long long first, long long end) {
+    for_pieces(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
         auto add = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
             if (t.type == MI_TYPE_F32)
@@ -138,8 +187,16 @@ __global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(float* __restri
 // The partial sums in 64 bits, in a fixed order; every thread gets the total.
 template <int NT>
 __device__ __forceinline__ double add_parts(const float* part, int parts, double* red) {
+    constexpr int AT_ONCE = 4;
     double s = 0.0;
-    for (int i = threadIdx.x; i < parts; i += NT) s += static_cast<double>(part[i]);
+    for (int i0 = threadIdx.x; i0 < parts; i0 += AT_ONCE * NT) {
+        float p[AT_ONCE];  // every load goes out, from a place that is there
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) p[i] = part[min(i0 + i * NT, parts - 1)];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            s += i0 + i * NT < parts ? static_cast<double>(p[i]) : 0.0;
+    }
 #pragma unroll
     for (int m = 1; m < kWave; m *= 2) s += __shfl_xor(s, m);
     if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = s;
@@ -236,11 +293,11 @@ struct Parts {
     float* clip;
 };
 
-template <bool WIDE, bool PARTS>
+template <bool WIDE, bool PARTS, class List>
 __global__ __launch_bounds__(kThreads) void tensors_scale_kernel(const float* __restrict__ scale,
-                                                                 unsigned units, bool nt,
-                                                                 const Parts parts,
-                                                                 const Batch b) {
+                                                                 unsigned first, unsigned units,
+                                                                 bool nt, const Parts parts,
+                                                                 const List b) {
     float c;
     if constexpr (PARTS) {
         __shared__ double red[kThreads / kWave];
@@ -255,11 +312,8 @@ __global__ __launch_bounds__(kThreads) void tensors_scale_kernel(const float* __
         c = *scale;
     }
     if (!WIDE && c == 1.0f) return;
-    const unsigned u0 = static_cast<unsigned>(static_cast<unsigned long long>(units) * blockIdx.x /
-                                              gridDim.x);
-    const unsigned u1 = static_cast<unsigned>(static_cast<unsigned long long>(units) *
-                                              (blockIdx.x + 1ull) / gridDim.x);
-    for_pieces(b, u0, u1, [&](const Tensor& t, long long first, long long end) {
+    const Share u = share_of(first, units);
+    for_pieces(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
         auto put = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
             if (t.type == MI_TYPE_F32)
@@ -292,14 +346,13 @@ long long units_of(long long elements, int shift) {
 struct Totals {
     long long elements = 0, units = 0;
     double bytes = 0.0;
-    int shift = kShift, batches = 0;
+    int shift = kShift, tensors = 0, batches = 0;
 };
 
 int check_list(const char* name, const List& l, Totals* total) {
     if (l.count < 0) return set_error(MI_ERR_INVALID_ARG, "%s: count=%d", name, l.count);
     if (l.count > 0 && (!l.tensors || !l.sizes))
         return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
-    int some = 0;
     for (int i = 0; i < l.count; ++i) {
         if (l.sizes[i] < 0 || l.sizes[i] > kMaxUnits << kShift)
             return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d has size %lld", name, i,
@@ -310,7 +363,7 @@ int check_list(const char* name, const List& l, Totals* total) {
         if (l.sizes[i] == 0) continue;
         if (!l.tensors[i] || (l.outs && !l.outs[i]))
             return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d: NULL pointer", name, i);
-        ++some;
+        ++total->tensors;
         total->elements += l.sizes[i];
         total->units += units_of(l.sizes[i], kShift);
         total->bytes += static_cast<double>(l.sizes[i]) * row_type_size(l.type(i));
@@ -318,7 +371,7 @@ int check_list(const char* name, const List& l, Totals* total) {
             return set_error(MI_ERR_INVALID_ARG, "%s: more than %lld elements", name,
                              kMaxUnits << kShift);
     }
-    total->batches = (some + kBatch - 1) / kBatch;
+    total->batches = (total->tensors + kBatch - 1) / kBatch;
     if (total->elements < kFew) {
         total->shift = kFewShift;
         total->units = 0;
@@ -327,13 +380,15 @@ int check_list(const char* name, const List& l, Totals* total) {
     return MI_OK;
 }
 
-// Calls f(batch, its units) for every kBatch tensors that have elements.
+// Calls f(batch, its units, tensors before it) for every kBatch tensors that have elements.
 template <class F>
 int for_batches(const List& l, int shift, F f) {
     Batch b;
     b.count = 0;
+    b.first = 0;
     b.shift = shift;
-    unsigned units = 0;
+    unsigned units = 0;  // up to here
+    int before = 0;
     for (int i = 0; i < l.count; ++i) {
         if (l.sizes[i] > 0) {
             const int n = b.count++;
@@ -344,33 +399,50 @@ int for_batches(const List& l, int shift, F f) {
         }
         if (b.count > 0 && (b.count == kBatch || i == l.count - 1)) {
             for (int n = b.count; n < kBatch; ++n) b.end[n] = UINT_MAX;
-            if (int rc = f(b, units)) return rc;
+            if (int rc = f(b, units - b.first, before)) return rc;
+            before += b.count;
             b.count = 0;
-            units = 0;
+            b.first = units;
         }
     }
     return MI_OK;
 }
 
-// Workgroups of a batch's norm launch: its share of kNormBlocks, at most a unit each.
-int norm_blocks(unsigned units, long long all) {
-    const long long share = (static_cast<long long>(kNormBlocks) * units + all - 1) / all;
-    return static_cast<int>(std::min<long long>(share, units));
+// What the library workspace holds: the norm's partial sums, the list's descriptions.
+struct Space {
+    float* part;
+    Tensor* tensor;
+    unsigned* end;
+};
+
+size_t parts_bytes(int batches) {
+    return round_up(static_cast<size_t>(kNormBlocks) * batches * sizeof(float), 256);
 }
 
-// The partial sums of all squares, in *part.
-int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t st, float** part,
+size_t space_bytes(int batches) {
+    const size_t tensors = static_cast<size_t>(kBatch) * batches;
+    return colsum_part_offset() + parts_bytes(batches) +
+           (batches > 1 ? tensors * (sizeof(Tensor) + sizeof(unsigned)) : 0);
+}
+
+// The partial sums of all squares, and where there are several batches the list's descriptions.
+int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t st, Space* space,
                int* parts) {
     int err = MI_OK;
-    char* ws = static_cast<char*>(workspace_get(mi_tensors_workspace(l.count), st, &err));
+    char* ws = static_cast<char*>(workspace_get(space_bytes(std::max(1, total.batches)), st, &err));
     if (!ws) return err;
-    *part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    const bool table = total.batches > 1;
+    space->part = reinterpret_cast<float*>(ws + colsum_part_offset());
+    space->tensor = reinterpret_cast<Tensor*>(ws + colsum_part_offset() + parts_bytes(total.batches));
+    space->end = reinterpret_cast<unsigned*>(space->tensor + kBatch * total.batches);
     *parts = 0;
     const bool nt = stream_loads(total.bytes);
-    return for_batches(l, total.shift, [&](const Batch& b, unsigned units) {
-        const int blocks = norm_blocks(units, total.units);
+    return for_batches(l, total.shift, [&](const Batch& b, unsigned units, int before) {
+        const int blocks = static_cast<int>(std::min<unsigned>(units, kNormBlocks));
         hipLaunchKernelGGL(tensors_sumsq_kernel, dim3(blocks), dim3(kThreads), 0, st,
-                           *part + *parts, units, nt, b);
+                           space->part + *parts, units, nt,
+                           table ? space->tensor + before : nullptr,
+                           table ? space->end + before : nullptr, b);
         *parts += blocks;
         return check_launch(name);
     });
@@ -383,19 +455,32 @@ int finish_norm(const char* name, const float* part, int parts, float* result, b
     return check_launch(name);
 }
 
-int scale_all(const char* name, const List& l, const Totals& total, const float* scale,
-              const Parts* parts, hipStream_t st) {
-    const bool nt = stream_loads(total.bytes);
-    return for_batches(l, total.shift, [&](const Batch& b, unsigned units) {
-        const dim3 grid(std::min<unsigned>(units, kScaleBlocks));
-        with_flag(l.outs != nullptr, [&](auto wide) {
-            with_flag(parts != nullptr, [&](auto add) {
-                hipLaunchKernelGGL(
-                    (tensors_scale_kernel<decltype(wide)::value, decltype(add)::value>), grid,
-                    dim3(kThreads), 0, st, scale, units, nt, parts ? *parts : Parts{}, b);
-            });
-        });
-        return check_launch(name);
+template <class Source>
+int launch_scale(const char* name, const List& l, const Totals& total, unsigned first,
+                 unsigned units, const float* scale, const Parts* parts, const Source& source,
+                 hipStream_t st) {
+    const unsigned most = l.outs ? kScaleBlocks : kInPlaceBlocks;
+    with_flag(l.outs != nullptr, [&](auto wide) {
+        constexpr bool WIDE = decltype(wide)::value;
+        const dim3 grid(std::min(units, most));
+        const bool nt = stream_loads(total.bytes);
+        if constexpr (std::is_same<Source, Batch>::value) {
+            if (parts) {
+                hipLaunchKernelGGL((tensors_scale_kernel<WIDE, true, Source>), grid,
+                                   dim3(kThreads), 0, st, scale, first, units, nt, *parts, source);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((tensors_scale_kernel<WIDE, false, Source>), grid, dim3(kThreads), 0,
+                           st, scale, first, units, nt, Parts{}, source);
+    });
+    return check_launch(name);
+}
+
+int scale_batches(const char* name, const List& l, const Totals& total, const float* scale,
+                  const Parts* parts, hipStream_t st) {
+    return for_batches(l, total.shift, [&](const Batch& b, unsigned units, int) {
+        return launch_scale(name, l, total, b.first, units, scale, parts, b, st);
     });
 }
 
@@ -408,9 +493,7 @@ extern "C" {
 
 size_t mi_tensors_workspace(int count) {
     if (count < 0) return 0;
-    // a launch's share of kNormBlocks is rounded up
-    return colsum_part_offset() +
-           (kNormBlocks + static_cast<size_t>(count) / kBatch + 1) * sizeof(float);
+    return space_bytes(static_cast<int>((static_cast<long long>(count) + kBatch - 1) / kBatch));
 }
 
 int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, const int* types,
@@ -422,10 +505,10 @@ int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, c
     if (!d_result) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
     if (total.units == 0) return MI_OK;
     hipStream_t st = to_stream(stream);
-    float* part = nullptr;
+    Space space;
     int parts = 0;
-    if (int rc = norm_parts(name, l, total, st, &part, &parts)) return rc;
-    return finish_norm(name, part, parts, d_result, true, nullptr, 0.0f, st);
+    if (int rc = norm_parts(name, l, total, st, &space, &parts)) return rc;
+    return finish_norm(name, space.part, parts, d_result, true, nullptr, 0.0f, st);
 }
 
 int mi_tensors_scale(const void* const* tensors, void* const* outs, const long long* sizes,
@@ -435,7 +518,7 @@ int mi_tensors_scale(const void* const* tensors, void* const* outs, const long l
     Totals total;
     if (int rc = check_list(name, l, &total)) return rc;
     if (!d_scale) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
-    return scale_all(name, l, total, d_scale, nullptr, to_stream(stream));
+    return scale_batches(name, l, total, d_scale, nullptr, to_stream(stream));
 }
 
 int mi_tensors_clip(const void* const* tensors, void* const* outs, const long long* sizes,
@@ -450,16 +533,19 @@ int mi_tensors_clip(const void* const* tensors, void* const* outs, const long lo
         return set_error(MI_ERR_INVALID_ARG, "%s: max_norm=%g", name,
                          static_cast<double>(max_norm));
     hipStream_t st = to_stream(stream);
-    float* part = nullptr;
+    Space space;
     int parts = 0;
-    if (int rc = norm_parts(name, l, total, st, &part, &parts)) return rc;
+    if (int rc = norm_parts(name, l, total, st, &space, &parts)) return rc;
     if (total.batches == 1 && parts <= kFewParts) {
-        const Parts p{part, parts, max_norm, d_norm_sq, d_clip_scale};
-        return scale_all(name, l, total, nullptr, &p, st);
+        const Parts p{space.part, parts, max_norm, d_norm_sq, d_clip_scale};
+        return scale_batches(name, l, total, nullptr, &p, st);
     }
-    if (int rc = finish_norm(name, part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
+    if (int rc = finish_norm(name, space.part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
         return rc;
-    return scale_all(name, l, total, d_clip_scale, nullptr, st);
+    if (total.batches <= 1) return scale_batches(name, l, total, d_clip_scale, nullptr, st);
+    const Table all{space.tensor, space.end, total.tensors, total.shift};
+    return launch_scale(name, l, total, 0u, static_cast<unsigned>(total.units), d_clip_scale,
+                        nullptr, all, st);
 }
 
 }  // extern "C"
