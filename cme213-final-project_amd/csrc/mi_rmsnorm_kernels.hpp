@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kGroupThreads<GT>) void rms_fwd_kernel(
                 float other[V];
                 row_unpack<T>(y[k], other);
 #pragma unroll
-                for (int e = 0; e < V; ++e) h[e] += other[e];
+                for (int e = 0; e < V; ++e) h[e] = rounded(h[e] + other[e]);
                 x[k] = row_pack<T>(h);  // as it is kept
             }
 #pragma unroll
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_walk_kernel(
         const size_t base = static_cast<size_t>(row) * cols;
         auto value = [&](int c) {
             float h = row_get<T>(a, base + c);
-            if constexpr (RESID) h += row_get<T>(b, base + c);
+            if constexpr (RESID) h = rounded(h + row_get<T>(b, base + c));
             return h;
         };
         float s = 0.0f;
@@ -473,11 +473,24 @@ __global__ __launch_bounds__(kBwdGroupThreads<GT>) void rms_bwd_kernel(
                 store16b(element_ptr<T>(dx, base + at[k].col), row_pack<T>(o));
         }
     };
-    for (long long row0 = static_cast<long long>(blockIdx.x) * PER; row0 < rows;
-         row0 += static_cast<long long>(gridDim.x) * PER) {
+    const long long stride = static_cast<long long>(gridDim.x) * PER;
+    long long row0 = static_cast<long long>(blockIdx.x) * PER;
+    if constexpr (GT <= kWave) {
+        // the next row's loads go out before a row is worked on
         Row w;
         load(row0 + grp, w);
-        process(row0 + grp, w);
+        for (; row0 < rows; row0 += stride) {
+            Row next;
+            load(row0 + stride + grp, next);
+            process(row0 + grp, w);
+            w = next;
+        }
+    } else {
+        for (; row0 < rows; row0 += stride) {
+            Row w;
+            load(row0 + grp, w);
+            process(row0 + grp, w);
+        }
     }
     float* prow = part + static_cast<size_t>(blockIdx.x) * cols;
     float* own = PER > 1 ? sums + static_cast<size_t>(grp) * cols : prow;

@@ -436,7 +436,10 @@ int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t
     space->tensor = reinterpret_cast<Tensor*>(ws + colsum_part_offset() + parts_bytes(total.batches));
     space->end = reinterpret_cast<unsigned*>(space->tensor + kBatch * total.batches);
     *parts = 0;
-    const bool nt = stream_loads(total.bytes);
+    // Streamed where nothing of it is read again soon: where a launch reads all of it next, only
+    // past 1 GB (bf16 of 215 MB, into fp32, 115 -> 102 us, of 495 MB 349 -> 318, fp32 of 990 MB 475
+    // -> 470, but bf16 of 3.1 GB 2131 -> 2160; the norm alone of 822 MB fp32 153, 171 kept).
+    const bool nt = l.outs ? total.bytes > 1073741824.0 : stream_loads(total.bytes);
     return for_batches(l, total.shift, [&](const Batch& b, unsigned units, int before) {
         const int blocks = static_cast<int>(std::min<unsigned>(units, kNormBlocks));
         hipLaunchKernelGGL(tensors_sumsq_kernel, dim3(blocks), dim3(kThreads), 0, st,
