@@ -52,20 +52,42 @@ struct Pieces {
     __device__ __forceinline__ bool own(int i, int e) const { return whole(i) || e >= skip[i]; }
 };
 
+// A row's pieces as they are in memory: converted only where they are used, so that nothing waits
+// for them before.
+template <int T, int P>
+struct RawPieces {
+    static constexpr int N = kPiece<T, P>;
+    typedef row_elem<T> small __attribute__((ext_vector_type(N < row_vec<T>() ? N : 1)));
+    typedef typename std::conditional<N == row_vec<T>(), u32x4, small>::type piece;
+    piece raw[P / N];
+    __device__ __forceinline__ void values(float (&v)[P]) const {
+#pragma unroll
+        for (int i = 0; i < P / N; ++i) {
+            float part[N];
+            if constexpr (N == row_vec<T>()) {
+                row_unpack<T>(raw[i], part);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) part[e] = static_cast<float>(raw[i][e]);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[i * N + e] = part[e];
+        }
+    }
+};
+
 template <int T, int L, int P, bool NT>
 __device__ __forceinline__ void load_pieces(const void* logits, size_t row, int experts,
-                                            const Pieces<T, L, P>& at, float (&v)[P]) {
+                                            const Pieces<T, L, P>& at, RawPieces<T, P>& r) {
     constexpr int N = Pieces<T, L, P>::N;
     const row_elem<T>* p = static_cast<const row_elem<T>*>(logits) + row * experts;
 #pragma unroll
     for (int i = 0; i < P / N; ++i) {
-        float part[N];
         if constexpr (N == row_vec<T>())
-            row_unpack<T>(load16b<NT>(p + at.begin[i]), part);
+            r.raw[i] = load16b<NT>(p + at.begin[i]);
         else
-            row_get_n<T, N>(p, at.begin[i], part);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i * N + e] = part[e];
+            r.raw[i] = load_piece<typename RawPieces<T, P>::piece>(
+                reinterpret_cast<const char*>(p + at.begin[i]));
     }
 }
 
@@ -139,47 +161,58 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
     const Pieces<T, L, P> at(gl, experts);
     const unsigned char* flags = valid ? valid : reinterpret_cast<const unsigned char*>(ids);
     struct Row {
-        float v[P];
+        RawPieces<T, P> raw;
         int id;
-        bool live;
+        unsigned char flag;
+        bool inside;
     };
     auto load = [&](long long base, Row& r) {
         const long long want = base + threadIdx.x / L;
         const bool inside = want < tokens;
         const size_t row = inside ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
-        load_pieces<T, L, P, NT>(logits, row, experts, at, r.v);
+        load_pieces<T, L, P, NT>(logits, row, experts, at, r.raw);
         r.id = ids[row * k + min(gl, k - 1)];
-        r.live = inside && (flags[row] != 0 || !valid);
+        r.flag = flags[row];
+        r.inside = inside;
     };
     const long long stride = static_cast<long long>(gridDim.x) * PER;
     long long base = static_cast<long long>(blockIdx.x) * PER;
-    Row r;
-    if (base < tokens) load(base, r);
-    for (int e = threadIdx.x; e <= experts; e += kFwdThreads) count[e] = 0;
-    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) finish->word = 0;
-    __syncthreads();
     float acc[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) acc[p] = 0.0f;
-    while (base < tokens) {
-        base += stride;
-        Row next;
-        if (base < tokens) load(base, next);
+    auto add = [&](const Row& r) {
+        const bool live_row = r.inside & ((r.flag != 0) | !valid);
+        float v[P];
+        r.raw.values(v);
 #pragma unroll
         for (int p = 0; p < P; ++p)
-            if (!at.own(p / N, p % N)) r.v[p] = -__builtin_inff();
-        const float inv = softmax_terms<L, P>(r.v);
-        const unsigned long long live = __ballot(r.live);
+            if (!at.own(p / N, p % N)) v[p] = -__builtin_inff();
+        const float inv = softmax_terms<L, P>(v);
+        const unsigned long long live = __ballot(live_row);
         if (live == ~0ull) {
 #pragma unroll
-            for (int p = 0; p < P; ++p) acc[p] += r.v[p] * inv;
+            for (int p = 0; p < P; ++p) acc[p] += v[p] * inv;
         } else {
 #pragma unroll
-            for (int p = 0; p < P; ++p) acc[p] += r.live ? r.v[p] * inv : 0.0f;
+            for (int p = 0; p < P; ++p) acc[p] += live_row ? v[p] * inv : 0.0f;
         }
-        if (r.live && gl < k && r.id >= 0 && r.id < experts) atomicAdd(&count[r.id], 1);
+        if (live_row & (gl < k) & (r.id >= 0) & (r.id < experts)) atomicAdd(&count[r.id], 1);
         if (lane == 0 && live) atomicAdd(&count[experts], __popcll(live) / L);
-        r = next;
+    };
+    // the next rows' loads go out before rows are worked on: two sets of registers in turn, for
+    // copies from one to the other would wait for the loads
+    Row r0, r1;
+    if (tokens > 0) load(base, r0);
+    for (int e = threadIdx.x; e <= experts; e += kFwdThreads) count[e] = 0;
+    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) finish->word = 0;
+    __syncthreads();
+    while (base < tokens) {
+        load(base + stride, r1);
+        add(r0);
+        if (base + stride >= tokens) break;
+        load(base + 2 * stride, r0);
+        add(r1);
+        base += 2 * stride;
     }
     // the wave's rows, then the waves
     if constexpr (L == 16) {
@@ -351,11 +384,15 @@ __global__ __launch_bounds__(kBwdThreads) void balance_bwd_kernel(
         const long long want = base + threadIdx.x / L;
         const bool inside = want < tokens;
         const size_t row = inside ? static_cast<size_t>(want) : static_cast<size_t>(tokens) - 1;
-        const bool live = flags[row] != 0 || !valid;
+        RawPieces<T, P> raw;
+        [[maybe_unused]] RawPieces<T, P> raw_old;
+        load_pieces<T, L, P, NT>(logits, row, experts, at, raw);
+        if constexpr (ADD) load_pieces<T, L, P, NT>(dlogits, row, experts, at, raw_old);
+        const bool live = (flags[row] != 0) | !valid;
         float v[P];
         [[maybe_unused]] float old[P];
-        load_pieces<T, L, P, NT>(logits, row, experts, at, v);
-        if constexpr (ADD) load_pieces<T, L, P, NT>(dlogits, row, experts, at, old);
+        raw.values(v);
+        if constexpr (ADD) raw_old.values(old);
         // e^(v - max) of shared elements is needed for what is written, not for the sum
         float top = -__builtin_inff();
 #pragma unroll

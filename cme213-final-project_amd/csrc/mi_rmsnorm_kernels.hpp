@@ -476,14 +476,17 @@ __global__ __launch_bounds__(kBwdGroupThreads<GT>) void rms_bwd_kernel(
     const long long stride = static_cast<long long>(gridDim.x) * PER;
     long long row0 = static_cast<long long>(blockIdx.x) * PER;
     if constexpr (GT <= kWave) {
-        // the next row's loads go out before a row is worked on
-        Row w;
-        load(row0 + grp, w);
-        for (; row0 < rows; row0 += stride) {
-            Row next;
-            load(row0 + stride + grp, next);
-            process(row0 + grp, w);
-            w = next;
+        // The next row's loads go out before a row is worked on: two sets of registers in turn,
+        // for copies from one to the other would wait for the loads.
+        Row w0, w1;
+        load(row0 + grp, w0);
+        while (row0 < rows) {
+            load(row0 + stride + grp, w1);
+            process(row0 + grp, w0);
+            if (row0 + stride >= rows) break;
+            load(row0 + 2 * stride + grp, w0);
+            process(row0 + stride + grp, w1);
+            row0 += 2 * stride;
         }
     } else {
         for (; row0 < rows; row0 += stride) {
