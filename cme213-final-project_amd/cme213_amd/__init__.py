@@ -680,25 +680,39 @@ class TensorList:
 
     def __init__(self, tensors, outs=None):
         import torch
+        codes = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
         self.tensors = list(tensors)
-        self.count = len(self.tensors)
+        self.count = n = len(self.tensors)
         self.out_tensors = None if outs is None else list(outs)
-        if outs is not None and len(self.out_tensors) != self.count:
-            raise ValueError(f"{self.count} tensors and {len(self.out_tensors)} outs")
-        self._data = (c_void_p * self.count)(*[_ptr(t) or None for t in self.tensors])
-        self._sizes = (c_longlong * self.count)(*[t.numel() for t in self.tensors])
-        self._types = (c_int * self.count)(*[_type_of(t, None) for t in self.tensors])
-        self._outs = None
+        if outs is not None and len(self.out_tensors) != n:
+            raise ValueError(f"{n} tensors and {len(self.out_tensors)} outs")
+        self.device = None
+        for i, t in enumerate(self.tensors):
+            if t.dtype not in codes:
+                raise ValueError(f"tensor {i} of dtype {t.dtype}: float32, float16 or bfloat16 "
+                                 "expected")
+        sizes = [t.numel() for t in self.tensors]
+        self._sizes = (c_longlong * n)(*sizes)
+        self._types = (c_int * n)(*[codes[t.dtype] for t in self.tensors])
+        self._data, self._outs = self._addresses(self.tensors), None
         if outs is not None:
-            for t, o in zip(self.tensors, self.out_tensors):
-                if o.numel() != t.numel():
-                    raise ValueError(f"an out of {o.numel()} elements for {t.numel()}")
-            self._outs = (c_void_p * self.count)(*[_ptr(o, torch.float32) or None
-                                                   for o in self.out_tensors])
-        devices = {t.get_device() for t in self.tensors + (self.out_tensors or [])}
+            for i, o in enumerate(self.out_tensors):
+                if o.dtype != torch.float32:
+                    raise ValueError(f"out {i} of dtype {o.dtype}, expected torch.float32")
+                if o.numel() != sizes[i]:
+                    raise ValueError(f"out {i} of {o.numel()} elements for {sizes[i]}")
+            self._outs = self._addresses(self.out_tensors)
+
+    def _addresses(self, tensors):
+        if not all([t.is_cuda for t in tensors]):
+            raise ValueError("tensors must live on the GPU")
+        if not all([t.is_contiguous() for t in tensors]):
+            raise ValueError("tensors must be contiguous")
+        devices = {t.get_device() for t in tensors} | ({self.device} - {None})
         if len(devices) > 1:
             raise ValueError(f"tensors on several devices: {sorted(devices)}")
         self.device = devices.pop() if devices else None
+        return (c_void_p * len(tensors))(*[t.data_ptr() or None for t in tensors])
 
     def args(self):
         """tensors, outs, sizes, types and count, for bind()."""
