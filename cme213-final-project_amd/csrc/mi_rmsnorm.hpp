@@ -53,9 +53,22 @@ constexpr int wide_steps(int type) { return type == MI_TYPE_F32 ? 3 : 2; }
 
 constexpr int kBwdThreads = 512;
 
-// Threads of a row's group in the backward kernel.
-inline int bwd_threads(int units, int steps) {
-    return units <= 16 ? 16 : units <= 32 ? 32 : units <= 64 * steps ? 64
+// Many rows whose units leave a wave's lanes idle share a wave, 16 or 32 lanes each with as many
+// units as this, at most.
+constexpr int kManyRows = 8192;
+constexpr int fwd_narrow_steps(int type) { return type == MI_TYPE_F32 ? 8 : 4; }
+constexpr int bwd_narrow_steps(int type) { return type == MI_TYPE_F32 ? 3 : 2; }
+
+// Nine tenths of a wave's lanes have a unit in every step.
+inline bool fills_wave(int units) { return units * 10 >= (units + 63) / 64 * 64 * 9; }
+
+// Threads of a row's group in the backward kernel.  [245487, 139] fp32, 35 units: a wave 108 us, 16
+// lanes 92; [88599, 342] fp16, 43 units: a wave 44.6, 32 lanes 37.5, 16 lanes 40.1; but [65536, 512]
+// bf16, 64 units: a wave 45.2, 32 lanes 47.1.
+inline int bwd_threads(int rows, int units, int type) {
+    const int steps = bwd_steps(type);
+    const int narrow = rows >= kManyRows && !fills_wave(units) ? bwd_narrow_steps(type) : 1;
+    return units <= 16 * narrow ? 16 : units <= 32 * narrow ? 32 : units <= 64 * steps ? 64
            : units <= 256 * steps ? 256 : 1024;
 }
 
@@ -67,7 +80,7 @@ inline int bwd_threads(int units, int steps) {
 inline int backward_blocks(int rows, int cols, int type) {
     int per = 1, most = 256;
     if (!walked(cols, type, 1024 * wide_steps(type))) {
-        const int units = units_of(cols, type), threads = bwd_threads(units, bwd_steps(type));
+        const int units = units_of(cols, type), threads = bwd_threads(rows, units, type);
         per = std::max(1, kBwdThreads / threads);
         const int steps = (units + threads - 1) / threads, values = 16 / row_type_size(type);
         if (threads == 256 && steps * (2 * values + 12) <= 64 && rows >= 4096) most = 512;

@@ -298,13 +298,20 @@ __global__ __launch_bounds__(kGroupThreads<GT>) void rms_fwd_kernel(
             }
             if constexpr (Q8) {
                 if constexpr (OUT == Out::Block8) {
-                    constexpr int L = MI_ROW8_BLOCK / V;  // lanes that hold a block
-                    const int skip = k == N - 1 ? at[k].skip : 0, j = t + k * GT;
-                    unsigned top = 0;
+                    constexpr int L = MI_ROW8_BLOCK / V;         // units of a block,
+                    constexpr int STEPS = L > GT ? L / GT : 1;   // in how many steps of the group
+                    const int j = t + k * GT;
+                    if (k % STEPS == 0) {
+                        unsigned top = 0;
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        top = larger(top, e < skip ? 0u : magnitude(v[k][e]));
-                    sc = scale_of(lanes_max<(L < GT ? L : GT)>(top), r, format);
+                        for (int i = k; i < k + STEPS && i < N; ++i)
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                top = larger(top, i == N - 1 && e < at[i].skip
+                                                      ? 0u
+                                                      : magnitude(v[i][e]));
+                        sc = scale_of(lanes_max<(L < GT ? L : GT)>(top), r, format);
+                    }
                     const int blocks = (cols + MI_ROW8_BLOCK - 1) / MI_ROW8_BLOCK;
                     if (stored && j % L == 0) scales[row * blocks + j / L] = sc.scale;
                 }
@@ -553,14 +560,20 @@ void with_steps(int units, F f) {
     f(std::integral_constant<int, GT>(), std::integral_constant<int, FROM>());
 }
 
-// A wave holds a row of up to 2048 columns; a few rows, and longer ones, take more waves each.
+// A wave holds a row of up to 2048 columns; a few rows, and longer ones, take more waves each.  Many
+// rows that do not fill one take 16 or 32 lanes: [34973, 339] fp16, 43 units, to e4m3 14.1 -> 9.9 us,
+// [44187, 576] bf16, 72 units, 20.6 -> 14.5, [100000, 256] fp32, 64 units, which a wave has one of a
+// lane, 31.8 -> 25.4; but [65536, 1024] bf16, 128 units, 75.1 -> 76.5.
 template <int T, class F>
 void with_fwd_shape(int rows, int units, F f) {
-    constexpr int STEPS = fwd_steps(T);
-    if (units <= 16)
-        with_steps<16, 1, 1>(units, f);
+    constexpr int STEPS = fwd_steps(T), NARROW = fwd_narrow_steps(T);
+    const bool narrow = rows >= kManyRows && (units <= 64 || !fills_wave(units));
+    if (units <= 16 || (narrow && units <= 16 * NARROW))
+        with_steps<16, 1, NARROW>(units, f);
     else if (units <= 32)
         with_steps<32, 1, 1>(units, f);
+    else if (narrow && units <= 32 * NARROW)
+        with_steps<32, NARROW / 2 + 1, NARROW>(units, f);
     else if (units <= 64 || (units <= 64 * STEPS && rows > kFewRows))
         with_steps<64, 1, STEPS>(units, f);
     else if (units <= 256 * STEPS)
@@ -613,11 +626,11 @@ void forward(const Forward& c, hipStream_t st) {
 }
 
 template <int T, class F>
-void with_bwd_shape(int units, F f) {
+void with_bwd_shape(int rows, int units, F f) {
     constexpr int STEPS = bwd_steps(T);
-    switch (bwd_threads(units, STEPS)) {
-        case 16: return with_steps<16, 1, 1>(units, f);
-        case 32: return with_steps<32, 1, 1>(units, f);
+    switch (bwd_threads(rows, units, T)) {
+        case 16: return with_steps<16, 1, bwd_narrow_steps(T)>(units, f);
+        case 32: return with_steps<32, 1, bwd_narrow_steps(T)>(units, f);
         case 64: return with_steps<64, 1, STEPS>(units, f);
         case 256: return with_steps<256, 1, STEPS>(units, f);
         default: return with_steps<1024, STEPS / 4 + 1, wide_steps(T)>(units, f);
@@ -636,7 +649,7 @@ void backward(const Backward& c, hipStream_t st) {
                                c.rows, c.cols, c.grad_out, c.x, c.inv_rms, c.gamma, c.dx, c.part);
             return;
         }
-        with_bwd_shape<T>(units_of(c.cols, T), [&](auto gt, auto n) {
+        with_bwd_shape<T>(c.rows, units_of(c.cols, T), [&](auto gt, auto n) {
             constexpr int GT = decltype(gt)::value, N = decltype(n)::value;
             constexpr int WG = kBwdGroupThreads<GT>, PER = WG / GT;
             with_flag(nt, [&](auto stream) {

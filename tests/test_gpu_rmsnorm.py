@@ -187,6 +187,54 @@ def test_backward(dev, n, c, t, resid):
     R.near("dgamma", host(DG), dg0 + dg, dg_bound + 2 * S.U * np.abs(dg0 + dg))
 
 
+MANY = [(8192, 8), (8200, 60), (9000, 116), (8193, 130), (8192, 200), (8300, 252), (8197, 256),
+        (8192, 339), (8199, 386), (8211, 450), (8192, 512), (8205, 576), (8192, 646), (8207, 771),
+        (8192, 782), (8199, 1000), (8193, 1030), (8192, 1330)]
+
+
+@pytest.mark.parametrize("t", list(R.TYPES))
+@pytest.mark.parametrize("n,c", MANY)
+def test_many_rows(dev, n, c, t):
+    """Many rows that share waves, in every number of steps: some rows against 64 bits, forward
+    with the residual as rows and in both kinds of 8 bits, backward; gamma's gradient whole."""
+    note(f"rmsnorm many rows {n}x{c} {t}")
+    r = np.random.default_rng(c)
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    a, b, dy = (torch.randn(n, c, device=dev, generator=gen).to(R.TYPES[t]) for _ in range(3))
+    gamma = (1 + 0.1 * r.standard_normal(c)).astype(np.float32)
+    A, B, DY, G = _off(a), _off(b), _off(dy), dev_t(gamma)
+    some = np.unique(np.concatenate([np.arange(20), r.integers(0, n, 60), np.arange(n - 20, n)]))
+    at = torch.from_numpy(some).to(dev)
+    g64 = gamma.astype(np.float64)
+    h, inv, y, rel_r, rel_y = S.rms(_h64(a[at]), _h64(b[at]), g64, EPS)
+    out, total, gi = torch.full_like(a, 77), torch.full_like(a, 77), torch.full((n,), 77.0, device=dev)
+    M.residual_rmsnorm_forward(A, B, G, total, out, gi, n, c, EPS)
+    _check_rows(t, out[at], y, np.full(len(some), rel_y))
+    R.near("sum", _h64(total[at]), h, S.U * np.abs(h) + R.half_step(t, h) * (1 + 2.0 ** -9))
+    R.near("inv_rms", _h64(gi[at]), inv, rel_r * inv)
+    q = torch.full((n, c), 77, dtype=torch.uint8, device=dev)
+    for block, fmt in ((0, "int8"), (128, "e4m3"), (128, "int8")):
+        code, largest, _ = FORMATS[fmt]
+        scales = torch.full((n, M.row8_scales(1, c, block)), 77.0, device=dev)
+        M.residual_rmsnorm_forward_row8(A, B, G, total, q, scales, None, None, n, c, EPS, block, code)
+        want, v = S.scales_of(y, block, largest)
+        R.near("scales", _h64(scales[at]), want, (rel_y + 2 * S.U) * want)
+        R.near("codes", S.code_values(host(q[at]), fmt), v, S.code_bound(v, fmt))
+    x, rr = total, gi
+    dg = torch.zeros(c, device=dev)
+    for resid in (False, True):
+        dx = b.clone()
+        f = M.rmsnorm_backward_residual if resid else M.rmsnorm_backward
+        f(DY, x, rr, G, dx, dg.zero_(), n, c)
+        want, bound, _, _ = S.rms_back(_h64(dy[at]), _h64(x[at]), _h64(rr[at]), g64,
+                                       _h64(b[at]) if resid else None)
+        R.near("dx", _h64(dx[at]), want, bound + R.half_step(t, want) * (1 + 2.0 ** -9))
+        terms = dy.double() * x.double() * rr.double()[:, None]
+        # as in step_ref.rms_back
+        R.near("dgamma", host(dg), host(terms.sum(0)),
+               host(terms.abs().sum(0)) * (n // 256 + 103) * S.U)
+
+
 def test_gradient_against_differences(dev):
     """The gradient of sum(c * out) by the backward call and by differences of the forward call.
     Step 2^-6: the difference's own error is about h^2 / 6 = 4e-5 of the third derivative (of
