@@ -56,7 +56,7 @@ constexpr int kBwdThreads = 512;
 // Many rows whose units leave a wave's lanes idle share a wave, 16 or 32 lanes each with as many
 // units as this, at most.
 constexpr int kManyRows = 8192;
-constexpr int fwd_narrow_steps(int type) { return type == MI_TYPE_F32 ? 8 : 4; }
+constexpr int kFwdNarrowSteps = 4;
 constexpr int bwd_narrow_steps(int type) { return type == MI_TYPE_F32 ? 3 : 2; }
 
 // Nine tenths of a wave's lanes have a unit in every step.

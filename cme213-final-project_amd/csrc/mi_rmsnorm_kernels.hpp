@@ -566,7 +566,7 @@ void with_steps(int units, F f) {
 // lane, 31.8 -> 25.4; but [65536, 1024] bf16, 128 units, 75.1 -> 76.5.
 template <int T, class F>
 void with_fwd_shape(int rows, int units, F f) {
-    constexpr int STEPS = fwd_steps(T), NARROW = fwd_narrow_steps(T);
+    constexpr int STEPS = fwd_steps(T), NARROW = kFwdNarrowSteps;
     const bool narrow = rows >= kManyRows && (units <= 64 || !fills_wave(units));
     if (units <= 16 || (narrow && units <= 16 * NARROW))
         with_steps<16, 1, NARROW>(units, f);

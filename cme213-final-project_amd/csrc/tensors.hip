@@ -21,22 +21,26 @@ namespace mi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 96;            // tensors of a launch: 3.4 KB of arguments
+constexpr int kBatch = 140;           // tensors of a launch: 3.9 KB of arguments
 constexpr int kShift = 13;            // a unit has 2^kShift elements,
 constexpr int kFewShift = 11;         // or 2^kFewShift where all tensors have less than
 constexpr long long kFew = 1ll << 23; // so many together
 constexpr int kNormBlocks = 2048;     // workgroups of a norm launch
+constexpr long long kFused = 1ll << 24;  // elements up to which the scaling launch finishes the norm,
+constexpr int kFusedParts = 1024;        // with about so many partial sums
 constexpr int kScaleBlocks = 131072;
 constexpr int kInPlaceBlocks = 32768;
-constexpr int kFewParts = 512;        // partial sums that every workgroup may add for itself
 constexpr int kFinThreads = 1024;
 constexpr long long kMaxUnits = 1ll << 30;
 
 struct Tensor {
     const void* data;
     void* out;
-    long long size;
-    int type, unused;
+    unsigned long long elements;  // and the type in the topmost byte
+    __host__ __device__ long long size() const {
+        return static_cast<long long>(elements & ((1ull << 56) - 1));
+    }
+    __host__ __device__ int type() const { return static_cast<int>(elements >> 56); }
 };
 
 // The tensors of a launch, in its arguments.
@@ -47,6 +51,8 @@ struct Batch {
     int count;
     int shift;
 };
+
+static_assert(sizeof(Batch) <= 3936, "a launch's arguments are 4 KB at most");
 
 // All of a list's tensors, in device memory.
 struct Table {
@@ -60,9 +66,15 @@ struct Table {
 // One round trip: the arguments may lie in host memory.
 __device__ __forceinline__ int tensor_of(const Batch& b, unsigned u) {
     const int lane = threadIdx.x & (kWave - 1);
-    static_assert(kBatch > kWave && kBatch <= 2 * kWave, "two ends a lane");
-    const unsigned e0 = b.end[lane], e1 = b.end[min(lane + kWave, kBatch - 1)];
-    return __popcll(__ballot(e0 <= u)) + __popcll(__ballot(lane < kBatch - kWave && e1 <= u));
+    constexpr int ENDS = (kBatch + kWave - 1) / kWave;  // a lane
+    unsigned end[ENDS];
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < ENDS; ++i) end[i] = b.end[min(lane + i * kWave, kBatch - 1)];
+#pragma unroll
+    for (int i = 0; i < ENDS; ++i)
+        before += __popcll(__ballot(lane + i * kWave < kBatch && end[i] <= u));
+    return before;
 }
 
 // A 64th of the range at a time.
@@ -95,7 +107,7 @@ __device__ __forceinline__ void for_pieces(const List& b, unsigned u, unsigned e
         const unsigned from = first_unit(b, i), to = min(end, b.end[i]);
         const Tensor t = b.tensor[i];
         f(t, static_cast<long long>(u - from) << shift,
-          min(t.size, static_cast<long long>(to - from) << shift));
+          min(t.size(), static_cast<long long>(to - from) << shift));
         u = to;
     }
 }
@@ -158,9 +170,9 @@ __global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(float* __restri
     for_pieces(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
         auto add = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
-            if (t.type == MI_TYPE_F32)
+            if (t.type() == MI_TYPE_F32)
                 add_squares<MI_TYPE_F32, NT>(t.data, first, end, acc);
-            else if (t.type == MI_TYPE_F16)
+            else if (t.type() == MI_TYPE_F16)
                 add_squares<MI_TYPE_F16, NT>(t.data, first, end, acc);
             else
                 add_squares<MI_TYPE_BF16, NT>(t.data, first, end, acc);
@@ -316,9 +328,9 @@ __global__ __launch_bounds__(kThreads) void tensors_scale_kernel(const float* __
     for_pieces(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
         auto put = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
-            if (t.type == MI_TYPE_F32)
+            if (t.type() == MI_TYPE_F32)
                 scale_piece<MI_TYPE_F32, WIDE, NT>(t, first, end, c);
-            else if (t.type == MI_TYPE_F16)
+            else if (t.type() == MI_TYPE_F16)
                 scale_piece<MI_TYPE_F16, WIDE, NT>(t, first, end, c);
             else
                 scale_piece<MI_TYPE_BF16, WIDE, NT>(t, first, end, c);
@@ -394,7 +406,8 @@ int for_batches(const List& l, int shift, F f) {
             const int n = b.count++;
             units += static_cast<unsigned>(units_of(l.sizes[i], shift));
             b.tensor[n] = {l.tensors[i], l.outs ? l.outs[i] : const_cast<void*>(l.tensors[i]),
-                           l.sizes[i], l.type(i), 0};
+                           static_cast<unsigned long long>(l.sizes[i]) |
+                               static_cast<unsigned long long>(l.type(i)) << 56};
             b.end[n] = units;
         }
         if (b.count > 0 && (b.count == kBatch || i == l.count - 1)) {
@@ -436,12 +449,14 @@ int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t
     space->tensor = reinterpret_cast<Tensor*>(ws + colsum_part_offset() + parts_bytes(total.batches));
     space->end = reinterpret_cast<unsigned*>(space->tensor + kBatch * total.batches);
     *parts = 0;
+    const unsigned most =
+        total.elements < kFused ? std::max(1, kFusedParts / std::max(1, total.batches)) : kNormBlocks;
     // Streamed where nothing of it is read again soon: where a launch reads all of it next, only
     // past 1 GB (bf16 of 215 MB, into fp32, 115 -> 102 us, of 495 MB 349 -> 318, fp32 of 990 MB 475
     // -> 470, but bf16 of 3.1 GB 2131 -> 2160; the norm alone of 822 MB fp32 153, 171 kept).
     const bool nt = l.outs ? total.bytes > 1073741824.0 : stream_loads(total.bytes);
     return for_batches(l, total.shift, [&](const Batch& b, unsigned units, int before) {
-        const int blocks = static_cast<int>(std::min<unsigned>(units, kNormBlocks));
+        const int blocks = static_cast<int>(std::min<unsigned>(units, most));
         hipLaunchKernelGGL(tensors_sumsq_kernel, dim3(blocks), dim3(kThreads), 0, st,
                            space->part + *parts, units, nt,
                            table ? space->tensor + before : nullptr,
@@ -467,15 +482,11 @@ int launch_scale(const char* name, const List& l, const Totals& total, unsigned 
         constexpr bool WIDE = decltype(wide)::value;
         const dim3 grid(std::min(units, most));
         const bool nt = stream_loads(total.bytes);
-        if constexpr (std::is_same<Source, Batch>::value) {
-            if (parts) {
-                hipLaunchKernelGGL((tensors_scale_kernel<WIDE, true, Source>), grid,
-                                   dim3(kThreads), 0, st, scale, first, units, nt, *parts, source);
-                return;
-            }
-        }
-        hipLaunchKernelGGL((tensors_scale_kernel<WIDE, false, Source>), grid, dim3(kThreads), 0,
-                           st, scale, first, units, nt, Parts{}, source);
+        with_flag(parts != nullptr, [&](auto add) {
+            hipLaunchKernelGGL((tensors_scale_kernel<WIDE, decltype(add)::value, Source>), grid,
+                               dim3(kThreads), 0, st, scale, first, units, nt,
+                               parts ? *parts : Parts{}, source);
+        });
     });
     return check_launch(name);
 }
@@ -539,16 +550,17 @@ int mi_tensors_clip(const void* const* tensors, void* const* outs, const long lo
     Space space;
     int parts = 0;
     if (int rc = norm_parts(name, l, total, st, &space, &parts)) return rc;
-    if (total.batches == 1 && parts <= kFewParts) {
-        const Parts p{space.part, parts, max_norm, d_norm_sq, d_clip_scale};
-        return scale_batches(name, l, total, nullptr, &p, st);
-    }
-    if (int rc = finish_norm(name, space.part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
-        return rc;
-    if (total.batches <= 1) return scale_batches(name, l, total, d_clip_scale, nullptr, st);
+    const bool fused = total.elements > 0 && total.elements < kFused;
+    const Parts p{space.part, parts, max_norm, d_norm_sq, d_clip_scale};
+    if (!fused)
+        if (int rc =
+                finish_norm(name, space.part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
+            return rc;
+    const float* scale = fused ? nullptr : d_clip_scale;
+    if (total.batches <= 1) return scale_batches(name, l, total, scale, fused ? &p : nullptr, st);
     const Table all{space.tensor, space.end, total.tensors, total.shift};
-    return launch_scale(name, l, total, 0u, static_cast<unsigned>(total.units), d_clip_scale,
-                        nullptr, all, st);
+    return launch_scale(name, l, total, 0u, static_cast<unsigned>(total.units), scale,
+                        fused ? &p : nullptr, all, st);
 }
 
 }  // extern "C"
