@@ -84,6 +84,8 @@ inline int backward_blocks(int rows, int cols, int type) {
         per = std::max(1, kBwdThreads / threads);
         const int steps = (units + threads - 1) / threads, values = 16 / row_type_size(type);
         if (threads == 256 && steps * (2 * values + 12) <= 64 && rows >= 4096) most = 512;
+    } else {
+        most = std::max(16, std::min(256, (1 << 25) / cols));  // 128 MB of partial rows, or 16
     }
     return static_cast<int>(
         std::min<long long>((static_cast<long long>(rows) + per - 1) / per, most));

@@ -216,6 +216,11 @@ __device__ __forceinline__ void store_codes(char* p, uint64_t q, int skip) {
 // ---------------------------------------------------------------------------
 // Forward: one row a group at a time.  out may be a (without RESID), residual_out
 // a or b: a row's loads all end before its first store.
+//
+// Bound by memory: [8192, 1600] bf16 with the residual 16.3 us (105 MB, 6.4 TB/s, partly the
+// last-level cache), [32768, 4096] to e4m3 with a scale for 128 columns 157 us (944 MB, 6.0 TB/s); 16
+// rows of 1600 by the launch (4.4 us, the kernel 2.9).  The squares' sum and a row's largest
+// |h gamma| are exchanged together: the codes need no second exchange, for r cancels in them.
 // ---------------------------------------------------------------------------
 enum class Out { Rows, Row8, Block8 };  // rows; 8 bits with a scale a row, or 128 columns
 
@@ -389,6 +394,10 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_walk_kernel(
 // Backward.  A group walks its rows, holding gamma and its columns' sums of
 // dgamma in registers; a workgroup's groups add theirs through LDS, in order, into
 // one partial row, and colsum_finalize adds the partial rows.
+//
+// Bound by memory, and the second launch: [8192, 768] fp32 into the residual stream's gradient 18.5
+// us (101 MB), [16384, 4096] bf16 92.7 us (537 MB, 5.8 TB/s; with loads that are kept in the caches
+// 100), [4095, 769] fp16, rows off any alignment, 8.3 (19 MB).
 // ---------------------------------------------------------------------------
 template <int GT>
 constexpr int kBwdGroupThreads = GT > kBwdThreads ? GT : kBwdThreads;

@@ -9,6 +9,11 @@
 // more, the norm's launches leave their descriptions in the workspace, and one launch scales all.
 // Tensors are cut into units, numbered through the whole list; a workgroup takes consecutive
 // units, whichever tensors they are in.
+//
+// Bound by memory: 434 tensors of 1.55 billion bf16 elements into fp32 2131 us, the norm 495 (6.3
+// TB/s), the scaling 1630 (9.3 GB, 5.7 TB/s; with 16 bytes read and 32 written a lane, whose stores
+// are not side by side, 1750).  In place the norm alone is read where nothing is clipped.  Small
+// lists are bound by their two launches (41 tensors of 3.7 MB 8.7 us).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -26,8 +31,13 @@ constexpr int kShift = 13;            // a unit has 2^kShift elements,
 constexpr int kFewShift = 11;         // or 2^kFewShift where all tensors have less than
 constexpr long long kFew = 1ll << 23; // so many together
 constexpr int kNormBlocks = 2048;     // workgroups of a norm launch
-constexpr long long kFused = 1ll << 24;  // elements up to which the scaling launch finishes the norm,
-constexpr int kFusedParts = 1024;        // with about so many partial sums
+// Elements up to which every workgroup of the scaling launch adds the norm's partial sums itself,
+// at most so many of them, which saves a launch: 20 tensors of 24.7 MB in place 12.4 -> 9.2 us.
+constexpr long long kFused = 1ll << 24;
+constexpr int kFusedParts = 1024;
+// Workgroups of the scaling launch, at most: short ones are faster (a billion fp32 elements in
+// place 1423 us with 131072, 1537 with 8192), but in place they mostly only read the scale and end
+// (434 tensors of 790 MB below the limit 151 us with 131072, 141 with 8192).
 constexpr int kScaleBlocks = 131072;
 constexpr int kInPlaceBlocks = 32768;
 constexpr int kFinThreads = 1024;
