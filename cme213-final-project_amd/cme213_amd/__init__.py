@@ -15,6 +15,7 @@ synchronisation see the kernels.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import os
 import re
@@ -676,7 +677,7 @@ class TensorList:
     """A program's gradients (float32, float16 and bfloat16 CUDA tensors, contiguous, on one
     device) as the mi_tensors_* calls take them, and where their clipped values go: `outs`,
     float32 tensors of as many elements each, or None for in place.  The tensors are kept alive
-    with the list; it is made once and used every step."""
+    with the list; it is made once and used every step, with the memory that they had then."""
 
     def __init__(self, tensors, outs=None):
         import torch
@@ -694,7 +695,7 @@ class TensorList:
         sizes = [t.numel() for t in self.tensors]
         self._sizes = (c_longlong * n)(*sizes)
         self._types = (c_int * n)(*[codes[t.dtype] for t in self.tensors])
-        self._data, self._outs = self._addresses(self.tensors), None
+        self._data, self._outs, self._apart = self._addresses(self.tensors), None, None
         if outs is not None:
             for i, o in enumerate(self.out_tensors):
                 if o.dtype != torch.float32:
@@ -726,6 +727,22 @@ class TensorList:
                              f"cuda:{_current_device()}")
         return self.args()
 
+    def _written(self):
+        """args(), where what is written overlaps nothing else of the list."""
+        if self._apart is None:
+            def ranges(tensors):
+                return sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                              for t in tensors if t.numel())
+            outs = ranges(self.tensors if self._outs is None else self.out_tensors)
+            self._apart = all(a[1] <= b[0] for a, b in zip(outs, outs[1:]))
+            if self._apart and self._outs is not None:
+                starts, ends = [a for a, _ in outs], [b for _, b in outs]
+                self._apart = all(bisect.bisect_right(ends, a) == bisect.bisect_left(starts, b)
+                                  for a, b in ranges(self.tensors))
+        if not self._apart:
+            raise ValueError("tensors that are written overlap others of the list")
+        return self._here()
+
 
 def tensors_norm_sq_acc(tensors, result, stream=None):
     """result += the sum of the squares of all elements of a TensorList."""
@@ -738,7 +755,7 @@ def tensors_norm_sq_acc(tensors, result, stream=None):
 def tensors_scale(tensors, scale, stream=None):
     """Every tensor of a TensorList times the device scalar, in place or into its outs."""
     import torch
-    _check(lib.mi_tensors_scale(*tensors._here(), _buf(scale, 1, torch.float32),
+    _check(lib.mi_tensors_scale(*tensors._written(), _buf(scale, 1, torch.float32),
                                 _stream(stream)))
 
 
@@ -746,7 +763,7 @@ def tensors_clip(tensors, max_norm, norm_sq, clip_scale, stream=None):
     """Clips a TensorList by its global norm: norm_sq and clip_scale are overwritten, then every
     tensor is scaled, in place or into its outs."""
     import torch
-    _check(lib.mi_tensors_clip(*tensors._here(), max_norm, _buf(norm_sq, 1, torch.float32),
+    _check(lib.mi_tensors_clip(*tensors._written(), max_norm, _buf(norm_sq, 1, torch.float32),
                                _buf(clip_scale, 1, torch.float32), _stream(stream)))
 
 

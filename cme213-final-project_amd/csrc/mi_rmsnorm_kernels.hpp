@@ -152,7 +152,7 @@ __device__ __forceinline__ Scale scale_of(unsigned top, float r, int format) {
     const float largest = format == MI_ROW8_INT8 ? 127.0f : 448.0f;
     const float v = __uint_as_float(top), m = v * r;
     if (!(m < __builtin_inff())) return {__builtin_nanf(""), 0.0f};
-    if (m >= kLeast) return {m / largest, largest / v};
+    if (m >= kLeast) return {m / largest, fminf(largest / v, 3.0e38f)};
     return {kLeast / largest, fminf(r * (largest / kLeast), 3.0e38f)};
 }
 

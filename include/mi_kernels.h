@@ -144,11 +144,12 @@ int mi_layernorm_backward_noalloc(const float* grad_out, const float* x,
 /* Beside the LayerNorm calls above; the reference has no RMS norm.  With h = x, or
  * a + b, and r = 1 / sqrt(mean(h^2) + eps) per row:  out = h r gamma.  Rows are fp32,
  * fp16 or bf16 (`type`, MI_TYPE_* below), passed as void*; gamma, inv_rms (r) and dgamma
- * are fp32.  Everything is computed in fp32, the squares' sum too (it has to stay in that
- * range), and rounded to its type at the end; out is that of the unrounded sum a + b, residual_out the rounded
- * sum.  cols is 1 to 2^24, eps finite and not negative; no alignment beyond the element's is
- * needed.  inv_rms may be NULL.  out may be x, residual_out may be a or b; other buffers must
- * not overlap.  Every result is the same bits on every call. */
+ * are fp32.  Everything is computed in fp32 (the squares' sum and h gamma have to stay in
+ * that range) and rounded to its type at the end; out is that of the unrounded sum a + b,
+ * residual_out the rounded sum.  cols is 1 to 2^24, eps finite and not negative; no alignment
+ * beyond the element's is needed.  inv_rms may be NULL.  out may be x, residual_out may be a
+ * or b; other buffers that are written must not overlap any.  Every result is the same bits on
+ * every call. */
 int mi_rmsnorm_forward(const void* x, const float* gamma, void* out, float* inv_rms, int rows,
                        int cols, float eps, int type, void* stream);
 int mi_residual_rmsnorm_forward(const void* a, const void* b, const float* gamma,
@@ -163,7 +164,8 @@ int mi_residual_rmsnorm_forward(const void* a, const void* b, const float* gamma
  *   MI_ROW8_INT8: s = m / 127, code = the integer nearest to y 127 / m;
  *   MI_ROW8_E4M3: s = m / 448, code = the OCP e4m3 number nearest to y 448 / m.
  * Half values round to even.  Where a NaN or an infinity is among them, s is NaN and the codes
- * are 0.  out (y as rows; NULL: not wanted) may be x. */
+ * are 0.  A code is that of h gamma times one factor, so y's own roundings are not in it.  out
+ * (y as rows; NULL: not wanted) may be x. */
 #define MI_ROW8_BLOCK 128
 #define MI_ROW8_INT8 0
 #define MI_ROW8_E4M3 1

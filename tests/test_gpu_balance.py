@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 COEF = 0.01
 SHAPES = [(1, 1, 1), (1, 8, 2), (16, 8, 2), (17, 16, 16), (5, 33, 4), (64, 64, 6), (300, 20, 3),
           (257, 8, 2), (256, 128, 8), (9, 160, 8), (700, 256, 1), (33, 257, 16), (450, 300, 5),
-          (270, 512, 8), (3, 1000, 3), (600, 1024, 16), (20001, 64, 6)]
+          (270, 512, 8), (3, 1000, 3), (600, 1024, 16), (20001, 64, 6), (5001, 1024, 2)]
 
 
 def _h64(t):

@@ -190,3 +190,51 @@ def test_step_replayed_from_a_graph(dev):
         calls()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(names, ref)), rep
+
+
+def test_two_graphs_share_the_workspace(dev):
+    """Two captured graphs of different shapes, replayed one after the other in either order:
+    what one leaves in the workspace does not reach the other."""
+    M.workspace_reserve(32 << 20)
+    graphs = []
+    for n, c, e, k, count in ((3000, 200, 24, 3, 300), (9001, 72, 160, 8, 500)):
+        r = np.random.default_rng(n)
+
+        def d(*shape, scale=1.0):
+            return dev_t((r.standard_normal(shape) * scale).astype(np.float32))
+        x, dy, gamma, logits = d(n, c), d(n, c), d(c), d(n, e)
+        ids = dev_t(r.integers(0, e, (n, k)).astype(np.int32))
+        grads = [d(1 + i * 97 % 500) for i in range(count)]
+        flat = torch.zeros(sum(g.numel() for g in grads), device=dev)
+        tensors = M.TensorList(grads, list(flat.split([g.numel() for g in grads])))
+        inv, dx, dg, dl = torch.ones(n, device=dev), torch.empty_like(x), torch.empty(c, device=dev), torch.empty_like(logits)
+        counts, probs = torch.empty(e + 1, dtype=torch.int32, device=dev), torch.empty(e, device=dev)
+        loss, n2, clip = torch.empty(3, 1, device=dev)
+
+        def step(n=n, c=c, e=e, k=k, x=x, dy=dy, gamma=gamma, logits=logits, ids=ids, tensors=tensors,
+                 inv=inv, dx=dx, dg=dg, dl=dl, counts=counts, probs=probs, loss=loss, n2=n2, clip=clip):
+            dg.fill_(0.0)
+            M.rmsnorm_backward(dy, x, inv, gamma, dx, dg, n, c)
+            M.moe_balance_forward(logits, ids, None, counts, probs, loss, n, e, k, COEF)
+            M.moe_balance_backward(logits, None, counts, loss, dl, n, e, k, COEF, False)
+            M.tensors_clip(tensors, 1.0, n2, clip)
+        step()
+        torch.cuda.synchronize()
+        results = [dx, dg, dl, counts, probs, loss, n2, clip, flat]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        graphs.append((graph, results, [t.clone() for t in results], step))
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for _, results, _, _ in graphs:
+            for t in results:
+                t.fill_(1)
+        for i in order:
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for _, results, want, step in graphs:
+            assert all(torch.equal(t, w) for t, w in zip(results, want)), order
+            step()
+        torch.cuda.synchronize()
+        for _, results, want, _ in graphs:
+            assert all(torch.equal(t, w) for t, w in zip(results, want)), order

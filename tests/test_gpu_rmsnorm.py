@@ -235,6 +235,41 @@ def test_many_rows(dev, n, c, t):
                host(terms.abs().sum(0)) * (n // 256 + 103) * S.U)
 
 
+@pytest.mark.parametrize("n,c", [(300, 140_003), (40, 2_097_155)])
+def test_very_long_rows(dev, n, c):
+    """Rows of so many columns that a workgroup for each would take too many partial rows: each
+    takes several rows, one after another."""
+    note(f"rmsnorm very long rows {n}x{c}")
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    a, b = (torch.randn(n, c, device=dev, generator=gen).bfloat16() for _ in range(2))
+    gamma = (1 + 0.1 * np.random.default_rng(c).standard_normal(c)).astype(np.float32)
+    G, g64 = dev_t(gamma), gamma.astype(np.float64)
+    out, total, inv = torch.empty_like(a), torch.empty_like(a), torch.empty(n, device=dev)
+    q, s = torch.empty(n, c, dtype=torch.uint8, device=dev), torch.empty(n, M.row8_scales(1, c, 128), device=dev)
+    M.residual_rmsnorm_forward_row8(a, b, G, total, q, s, out, inv, n, c, EPS, 128)
+    some = [0, 1, n - 17, n - 1]
+    _, r, y, rel_r, rel_y = S.rms(_h64(a[some]), _h64(b[some]), g64, EPS)
+    R.near("inv_rms", _h64(inv[some]), r, rel_r * r)
+    _check_rows("bf16", out[some], y, np.full(len(some), rel_y))
+    want, v = S.scales_of(y, 128, 448.0)
+    R.near("scales", _h64(s[some]), want, (rel_y + 2 * S.U) * want)
+    R.near("codes", S.code_values(host(q[some]), "e4m3"), v, S.code_bound(v, "e4m3"))
+    terms = torch.zeros(2, c, dtype=torch.float64, device=dev)
+    for i in range(n):
+        t = out[i].double() * total[i].double() * inv[i].double()
+        terms += torch.stack([t, t.abs()])
+    for resid in (False, True):
+        dx, dg = b.clone(), torch.zeros(c, device=dev)
+        f = M.rmsnorm_backward_residual if resid else M.rmsnorm_backward
+        f(out, total, inv, G, dx, dg, n, c)
+        want, bound, _, _ = S.rms_back(_h64(out[some]), _h64(total[some]), _h64(inv[some]), g64,
+                                       _h64(b[some]) if resid else None)
+        R.near("dx", _h64(dx[some]), want, bound + R.half_step("bf16", want) * (1 + 2.0 ** -9))
+        # a term's two products and fewer than 400 additions: 300 rows at most, 100 partial rows
+        # to a slice, the old value
+        R.near("dgamma", host(dg), host(terms[0]), host(terms[1]) * 403 * S.U)
+
+
 def test_gradient_against_differences(dev):
     """The gradient of sum(c * out) by the backward call and by differences of the forward call.
     Step 2^-6: the difference's own error is about h^2 / 6 = 4e-5 of the third derivative (of

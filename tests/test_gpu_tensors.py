@@ -169,6 +169,14 @@ def test_views_and_refused_lists(dev):
         M.TensorList([x], [x.half()])
     with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
         M.TensorList([x.double()])
+    # what is written may overlap nothing: two calls' worth of scaling could meet in one element
+    twice = M.TensorList([x, x.view(-1)[60:]])
+    for call in (lambda: M.tensors_scale(twice, _one(2)),
+                 lambda: M.tensors_clip(twice, 1.0, _one(0), _one(0)),
+                 lambda: M.tensors_scale(M.TensorList([x], [x]), _one(2))):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    M.tensors_norm_sq_acc(twice, _one(0))
     # the same tensor twice counts twice in the norm, and may be read twice into other buffers
     y = torch.full((10,), 2.0, device=dev)
     a, b = torch.empty(2, 10, device=dev)

@@ -136,6 +136,30 @@ def test_wrappers_check_their_tensors():
     M.tensors_scale(empty, P, stream=0)  # an empty list is a successful no-op
 
 
+def _apart(tensors, outs=None):
+    """Whether a list of host tensors would be taken where it is written (no kernel runs)."""
+    x = M.TensorList([])
+    x.tensors, x.out_tensors, x._outs = tensors, outs, None if outs is None else x._data
+    try:
+        x._written()
+        return True
+    except ValueError as e:
+        assert "overlap" in str(e)
+        return False
+
+
+def test_lists_that_are_written_must_not_overlap():
+    x, y = torch.zeros(100), torch.zeros(100)
+    assert _apart([]) and _apart([x, y]) and _apart([x[50:], x[:50], x[50:50]])
+    assert not _apart([x, x]) and not _apart([x[:51], y, x[50:]]) and not _apart([x, x[3:4]])
+    assert not _apart([x.half(), y, y[99:].view(torch.float16)])
+    # the tensors may overlap each other where they are only read
+    assert _apart([x, x], [y[:50], y[50:]]) and _apart([x[:51], x[50:]], [y[1:], y[:1]])
+    assert not _apart([x, y], [y[:50], torch.zeros(5)]) and not _apart([x, x], [y, y[10:20]])
+    assert not _apart([x[10:20]], [x]) and not _apart([x], [x[99:]]) and not _apart([x], [x])
+    assert _apart([x[10:20]], [x[20:30]]) and _apart([x[10:20], y], [x[20:30], x[:10]])
+
+
 def test_plain_codes_are_the_nearest():
     r = np.random.default_rng(0)
     y = r.standard_normal((20, 300)) * np.exp2(r.integers(-20, 20, (20, 1)))
