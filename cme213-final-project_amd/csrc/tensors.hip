@@ -7,6 +7,8 @@
 // A launch takes up to kBatch tensors, described in its arguments: no table in device
 // memory has to be kept or copied, and a captured graph holds what it needs.  Where there are
 // more, the norm's launches leave their descriptions in the workspace, and one launch scales all.
+// A launch with such arguments costs 4.3 us of the host's time, of however many tensors, so that
+// small lists take as long as their launches: tensors are described in few bytes.
 // Tensors are cut into units, numbered through the whole list; a workgroup takes consecutive
 // units, whichever tensors they are in.
 //
@@ -26,7 +28,9 @@ namespace mi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 140;           // tensors of a launch: 3.9 KB of arguments
+// Tensors of a launch, in at most 3.9 KB of arguments: in place, or with outs.
+template <bool WIDE>
+constexpr int kBatch = WIDE ? 192 : 320;
 constexpr int kShift = 13;            // a unit has 2^kShift elements,
 constexpr int kFewShift = 11;         // or 2^kFewShift where all tensors have less than
 constexpr long long kFew = 1ll << 23; // so many together
@@ -43,47 +47,71 @@ constexpr int kInPlaceBlocks = 32768;
 constexpr int kFinThreads = 1024;
 constexpr long long kMaxUnits = 1ll << 30;
 
+// A tensor's address, above it (13 bits) the elements of its last unit less one, and its type.
+using Packed = unsigned long long;
+constexpr int kAddressBits = 48;
+constexpr int kTypeShift = 61;
+static_assert(kAddressBits + kShift == kTypeShift, "the last unit's elements fit between");
+
+Packed pack(const void* data, long long elements, int type, int shift) {
+    const unsigned long long last = static_cast<unsigned long long>(elements - 1) & ((1ull << shift) - 1);
+    return reinterpret_cast<Packed>(data) | last << kAddressBits |
+           static_cast<Packed>(type) << kTypeShift;
+}
+
 struct Tensor {
     const void* data;
     void* out;
-    unsigned long long elements;  // and the type in the topmost byte
-    __host__ __device__ long long size() const {
-        return static_cast<long long>(elements & ((1ull << 56) - 1));
-    }
-    __host__ __device__ int type() const { return static_cast<int>(elements >> 56); }
+    long long elements;
+    int type;
 };
 
 // The tensors of a launch, in its arguments.
-struct Batch {
-    Tensor tensor[kBatch];
-    unsigned end[kBatch];  // units up to the tensor's last; the largest number behind the last one
-    unsigned first;        // units before the first tensor
+template <bool WIDE>
+struct Batch;
+template <>
+struct Batch<false> {
+    Packed tensor[kBatch<false>];
+    unsigned end[kBatch<false>];  // units up to the tensor's last; the largest number behind the last one
+    unsigned first;               // units before the first tensor
+    int count;
+    int shift;
+};
+template <>
+struct Batch<true> {
+    Packed tensor[kBatch<true>];
+    void* out[kBatch<true>];
+    unsigned end[kBatch<true>];
+    unsigned first;
     int count;
     int shift;
 };
 
-static_assert(sizeof(Batch) <= 3936, "a launch's arguments are 4 KB at most");
+static_assert(sizeof(Batch<false>) <= 3936 && sizeof(Batch<true>) <= 3936,
+              "a launch's arguments are 4 KB at most");
 
-// All of a list's tensors, in device memory.
+// All of a list's tensors, in device memory.  out: NULL in place.
 struct Table {
-    const Tensor* tensor;
-    const unsigned* end;
+    Packed* tensor;
+    void** out;
+    unsigned* end;
     int count;
     int shift;
 };
 
 // The first tensor that ends behind unit u: the number of ends up to u, which the lanes count.
 // One round trip: the arguments may lie in host memory.
-__device__ __forceinline__ int tensor_of(const Batch& b, unsigned u) {
+template <bool WIDE>
+__device__ __forceinline__ int tensor_of(const Batch<WIDE>& b, unsigned u) {
     const int lane = threadIdx.x & (kWave - 1);
-    constexpr int ENDS = (kBatch + kWave - 1) / kWave;  // a lane
+    constexpr int ENDS = kBatch<WIDE> / kWave;  // a lane
+    static_assert(kBatch<WIDE> % kWave == 0, "every lane has as many");
     unsigned end[ENDS];
     int before = 0;
 #pragma unroll
-    for (int i = 0; i < ENDS; ++i) end[i] = b.end[min(lane + i * kWave, kBatch - 1)];
+    for (int i = 0; i < ENDS; ++i) end[i] = b.end[lane + i * kWave];
 #pragma unroll
-    for (int i = 0; i < ENDS; ++i)
-        before += __popcll(__ballot(lane + i * kWave < kBatch && end[i] <= u));
+    for (int i = 0; i < ENDS; ++i) before += __popcll(__ballot(end[i] <= u));
     return before;
 }
 
@@ -101,7 +129,8 @@ __device__ __forceinline__ int tensor_of(const Table& b, unsigned u) {
     return from;
 }
 
-__device__ __forceinline__ unsigned first_unit(const Batch& b, int i) {
+template <bool WIDE>
+__device__ __forceinline__ unsigned first_unit(const Batch<WIDE>& b, int i) {
     return i ? b.end[i - 1] : b.first;
 }
 __device__ __forceinline__ unsigned first_unit(const Table& b, int i) {
@@ -109,15 +138,24 @@ __device__ __forceinline__ unsigned first_unit(const Table& b, int i) {
 }
 
 // Calls f(tensor, first element, end element) for the pieces of units [u, end).
-template <class List, class F>
+template <bool WIDE, class List, class F>
 __device__ __forceinline__ void for_pieces(const List& b, unsigned u, unsigned end, F f) {
     if (u >= end) return;
     const int shift = b.shift;
     for (int i = __builtin_amdgcn_readfirstlane(tensor_of(b, u)); u < end; ++i) {
-        const unsigned from = first_unit(b, i), to = min(end, b.end[i]);
-        const Tensor t = b.tensor[i];
+        const unsigned from = first_unit(b, i), all = b.end[i], to = min(end, all);
+        const Packed p = b.tensor[i];
+        Tensor t;
+        t.data = reinterpret_cast<const void*>(p & ((1ull << kAddressBits) - 1));
+        if constexpr (WIDE)
+            t.out = b.out[i];
+        else
+            t.out = const_cast<void*>(t.data);
+        t.elements = (static_cast<long long>(all - from - 1u) << shift) +
+                     static_cast<int>(p >> kAddressBits & ((1u << kShift) - 1u)) + 1;
+        t.type = static_cast<int>(p >> kTypeShift);
         f(t, static_cast<long long>(u - from) << shift,
-          min(t.size(), static_cast<long long>(to - from) << shift));
+          min(t.elements, static_cast<long long>(to - from) << shift));
         u = to;
     }
 }
@@ -162,27 +200,30 @@ __device__ __forceinline__ void add_squares(const void* data, long long first, l
     }
 }
 
-// tensor, end: where the descriptions go (NULL: nowhere).
+// table: where the descriptions go (tensor NULL: nowhere).
+template <bool WIDE>
 __global__ __launch_bounds__(kThreads) void tensors_sumsq_kernel(float* __restrict__ part,
                                                                  unsigned units, bool nt,
-                                                                 Tensor* __restrict__ tensor,
-                                                                 unsigned* __restrict__ end,
-                                                                 const Batch b) {
+                                                                 const Table table,
+                                                                 const Batch<WIDE> b) {
     __shared__ float red[kThreads / kWave];
-    if (tensor && blockIdx.x == 0 && static_cast<int>(threadIdx.x) < b.count) {
-        tensor[threadIdx.x] = b.tensor[threadIdx.x];
-        end[threadIdx.x] = b.end[threadIdx.x];
+    if (table.tensor && blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < b.count; i += kThreads) {
+            table.tensor[i] = b.tensor[i];
+            table.end[i] = b.end[i];
+            if constexpr (WIDE) table.out[i] = b.out[i];
+        }
     }
     const Share u = share_of(b.first, units);
     float acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-    for_pieces(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
+    for_pieces<false>(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
         auto add = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
-            if (t.type() == MI_TYPE_F32)
+            if (t.type == MI_TYPE_F32)
                 add_squares<MI_TYPE_F32, NT>(t.data, first, end, acc);
-            else if (t.type() == MI_TYPE_F16)
+            else if (t.type == MI_TYPE_F16)
                 add_squares<MI_TYPE_F16, NT>(t.data, first, end, acc);
             else
                 add_squares<MI_TYPE_BF16, NT>(t.data, first, end, acc);
@@ -335,12 +376,12 @@ __global__ __launch_bounds__(kThreads) void tensors_scale_kernel(const float* __
     }
     if (!WIDE && c == 1.0f) return;
     const Share u = share_of(first, units);
-    for_pieces(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
+    for_pieces<WIDE>(b, u.begin, u.end, [&](const Tensor& t, long long first, long long end) {
         auto put = [&](auto stream) {
             constexpr bool NT = decltype(stream)::value;
-            if (t.type() == MI_TYPE_F32)
+            if (t.type == MI_TYPE_F32)
                 scale_piece<MI_TYPE_F32, WIDE, NT>(t, first, end, c);
-            else if (t.type() == MI_TYPE_F16)
+            else if (t.type == MI_TYPE_F16)
                 scale_piece<MI_TYPE_F16, WIDE, NT>(t, first, end, c);
             else
                 scale_piece<MI_TYPE_BF16, WIDE, NT>(t, first, end, c);
@@ -371,6 +412,10 @@ struct Totals {
     int shift = kShift, tensors = 0, batches = 0;
 };
 
+int batches_of(int tensors, int most) {
+    return static_cast<int>((static_cast<long long>(tensors) + most - 1) / most);
+}
+
 int check_list(const char* name, const List& l, Totals* total) {
     if (l.count < 0) return set_error(MI_ERR_INVALID_ARG, "%s: count=%d", name, l.count);
     if (l.count > 0 && (!l.tensors || !l.sizes))
@@ -385,6 +430,8 @@ int check_list(const char* name, const List& l, Totals* total) {
         if (l.sizes[i] == 0) continue;
         if (!l.tensors[i] || (l.outs && !l.outs[i]))
             return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d: NULL pointer", name, i);
+        if (reinterpret_cast<uintptr_t>(l.tensors[i]) >> kAddressBits)
+            return set_error(MI_ERR_INVALID_ARG, "%s: tensor %d is at no address", name, i);
         ++total->tensors;
         total->elements += l.sizes[i];
         total->units += units_of(l.sizes[i], kShift);
@@ -393,7 +440,7 @@ int check_list(const char* name, const List& l, Totals* total) {
             return set_error(MI_ERR_INVALID_ARG, "%s: more than %lld elements", name,
                              kMaxUnits << kShift);
     }
-    total->batches = (total->tensors + kBatch - 1) / kBatch;
+    total->batches = batches_of(total->tensors, l.outs ? kBatch<true> : kBatch<false>);
     if (total->elements < kFew) {
         total->shift = kFewShift;
         total->units = 0;
@@ -403,9 +450,10 @@ int check_list(const char* name, const List& l, Totals* total) {
 }
 
 // Calls f(batch, its units, tensors before it) for every kBatch tensors that have elements.
-template <class F>
+template <bool WIDE, class F>
 int for_batches(const List& l, int shift, F f) {
-    Batch b;
+    constexpr int MOST = kBatch<WIDE>;
+    Batch<WIDE> b;
     b.count = 0;
     b.first = 0;
     b.shift = shift;
@@ -415,13 +463,12 @@ int for_batches(const List& l, int shift, F f) {
         if (l.sizes[i] > 0) {
             const int n = b.count++;
             units += static_cast<unsigned>(units_of(l.sizes[i], shift));
-            b.tensor[n] = {l.tensors[i], l.outs ? l.outs[i] : const_cast<void*>(l.tensors[i]),
-                           static_cast<unsigned long long>(l.sizes[i]) |
-                               static_cast<unsigned long long>(l.type(i)) << 56};
+            b.tensor[n] = pack(l.tensors[i], l.sizes[i], l.type(i), shift);
+            if constexpr (WIDE) b.out[n] = l.outs[i];
             b.end[n] = units;
         }
-        if (b.count > 0 && (b.count == kBatch || i == l.count - 1)) {
-            for (int n = b.count; n < kBatch; ++n) b.end[n] = UINT_MAX;
+        if (b.count > 0 && (b.count == MOST || i == l.count - 1)) {
+            for (int n = b.count; n < MOST; ++n) b.end[n] = UINT_MAX;
             if (int rc = f(b, units - b.first, before)) return rc;
             before += b.count;
             b.count = 0;
@@ -434,30 +481,39 @@ int for_batches(const List& l, int shift, F f) {
 // What the library workspace holds: the norm's partial sums, the list's descriptions.
 struct Space {
     float* part;
-    Tensor* tensor;
-    unsigned* end;
+    Table table;
 };
 
 size_t parts_bytes(int batches) {
     return round_up(static_cast<size_t>(kNormBlocks) * batches * sizeof(float), 256);
 }
 
+template <bool WIDE>
 size_t space_bytes(int batches) {
-    const size_t tensors = static_cast<size_t>(kBatch) * batches;
-    return colsum_part_offset() + parts_bytes(batches) +
-           (batches > 1 ? tensors * (sizeof(Tensor) + sizeof(unsigned)) : 0);
+    const size_t tensors = static_cast<size_t>(kBatch<WIDE>) * batches;
+    const size_t each = sizeof(Packed) + (WIDE ? sizeof(void*) : 0) + sizeof(unsigned);
+    return colsum_part_offset() + parts_bytes(batches) + (batches > 1 ? tensors * each : 0);
 }
 
 // The partial sums of all squares, and where there are several batches the list's descriptions.
+template <bool WIDE>
 int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t st, Space* space,
                int* parts) {
     int err = MI_OK;
-    char* ws = static_cast<char*>(workspace_get(space_bytes(std::max(1, total.batches)), st, &err));
+    char* ws = static_cast<char*>(
+        workspace_get(space_bytes<WIDE>(std::max(1, total.batches)), st, &err));
     if (!ws) return err;
-    const bool table = total.batches > 1;
     space->part = reinterpret_cast<float*>(ws + colsum_part_offset());
-    space->tensor = reinterpret_cast<Tensor*>(ws + colsum_part_offset() + parts_bytes(total.batches));
-    space->end = reinterpret_cast<unsigned*>(space->tensor + kBatch * total.batches);
+    space->table = Table{};
+    if (total.batches > 1) {
+        const size_t most = static_cast<size_t>(kBatch<WIDE>) * total.batches;
+        Packed* tensor =
+            reinterpret_cast<Packed*>(ws + colsum_part_offset() + parts_bytes(total.batches));
+        void** out = reinterpret_cast<void**>(tensor + most);
+        space->table = Table{tensor, WIDE ? out : nullptr,
+                             reinterpret_cast<unsigned*>(WIDE ? out + most : out), total.tensors,
+                             total.shift};
+    }
     *parts = 0;
     const unsigned most =
         total.elements < kFused ? std::max(1, kFusedParts / std::max(1, total.batches)) : kNormBlocks;
@@ -465,12 +521,16 @@ int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t
     // past 1 GB (bf16 of 215 MB, into fp32, 115 -> 102 us, of 495 MB 349 -> 318, fp32 of 990 MB 475
     // -> 470, but bf16 of 3.1 GB 2131 -> 2160; the norm alone of 822 MB fp32 153, 171 kept).
     const bool nt = l.outs ? total.bytes > 1073741824.0 : stream_loads(total.bytes);
-    return for_batches(l, total.shift, [&](const Batch& b, unsigned units, int before) {
+    return for_batches<WIDE>(l, total.shift, [&](const Batch<WIDE>& b, unsigned units, int before) {
         const int blocks = static_cast<int>(std::min<unsigned>(units, most));
-        hipLaunchKernelGGL(tensors_sumsq_kernel, dim3(blocks), dim3(kThreads), 0, st,
-                           space->part + *parts, units, nt,
-                           table ? space->tensor + before : nullptr,
-                           table ? space->end + before : nullptr, b);
+        Table table = space->table;
+        if (table.tensor) {
+            table.tensor += before;
+            table.end += before;
+            if (WIDE) table.out += before;
+        }
+        hipLaunchKernelGGL(tensors_sumsq_kernel<WIDE>, dim3(blocks), dim3(kThreads), 0, st,
+                           space->part + *parts, units, nt, table, b);
         *parts += blocks;
         return check_launch(name);
     });
@@ -483,29 +543,44 @@ int finish_norm(const char* name, const float* part, int parts, float* result, b
     return check_launch(name);
 }
 
-template <class Source>
-int launch_scale(const char* name, const List& l, const Totals& total, unsigned first,
-                 unsigned units, const float* scale, const Parts* parts, const Source& source,
-                 hipStream_t st) {
-    const unsigned most = l.outs ? kScaleBlocks : kInPlaceBlocks;
-    with_flag(l.outs != nullptr, [&](auto wide) {
-        constexpr bool WIDE = decltype(wide)::value;
-        const dim3 grid(std::min(units, most));
-        const bool nt = stream_loads(total.bytes);
-        with_flag(parts != nullptr, [&](auto add) {
-            hipLaunchKernelGGL((tensors_scale_kernel<WIDE, decltype(add)::value, Source>), grid,
-                               dim3(kThreads), 0, st, scale, first, units, nt,
-                               parts ? *parts : Parts{}, source);
-        });
+template <bool WIDE, class Source>
+int launch_scale(const char* name, const Totals& total, unsigned first, unsigned units,
+                 const float* scale, const Parts* parts, const Source& source, hipStream_t st) {
+    const dim3 grid(std::min<unsigned>(units, WIDE ? kScaleBlocks : kInPlaceBlocks));
+    const bool nt = stream_loads(total.bytes);
+    with_flag(parts != nullptr, [&](auto add) {
+        hipLaunchKernelGGL((tensors_scale_kernel<WIDE, decltype(add)::value, Source>), grid,
+                           dim3(kThreads), 0, st, scale, first, units, nt,
+                           parts ? *parts : Parts{}, source);
     });
     return check_launch(name);
 }
 
+template <bool WIDE>
 int scale_batches(const char* name, const List& l, const Totals& total, const float* scale,
                   const Parts* parts, hipStream_t st) {
-    return for_batches(l, total.shift, [&](const Batch& b, unsigned units, int) {
-        return launch_scale(name, l, total, b.first, units, scale, parts, b, st);
+    return for_batches<WIDE>(l, total.shift, [&](const Batch<WIDE>& b, unsigned units, int) {
+        return launch_scale<WIDE>(name, total, b.first, units, scale, parts, b, st);
     });
+}
+
+template <bool WIDE>
+int clip(const char* name, const List& l, const Totals& total, float max_norm, float* d_norm_sq,
+         float* d_clip_scale, hipStream_t st) {
+    Space space;
+    int parts = 0;
+    if (int rc = norm_parts<WIDE>(name, l, total, st, &space, &parts)) return rc;
+    const bool fused = total.elements > 0 && total.elements < kFused;
+    const Parts p{space.part, parts, max_norm, d_norm_sq, d_clip_scale};
+    if (!fused)
+        if (int rc =
+                finish_norm(name, space.part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
+            return rc;
+    const float* scale = fused ? nullptr : d_clip_scale;
+    if (total.batches <= 1)
+        return scale_batches<WIDE>(name, l, total, scale, fused ? &p : nullptr, st);
+    return launch_scale<WIDE>(name, total, 0u, static_cast<unsigned>(total.units), scale,
+                              fused ? &p : nullptr, space.table, st);
 }
 
 }  // namespace
@@ -517,7 +592,8 @@ extern "C" {
 
 size_t mi_tensors_workspace(int count) {
     if (count < 0) return 0;
-    return space_bytes(static_cast<int>((static_cast<long long>(count) + kBatch - 1) / kBatch));
+    // with outs: fewer tensors a launch, in as many bytes, than in place
+    return space_bytes<true>(batches_of(count, kBatch<true>));
 }
 
 int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, const int* types,
@@ -531,7 +607,7 @@ int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, c
     hipStream_t st = to_stream(stream);
     Space space;
     int parts = 0;
-    if (int rc = norm_parts(name, l, total, st, &space, &parts)) return rc;
+    if (int rc = norm_parts<false>(name, l, total, st, &space, &parts)) return rc;
     return finish_norm(name, space.part, parts, d_result, true, nullptr, 0.0f, st);
 }
 
@@ -542,7 +618,9 @@ int mi_tensors_scale(const void* const* tensors, void* const* outs, const long l
     Totals total;
     if (int rc = check_list(name, l, &total)) return rc;
     if (!d_scale) return set_error(MI_ERR_INVALID_ARG, "%s: NULL pointer", name);
-    return scale_batches(name, l, total, d_scale, nullptr, to_stream(stream));
+    hipStream_t st = to_stream(stream);
+    return outs ? scale_batches<true>(name, l, total, d_scale, nullptr, st)
+                : scale_batches<false>(name, l, total, d_scale, nullptr, st);
 }
 
 int mi_tensors_clip(const void* const* tensors, void* const* outs, const long long* sizes,
@@ -557,20 +635,8 @@ int mi_tensors_clip(const void* const* tensors, void* const* outs, const long lo
         return set_error(MI_ERR_INVALID_ARG, "%s: max_norm=%g", name,
                          static_cast<double>(max_norm));
     hipStream_t st = to_stream(stream);
-    Space space;
-    int parts = 0;
-    if (int rc = norm_parts(name, l, total, st, &space, &parts)) return rc;
-    const bool fused = total.elements > 0 && total.elements < kFused;
-    const Parts p{space.part, parts, max_norm, d_norm_sq, d_clip_scale};
-    if (!fused)
-        if (int rc =
-                finish_norm(name, space.part, parts, d_norm_sq, false, d_clip_scale, max_norm, st))
-            return rc;
-    const float* scale = fused ? nullptr : d_clip_scale;
-    if (total.batches <= 1) return scale_batches(name, l, total, scale, fused ? &p : nullptr, st);
-    const Table all{space.tensor, space.end, total.tensors, total.shift};
-    return launch_scale(name, l, total, 0u, static_cast<unsigned>(total.units), scale,
-                        fused ? &p : nullptr, all, st);
+    return outs ? clip<true>(name, l, total, max_norm, d_norm_sq, d_clip_scale, st)
+                : clip<false>(name, l, total, max_norm, d_norm_sq, d_clip_scale, st);
 }
 
 }  // extern "C"

@@ -16,8 +16,9 @@ pytestmark = pytest.mark.gpu
 # elements of each tensor: around the unit of 8192 and a step of 1024 or 2048
 LISTS = {"one": [1], "none": [0], "empty": [], "odd": [7, 0, 1, 8191, 8192, 8193, 3, 0],
          "one large": [300_001], "many": [5 + 37 * i % 3000 for i in range(500)],
-         "a batch": [100] * 140, "a batch and one": [100] * 141,
-         "three batches, large": [40_000 + 97 * i for i in range(400)], "mixed": [1 << 20, 5, 99_999, 17, 1025] * 7}
+         "a batch with outs": [100] * 192, "and one": [100] * 193, "a batch": [100] * 320,
+         "a batch and one": [100] * 321, "three batches": [1 + 53 * i % 700 for i in range(700)],
+         "batches, large": [40_000 + 97 * i for i in range(400)], "mixed": [1 << 20, 5, 99_999, 17, 1025] * 7}
 
 
 def _h64(t):
