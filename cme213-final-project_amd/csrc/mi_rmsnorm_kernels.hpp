@@ -31,6 +31,10 @@ namespace rms {
 
 constexpr int kThreads = 256;
 constexpr int kMaxGrid = 1 << 20;  // workgroups over the rows, which are taken in strides
+// What reads one row and writes 8 bits moves so little that starting a workgroup for each counts:
+// [32768, 4096] bf16 to e4m3 81 -> 75 us, [20000, 8192] 100 -> 91; but with the residual, or a row
+// out, they are the faster ones ([32768, 4096] with both 157 -> 161, [100000, 768] fp32 96 -> 101).
+constexpr int kRow8Grid = 8192;
 constexpr int kFewRows = 1024;
 constexpr float kLeast = 0x1p-100f;  // a row or block counts as at least this large
 
@@ -573,9 +577,13 @@ void with_steps(int units, F f) {
 // rows that do not fill one take 16 or 32 lanes: [34973, 339] fp16, 43 units, to e4m3 14.1 -> 9.9 us,
 // [44187, 576] bf16, 72 units, 20.6 -> 14.5, [100000, 256] fp32, 64 units, which a wave has one of a
 // lane, 31.8 -> 25.4; but [65536, 1024] bf16, 128 units, 75.1 -> 76.5.
-template <int T, class F>
+// 16-bit rows of up to 4096 columns, without the residual, that are too long for a wave take two:
+// [39009, 2688] bf16 to e4m3 75 -> 65, as rows 74 -> 71; but with the residual [30227, 3469] 150 ->
+// 154, and fp32 [11872, 4000] 45 -> 50.
+template <int T, bool RESID, class F>
 void with_fwd_shape(int rows, int units, F f) {
     constexpr int STEPS = fwd_steps(T), NARROW = kFwdNarrowSteps;
+    constexpr bool PAIRS = T != MI_TYPE_F32 && !RESID;
     const bool narrow = rows >= kManyRows && (units <= 64 || !fills_wave(units));
     if (units <= 16 || (narrow && units <= 16 * NARROW))
         with_steps<16, 1, NARROW>(units, f);
@@ -585,36 +593,39 @@ void with_fwd_shape(int rows, int units, F f) {
         with_steps<32, NARROW / 2 + 1, NARROW>(units, f);
     else if (units <= 64 || (units <= 64 * STEPS && rows > kFewRows))
         with_steps<64, 1, STEPS>(units, f);
+    else if (PAIRS && units <= 128 * STEPS && rows > kFewRows)
+        with_steps<PAIRS ? 128 : 256, STEPS / 2 + 1, STEPS>(units, f);
     else if (units <= 256 * STEPS)
         with_steps<256, 1, STEPS>(units, f);
     else
         with_steps<1024, STEPS / 4 + 1, wide_steps(T)>(units, f);
 }
 
-inline unsigned row_grid(int rows, int per) {
+inline unsigned row_grid(int rows, int per, int most) {
     return static_cast<unsigned>(
-        std::min<long long>((static_cast<long long>(rows) + per - 1) / per, kMaxGrid));
+        std::min<long long>((static_cast<long long>(rows) + per - 1) / per, most));
 }
 
 template <int T, bool RESID, Out OUT>
 void launch_forward(const Forward& c, hipStream_t st) {
     char* q = static_cast<char*>(c.q);
     if (walked(c.cols, T, 1024 * wide_steps(T))) {
-        hipLaunchKernelGGL((rms_fwd_walk_kernel<T, RESID, OUT>), dim3(row_grid(c.rows, 1)),
+        hipLaunchKernelGGL((rms_fwd_walk_kernel<T, RESID, OUT>), dim3(row_grid(c.rows, 1, kMaxGrid)),
                            dim3(kThreads), 0, st, c.rows, c.cols, c.a, c.b, c.gamma,
                            c.residual_out, c.out, c.eps, c.inv_rms, q, c.scales, c.format);
         return;
     }
     const bool nt = stream_loads(static_cast<double>(c.rows) * c.cols * row_type_size(T) *
                                  (RESID ? 2 : 1));
-    with_fwd_shape<T>(c.rows, units_of(c.cols, T), [&](auto gt, auto n) {
+    const int most = !RESID && !c.out ? kRow8Grid : kMaxGrid;
+    with_fwd_shape<T, RESID>(c.rows, units_of(c.cols, T), [&](auto gt, auto n) {
         constexpr int GT = decltype(gt)::value, N = decltype(n)::value;
         // a few rows alone have four waves for what one holds: they are never streamed
         constexpr bool FEW = GT == 256 && N <= fwd_steps(T) / 4;
         with_flag(nt && !FEW, [&](auto stream) {
             constexpr bool NT = decltype(stream)::value && !FEW;
             hipLaunchKernelGGL((rms_fwd_kernel<T, GT, N, RESID, OUT, NT>),
-                               dim3(row_grid(c.rows, kGroupThreads<GT> / GT)),
+                               dim3(row_grid(c.rows, kGroupThreads<GT> / GT, most)),
                                dim3(kGroupThreads<GT>), 0, st, c.rows, c.cols, c.a, c.b, c.gamma,
                                c.residual_out, c.out, c.eps, c.inv_rms, q, c.scales, c.format);
         });

@@ -18,7 +18,7 @@ EPS = 1e-5
 # rows up to 1024 take more waves each than more rows do; widths on both sides of each step
 SHAPES = [(1, 1), (5, 3), (3, 7), (1, 8), (4, 4), (2, 64), (9, 100), (5, 127), (16, 129), (33, 256),
           (7, 257), (3, 300), (17, 512), (2, 516), (17, 768), (1030, 769), (1025, 1026), (1027, 1300),
-          (1026, 1600), (1025, 2047), (4, 1600), (3, 2050), (2, 3999), (5, 4096), (3, 5003), (2, 6145),
+          (1026, 1600), (1025, 2047), (1026, 2101), (1025, 3002), (1026, 4093), (4, 1600), (3, 2050), (2, 3999), (5, 4096), (3, 5003), (2, 6145),
           (2, 8192), (1, 8200), (3, 12289), (2, 16384), (1, 16387), (1, 40001)]
 FORMATS = {"int8": (M.ROW8_INT8, 127.0, torch.int8), "e4m3": (M.ROW8_E4M3, 448.0, torch.float8_e4m3fn)}
 
@@ -233,6 +233,36 @@ def test_many_rows(dev, n, c, t):
         # as in step_ref.rms_back
         R.near("dgamma", host(dg), host(terms.sum(0)),
                host(terms.abs().sum(0)) * (n // 256 + 103) * S.U)
+
+
+@pytest.mark.parametrize("t", list(R.TYPES))
+@pytest.mark.parametrize("n,c", [(140_001, 60), (40_003, 600), (17_001, 2101), (8_300, 4200)])
+def test_more_rows_than_workgroups(dev, n, c, t):
+    """Rows in 8 bits, without the residual: a workgroup takes several, one after another."""
+    note(f"rmsnorm more rows than workgroups {n}x{c} {t}")
+    r = np.random.default_rng(c)
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    a = torch.randn(n, c, device=dev, generator=gen).to(R.TYPES[t])
+    gamma = (1 + 0.1 * r.standard_normal(c)).astype(np.float32)
+    A, G = _off(a), dev_t(gamma)
+    some = np.unique(np.concatenate([np.arange(20), r.integers(0, n, 80), np.arange(n - 20, n)]))
+    at = torch.from_numpy(some).to(dev)
+    _, inv, y, rel_r, rel_y = S.rms(_h64(a[at]), None, gamma.astype(np.float64), EPS)
+    q = torch.full((n + 1, c), 77, dtype=torch.uint8, device=dev)
+    for block, fmt in ((0, "int8"), (128, "e4m3")):
+        code, largest, _ = FORMATS[fmt]
+        scales = torch.full((n + 1, M.row8_scales(1, c, block)), 77.0, device=dev)
+        gi = torch.full((n + 1,), 77.0, device=dev)
+        M.rmsnorm_forward_row8(A, G, q, scales, None, gi, n, c, EPS, block, code)
+        want, v = S.scales_of(y, block, largest)
+        R.near("inv_rms", _h64(gi[at]), inv, rel_r * inv)
+        R.near("scales", _h64(scales[at]), want, (rel_y + 2 * S.U) * want)
+        R.near("codes", S.code_values(host(q[at]), fmt), v, S.code_bound(v, fmt))
+        # in place of the input's rows, and none left out
+        assert (scales[:n] < 77).all() and (scales[n:] == 77).all() and (q[n] == 77).all()
+        q0, s0, X = q.clone(), scales.clone(), A.clone()
+        M.rmsnorm_forward_row8(X, G, q.fill_(77), scales.fill_(77), X, None, n, c, EPS, block, code)
+        assert torch.equal(q, q0) and torch.equal(scales, s0)
 
 
 @pytest.mark.parametrize("n,c", [(300, 140_003), (40, 2_097_155)])
