@@ -36,6 +36,7 @@ constexpr int kMaxGrid = 1 << 20;  // workgroups over the rows, which are taken 
 // out, they are the faster ones ([32768, 4096] with both 157 -> 161, [100000, 768] fp32 96 -> 101).
 constexpr int kRow8Grid = 8192;
 constexpr int kFewRows = 1024;
+constexpr int kLine = 128;  // bytes of a cache line
 constexpr float kLeast = 0x1p-100f;  // a row or block counts as at least this large
 
 template <int GT>
@@ -580,11 +581,20 @@ void with_steps(int units, F f) {
 // 16-bit rows of up to 4096 columns, without the residual, that are too long for a wave take two:
 // [39009, 2688] bf16 to e4m3 75 -> 65, as rows 74 -> 71; but with the residual [30227, 3469] 150 ->
 // 154, and fp32 [11872, 4000] 45 -> 50.
+//
+// Streamed rows that end inside cache lines take a wave where one unit a lane is enough, with the
+// residual, or for nine tenths of its lanes: a part of a wave's access to each of several rows
+// splits a line at either end ([120000, 500] bf16 with the residual 108 -> 81, without 80 -> 67,
+// [148883, 403] with it 112 -> 86; but [302114, 331] without 83 -> 89, and whole lines, [157108,
+// 384] with it, 67 -> 75).
 template <int T, bool RESID, class F>
-void with_fwd_shape(int rows, int units, F f) {
+void with_fwd_shape(int rows, int cols, bool streamed, F f) {
     constexpr int STEPS = fwd_steps(T), NARROW = kFwdNarrowSteps;
     constexpr bool PAIRS = T != MI_TYPE_F32 && !RESID;
-    const bool narrow = rows >= kManyRows && (units <= 64 || !fills_wave(units));
+    const int units = units_of(cols, T);
+    const bool split = streamed && cols * row_type_size(T) % kLine != 0;
+    const bool narrow =
+        rows >= kManyRows && (units > 64 ? !fills_wave(units) : !split || !(RESID || fills_wave(units)));
     if (units <= 16 || (narrow && units <= 16 * NARROW))
         with_steps<16, 1, NARROW>(units, f);
     else if (units <= 32)
@@ -618,7 +628,7 @@ void launch_forward(const Forward& c, hipStream_t st) {
     const bool nt = stream_loads(static_cast<double>(c.rows) * c.cols * row_type_size(T) *
                                  (RESID ? 2 : 1));
     const int most = !RESID && !c.out ? kRow8Grid : kMaxGrid;
-    with_fwd_shape<T, RESID>(c.rows, units_of(c.cols, T), [&](auto gt, auto n) {
+    with_fwd_shape<T, RESID>(c.rows, c.cols, nt, [&](auto gt, auto n) {
         constexpr int GT = decltype(gt)::value, N = decltype(n)::value;
         // a few rows alone have four waves for what one holds: they are never streamed
         constexpr bool FEW = GT == 256 && N <= fwd_steps(T) / 4;

@@ -236,9 +236,11 @@ def test_many_rows(dev, n, c, t):
 
 
 @pytest.mark.parametrize("t", list(R.TYPES))
-@pytest.mark.parametrize("n,c", [(140_001, 60), (40_003, 600), (17_001, 2101), (8_300, 4200)])
+@pytest.mark.parametrize("n,c", [(140_001, 60), (40_003, 600), (17_001, 2101), (8_300, 4200),
+                                 (290_001, 251)])
 def test_more_rows_than_workgroups(dev, n, c, t):
-    """Rows in 8 bits, without the residual: a workgroup takes several, one after another."""
+    """Rows in 8 bits, without the residual: a workgroup takes several, one after another.  Rows
+    with it, among them rows that are streamed and end inside cache lines."""
     note(f"rmsnorm more rows than workgroups {n}x{c} {t}")
     r = np.random.default_rng(c)
     gen = torch.Generator(device="cuda").manual_seed(c)
@@ -263,6 +265,13 @@ def test_more_rows_than_workgroups(dev, n, c, t):
         q0, s0, X = q.clone(), scales.clone(), A.clone()
         M.rmsnorm_forward_row8(X, G, q.fill_(77), scales.fill_(77), X, None, n, c, EPS, block, code)
         assert torch.equal(q, q0) and torch.equal(scales, s0)
+    # a + a, exactly twice as large
+    out, total = torch.full_like(a, 77), torch.full_like(a, 77)
+    M.residual_rmsnorm_forward(A, A, G, total, out, gi, n, c, EPS)
+    h, inv, y, rel_r, rel_y = S.rms(_h64(a[at]), _h64(a[at]), gamma.astype(np.float64), EPS)
+    R.near("inv_rms", _h64(gi[at]), inv, rel_r * inv)
+    _check_rows(t, out[at], y, np.full(len(some), rel_y))
+    assert torch.equal(total, a + a)
 
 
 @pytest.mark.parametrize("n,c", [(300, 140_003), (40, 2_097_155)])
