@@ -117,7 +117,8 @@ def balance(l, ids, valid, k, coef):
     some = some[(some >= 0) & (some < experts)]
     counts = np.bincount(some, minlength=experts)
     probs = p.sum(0) / max(n, 1)
-    # tokens of a lane one after another (32 a trip of 256 workgroups), 4 + 8 + 256 partial rows
+    # tokens of a lane one after another (16 or 64 a trip of each of 256 workgroups, of which 8 are
+    # counted here), 4 + 8 lanes and waves, 256 partial rows
     chain = n_tokens // (256 * 8) + 280
     bound = (p * rel).sum(0) / max(n, 1) + (chain + 3) * U * probs
     scale = coef * experts / (k * max(n, 1))
@@ -149,7 +150,9 @@ def balance_back(l, valid, counts, dloss, k, coef):
 # ----- clipping ---------------------------------------------------------------------------
 
 def norm_chain(total):
-    """Additions of a square: a thread's part of its workgroup's elements (2048 workgroups of
-    256 threads with 8 sums each at 16 bits, 4 at fp32, whole units of 8192 elements), 8 sums,
-    lanes and waves."""
-    return total // (2048 * 256 * 4) + 8192 // (256 * 4) + 8 + 16
+    """Additions of a square in fp32: a thread's part of its workgroup's elements (at least 2048
+    workgroups, or 1024 over the launches of fewer than 2^24 elements, 256 where these are four and
+    one has all; 256 threads with 4 sums each; whole units of 8192 elements), 8 sums, lanes and
+    waves."""
+    workgroups = 2048 if total >= 1 << 24 else 256
+    return total // (workgroups * 256 * 4) + 8192 // (256 * 4) + 8 + 16
