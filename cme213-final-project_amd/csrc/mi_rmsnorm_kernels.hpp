@@ -227,6 +227,19 @@ __device__ __forceinline__ void store_codes(char* p, uint64_t q, int skip) {
 // rows of 1600 by the launch (4.4 us, the kernel 2.9).  The squares' sum and a row's largest
 // |h gamma| are exchanged together: the codes need no second exchange, for r cancels in them.
 // ---------------------------------------------------------------------------
+
+// The workgroup's turn among the rows.  Consecutive workgroups run on different XCDs, each with its
+// own L2: of every 128 those on one XCD take consecutive rows, which share cache lines where rows
+// end inside them ([40000, 2143] fp16 with the residual to e4m3 155 -> 142 us, [12000, 8111] bf16
+// 166 -> 162, [32768, 4096] to e4m3 157 -> 156; the backward kernel, whose workgroups take many
+// rows, gains nothing by it, and takes longer with consecutive rows each, 171 -> 187).
+__device__ __forceinline__ unsigned rows_turn() {
+    constexpr unsigned XCDS = 8, EACH = 16, ALL = XCDS * EACH;
+    const unsigned b = blockIdx.x;
+    if (b >= gridDim.x / ALL * ALL) return b;
+    return b / ALL * ALL + b % XCDS * EACH + b / XCDS % EACH;
+}
+
 enum class Out { Rows, Row8, Block8 };  // rows; 8 bits with a scale a row, or 128 columns
 
 template <int T, int GT, int N, bool RESID, Out OUT, bool NT>
@@ -241,7 +254,7 @@ __global__ __launch_bounds__(kGroupThreads<GT>) void rms_fwd_kernel(
     GroupRed<GT> group{red};
     const int t = threadIdx.x & (GT - 1);
     const int units = (cols + V - 1) / V;
-    for (long long row0 = static_cast<long long>(blockIdx.x) * PER; row0 < rows;
+    for (long long row0 = static_cast<long long>(rows_turn()) * PER; row0 < rows;
          row0 += static_cast<long long>(gridDim.x) * PER) {
         const long long want = row0 + threadIdx.x / GT;
         const bool valid = want < rows;  // the others repeat the last row and store nothing
