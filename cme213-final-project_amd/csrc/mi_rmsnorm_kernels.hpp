@@ -218,16 +218,6 @@ __device__ __forceinline__ void store_codes(char* p, uint64_t q, int skip) {
     if (n & 1) store_piece(p, static_cast<uint8_t>(q));
 }
 
-// ---------------------------------------------------------------------------
-// Forward: one row a group at a time.  out may be a (without RESID), residual_out
-// a or b: a row's loads all end before its first store.
-//
-// Bound by memory: [8192, 1600] bf16 with the residual 16.3 us (105 MB, 6.4 TB/s, partly the
-// last-level cache), [32768, 4096] to e4m3 with a scale for 128 columns 157 us (944 MB, 6.0 TB/s); 16
-// rows of 1600 by the launch (4.4 us, the kernel 2.9).  The squares' sum and a row's largest
-// |h gamma| are exchanged together: the codes need no second exchange, for r cancels in them.
-// ---------------------------------------------------------------------------
-
 // The workgroup's turn among the rows.  Consecutive workgroups run on different XCDs, each with its
 // own L2: of every 128 those on one XCD take consecutive rows, which share cache lines where rows
 // end inside them ([40000, 2143] fp16 with the residual to e4m3 155 -> 142 us, [12000, 8111] bf16
@@ -240,6 +230,15 @@ __device__ __forceinline__ unsigned rows_turn() {
     return b / ALL * ALL + b % XCDS * EACH + b / XCDS % EACH;
 }
 
+// ---------------------------------------------------------------------------
+// Forward: one row a group at a time.  out may be a (without RESID), residual_out
+// a or b: a row's loads all end before its first store.
+//
+// Bound by memory: [8192, 1600] bf16 with the residual 16.3 us (105 MB, 6.4 TB/s, partly the
+// last-level cache), [32768, 4096] to e4m3 with a scale for 128 columns 157 us (944 MB, 6.0 TB/s); 16
+// rows of 1600 by the launch (4.4 us, the kernel 2.9).  The squares' sum and a row's largest
+// |h gamma| are exchanged together: the codes need no second exchange, for r cancels in them.
+// ---------------------------------------------------------------------------
 enum class Out { Rows, Row8, Block8 };  // rows; 8 bits with a scale a row, or 128 columns
 
 template <int T, int GT, int N, bool RESID, Out OUT, bool NT>

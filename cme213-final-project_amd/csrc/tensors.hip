@@ -13,7 +13,7 @@
 // units, whichever tensors they are in.
 //
 // Bound by memory: 434 tensors of 1.55 billion bf16 elements into fp32 2131 us, the norm 495 (6.3
-// TB/s), the scaling 1630 (9.3 GB, 5.7 TB/s; with 16 bytes read and 32 written a lane, whose stores
+// TB/s), the scaling 1660 (9.3 GB, 5.6 TB/s; with 16 bytes read and 32 written a lane, whose stores
 // are not side by side, 1750).  In place the norm alone is read where nothing is clipped.  Small
 // lists are bound by their two launches (41 tensors of 3.7 MB 8.7 us).
 #include <algorithm>
