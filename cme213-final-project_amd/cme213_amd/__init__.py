@@ -260,8 +260,9 @@ class Bound:
     sizes, scalars), for callers that issue the same call many times: a
     call costs the ctypes dispatch alone, not the per-call tensor checks and
     conversions of the wrapper functions.  The stream is torch's current one
-    at call time unless one was given.  The tensors are kept alive with the
-    binding.  Raises MIError on a non-zero status, like the wrappers."""
+    at call time unless one was given.  The tensors, and a TensorList whose
+    args() are among the arguments, are kept alive with the binding.  Raises
+    MIError on a non-zero status, like the wrappers."""
 
     def __init__(self, name, *args, stream=None):
         import torch
@@ -270,7 +271,7 @@ class Bound:
         if len(args) != len(types) - 1:
             raise TypeError(f"{name}: {len(types) - 1} arguments before the stream, "
                             f"got {len(args)}")
-        self._keep = [a for a in args if isinstance(a, torch.Tensor)]
+        self._keep = [a for a in args if isinstance(a, (torch.Tensor, _ListAddress))]
         conv = []
         for a, t in zip(args, types[:-1]):
             if isinstance(a, torch.Tensor):
@@ -673,6 +674,15 @@ def rmsnorm_backward_residual(grad_out, x, inv_rms, gamma, grad_residual, dgamma
 
 # ----- gradients in many tensors ----------------------------------------------------
 
+class _ListAddress(int):
+    """Address of a host array of a TensorList, which lives as long as the address."""
+
+    def __new__(cls, address, tensors):
+        a = super().__new__(cls, address)
+        a.tensors = tensors
+        return a
+
+
 class TensorList:
     """A program's gradients (float32, float16 and bfloat16 CUDA tensors, contiguous, on one
     device) as the mi_tensors_* calls take them, and where their clipped values go: `outs`,
@@ -703,6 +713,8 @@ class TensorList:
                 if o.numel() != sizes[i]:
                     raise ValueError(f"out {i} of {o.numel()} elements for {sizes[i]}")
             self._outs = self._addresses(self.out_tensors)
+        self._arrays = tuple(None if a is None else ctypes.addressof(a)
+                             for a in (self._data, self._outs, self._sizes, self._types))
 
     def _addresses(self, tensors):
         if not all([t.is_cuda for t in tensors]):
@@ -716,16 +728,16 @@ class TensorList:
         return (c_void_p * len(tensors))(*[t.data_ptr() or None for t in tensors])
 
     def args(self):
-        """tensors, outs, sizes, types and count, for bind()."""
-        return (ctypes.addressof(self._data),
-                None if self._outs is None else ctypes.addressof(self._outs),
-                ctypes.addressof(self._sizes), ctypes.addressof(self._types), self.count)
+        """tensors, outs, sizes, types and count, for bind() or the library's own functions.  The
+        list lives as long as they do."""
+        return tuple(None if a is None else _ListAddress(a, self)
+                     for a in self._arrays) + (self.count,)
 
     def _here(self):
         if self.device is not None and self.device != _current_device():
             raise ValueError(f"tensors on cuda:{self.device}, the current device is "
                              f"cuda:{_current_device()}")
-        return self.args()
+        return self._arrays + (self.count,)
 
     def _written(self):
         """args(), where what is written overlaps nothing else of the list."""
