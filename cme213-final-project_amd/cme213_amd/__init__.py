@@ -261,8 +261,10 @@ class Bound:
     call costs the ctypes dispatch alone, not the per-call tensor checks and
     conversions of the wrapper functions.  The stream is torch's current one
     at call time unless one was given.  The tensors, and a TensorList whose
-    args() are among the arguments, are kept alive with the binding.  Raises
-    MIError on a non-zero status, like the wrappers."""
+    args() are among the arguments, are kept alive with the binding.  A
+    list's own checks are made: that what is written overlaps nothing else of
+    it, once, and the current device, at every call.  Raises MIError on a
+    non-zero status, like the wrappers."""
 
     def __init__(self, name, *args, stream=None):
         import torch
@@ -280,8 +282,17 @@ class Bound:
                 conv.append(t(a) if a is not None else None)
         self._fn, self._args, self._stream = fn, tuple(conv), stream
         self.name = name
+        self._device = None  # of its lists
+        for x in {id(a.tensors): a.tensors for a in args if isinstance(a, _ListAddress)}.values():
+            if name in ("mi_tensors_scale", "mi_tensors_clip"):
+                # without its outs a list's tensors are what is written
+                (x if args[1] is not None else TensorList(x.tensors))._written()
+            _same_device(x.device)
+            self._device = x.device
 
     def __call__(self):
+        if self._device is not None:
+            _same_device(self._device)
         st = self._stream
         if st is None:
             st = _current_stream()
@@ -674,6 +685,12 @@ def rmsnorm_backward_residual(grad_out, x, inv_rms, gamma, grad_residual, dgamma
 
 # ----- gradients in many tensors ----------------------------------------------------
 
+def _same_device(device):
+    if device is not None and device != _current_device():
+        raise ValueError(f"tensors on cuda:{device}, the current device is "
+                         f"cuda:{_current_device()}")
+
+
 class _ListAddress(int):
     """Address of a host array of a TensorList, which lives as long as the address."""
 
@@ -734,9 +751,7 @@ class TensorList:
                      for a in self._arrays) + (self.count,)
 
     def _here(self):
-        if self.device is not None and self.device != _current_device():
-            raise ValueError(f"tensors on cuda:{self.device}, the current device is "
-                             f"cuda:{_current_device()}")
+        _same_device(self.device)
         return self._arrays + (self.count,)
 
     def _written(self):

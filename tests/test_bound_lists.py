@@ -76,3 +76,42 @@ def test_the_arguments_alone_keep_the_list():
     del keeper, args
     gc.collect()
     assert ref() is None
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_bound_call_makes_the_lists_checks(name, monkeypatch):
+    """What is written overlaps nothing else of the list; the current device is the tensors', when
+    the call is bound and when it is made."""
+    def args(tensors, outs=None):
+        return M.TensorList([Stand(*t) for t in tensors],
+                            outs and [Stand(*t) for t in outs]).args()
+    writes = name != "mi_tensors_norm_sq_acc"
+    apart = args([(0x1000, 64), (0x1100, 10)])
+    for bad in (args([(0x1000, 65), (0x1100, 10)]), args([(0x1000, 4), (0x1000, 4)]),
+                args([(0x1000, 4)], [(0x1000, 4)]), args([(0x1000, 4)] * 2, [(0x2000, 4), (0x2008, 4)])):
+        if writes:
+            with pytest.raises(ValueError, match="overlap"):
+                _bind(name, bad)
+        else:
+            _bind(name, bad)
+    _bind(name, apart)
+    _bind(name, args([(0x1000, 4), (0x1000, 4)], [(0x2000, 4), (0x2010, 4)]))
+    if writes:  # a list with outs, bound without them: its tensors are what is written
+        both = args([(0x1000, 4), (0x1008, 4)], [(0x2000, 4), (0x2010, 4)])
+        _bind(name, both)
+        with pytest.raises(ValueError, match="overlap"):
+            _bind(name, (both[0], None) + both[2:])
+    elsewhere = args([(0x1000, 4, torch.float32, 1)])
+    with pytest.raises(ValueError, match="current device"):
+        _bind(name, elsewhere)
+    calls = []
+    monkeypatch.setattr(M.lib, name, lambda *a: calls.append(a) or M.MI_OK)
+    monkeypatch.setattr(M, "_current_stream", lambda: None)
+    bound = _bind(name, apart)
+    bound()
+    monkeypatch.setattr(M, "_current_device", lambda: 1)
+    with pytest.raises(ValueError, match="current device"):
+        bound()
+    assert len(calls) == 1
+    _bind(name, elsewhere)()
+    assert len(calls) == 2
