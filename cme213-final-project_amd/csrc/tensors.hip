@@ -488,8 +488,10 @@ size_t parts_bytes(int batches) {
     return round_up(static_cast<size_t>(kNormBlocks) * batches * sizeof(float), 256);
 }
 
+// Without tensors the norm is written all the same, through one batch's place.
 template <bool WIDE>
 size_t space_bytes(int batches) {
+    batches = std::max(1, batches);
     const size_t tensors = static_cast<size_t>(kBatch<WIDE>) * batches;
     const size_t each = sizeof(Packed) + (WIDE ? sizeof(void*) : 0) + sizeof(unsigned);
     return colsum_part_offset() + parts_bytes(batches) + (batches > 1 ? tensors * each : 0);
@@ -500,8 +502,7 @@ template <bool WIDE>
 int norm_parts(const char* name, const List& l, const Totals& total, hipStream_t st, Space* space,
                int* parts) {
     int err = MI_OK;
-    char* ws = static_cast<char*>(
-        workspace_get(space_bytes<WIDE>(std::max(1, total.batches)), st, &err));
+    char* ws = static_cast<char*>(workspace_get(space_bytes<WIDE>(total.batches), st, &err));
     if (!ws) return err;
     space->part = reinterpret_cast<float*>(ws + colsum_part_offset());
     space->table = Table{};

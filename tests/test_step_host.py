@@ -114,6 +114,11 @@ def test_tensor_list_refusals():
     assert M.lib.mi_tensors_workspace(-1) == 0
 
 
+def test_workspace_of_a_list_without_tensors():
+    """Clipping it still writes the norm, through the partial sums' place of one launch: 2048."""
+    assert M.lib.mi_tensors_workspace(0) == M.lib.mi_tensors_workspace(1) == 256 + 2048 * 4
+
+
 def test_wrappers_check_their_tensors():
     x = torch.zeros(4, 8)
     for f in (lambda: M.rmsnorm_forward(x, x, x, None, 4, 8),
