@@ -345,7 +345,9 @@ __global__ __launch_bounds__(kGroupThreads<GT>) void rms_fwd_kernel(
 }
 
 // Forward, rows of less than a unit or more than the registers hold: a workgroup a row,
-// which it walks twice.  A wave takes 128 columns at a time, the columns of a scale.
+// which it walks twice.  A wave takes 128 columns at a time, the columns of a scale.  A thread adds
+// up to 65536 columns one after another, in 64 bits: in 32 the roundings of equal values go the
+// same way, and the sum is off by 9e-4.
 template <int T, bool RESID, Out OUT>
 __global__ __launch_bounds__(kThreads) void rms_fwd_walk_kernel(
     int rows, int cols, const void* a, const void* b, const float* __restrict__ gamma,
@@ -363,12 +365,13 @@ __global__ __launch_bounds__(kThreads) void rms_fwd_walk_kernel(
             if constexpr (RESID) h = rounded(h + row_get<T>(b, base + c));
             return h;
         };
-        float s = 0.0f;
+        double s = 0.0;
         for (int c = threadIdx.x; c < cols; c += kThreads) {
             const float h = value(c);
-            s += h * h;
+            s += static_cast<double>(h) * static_cast<double>(h);
         }
-        const float r = 1.0f / sqrtf(group.sum(s) / static_cast<float>(cols) + eps);
+        const float mean = group.sum(static_cast<float>(s)) / static_cast<float>(cols);
+        const float r = 1.0f / sqrtf(mean + eps);
         Scale sc{};
         if constexpr (OUT == Out::Row8) {
             unsigned top = 0;
@@ -546,7 +549,8 @@ __global__ __launch_bounds__(kBwdGroupThreads<GT>) void rms_bwd_kernel(
 }
 
 // Backward, rows of less than a unit or too long for registers: a workgroup walks a row twice
-// and keeps its columns' sums in its partial row, each column with one thread.
+// and keeps its columns' sums in its partial row, each column with one thread.  A row's products
+// are added in 64 bits, as the forward kernel's squares are.
 template <int T, bool ADD>
 __global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
     int rows, int cols, const void* dy, const void* __restrict__ x,
@@ -559,10 +563,11 @@ __global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const size_t base = static_cast<size_t>(row) * cols;
         const float r = inv_rms[row];
-        float s = 0.0f;
+        double s = 0.0;
         for (int c = threadIdx.x; c < cols; c += kThreads)
-            s += row_get<T>(dy, base + c) * (row_get<T>(x, base + c) * r) * gamma[c];
-        const float m = group.sum(s) / static_cast<float>(cols);
+            s += static_cast<double>(row_get<T>(dy, base + c) * (row_get<T>(x, base + c) * r)) *
+                 static_cast<double>(gamma[c]);
+        const float m = group.sum(static_cast<float>(s)) / static_cast<float>(cols);
         for (int c = threadIdx.x; c < cols; c += kThreads) {
             const float d = row_get<T>(dy, base + c), n = row_get<T>(x, base + c) * r;
             float v = r * (d * gamma[c] - n * m);
