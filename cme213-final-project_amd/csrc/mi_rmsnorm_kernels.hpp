@@ -148,24 +148,36 @@ struct GroupRed {
 
 // The scale of values v r (v = h gamma) whose largest magnitude of v has the bits `top`, and
 // what v is multiplied by (0 where one of them is no number: their codes are 0, the scale NaN).
-// r, the same for all of them, cancels in the codes and adds no rounding to them.
+// r, the same for all of them, cancels in the codes and adds no rounding to them.  The factor of
+// the smallest v passes fp32's range (where r is large, as eps far below its usual sizes allows):
+// they are first multiplied by kUp, exactly.  Others need no factor above 2^119.
 struct Scale {
     float scale, mul;
+    bool up;
 };
+constexpr float kUp = 0x1p64f, kSmall = 0x1p-110f;
 
 __device__ __forceinline__ Scale scale_of(unsigned top, float r, int format) {
     const float largest = format == MI_ROW8_INT8 ? 127.0f : 448.0f;
     const float v = __uint_as_float(top), m = v * r;
-    if (!(m < __builtin_inff())) return {__builtin_nanf(""), 0.0f};
-    if (m >= kLeast) return {m / largest, fminf(largest / v, 3.0e38f)};
-    return {kLeast / largest, fminf(r * (largest / kLeast), 3.0e38f)};
+    if (!(m < __builtin_inff())) return {__builtin_nanf(""), 0.0f, false};
+    const bool up = v < kSmall;
+    if (m >= kLeast) return {m / largest, largest / (up ? v * kUp : v), up};
+    return {kLeast / largest, (up ? r / kUp : r) * (largest / kLeast), up};
 }
 
 // The codes of N values (4 or 8), the first in the lowest byte.  int8: adding 1.5 2^23
 // leaves rint(v mul) in the low bits of the sum, two's complement.
 template <int N>
-__device__ __forceinline__ uint64_t codes_of(const float (&v)[N], const Scale& s, int format) {
+__device__ __forceinline__ uint64_t codes_of(const float (&values)[N], const Scale& s, int format) {
     uint32_t q[2] = {0, 0};
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = values[e];
+    if (__ballot(s.up)) {  // hardly ever: no lane pays for it otherwise
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= s.up ? kUp : 1.0f;
+    }
     if (s.mul != 0.0f) {
 #pragma unroll
         for (int h = 0; h < N / 4; ++h) {

@@ -469,3 +469,30 @@ def test_past_2_31_elements(dev):
         want += terms.sum(0)
         size += terms.abs().sum(0)
     R.near("dgamma", host(dg), host(want), host(size) * (n / 256 / 2 + 100) * S.U)
+
+
+@pytest.mark.parametrize("block", [0, 128])
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("n,c", [(3, 5), (4, 40), (1030, 300), (1030, 1600), (5, 5000), (2, 14000)])
+def test_codes_of_small_products(dev, n, c, fmt, block):
+    """Without eps tiny rows are normalised like any others.  h gamma below 2^-110, whose factor
+    to a code passes fp32's range, but above its smallest normal numbers, 2^-126: rows whose
+    largest y is ordinary, one whose values are all small but in one block, and one below 2^-100."""
+    note(f"rmsnorm codes of small products {n}x{c} {fmt} block={block}")
+    code, largest, _ = FORMATS[fmt]
+    r = np.random.default_rng(c)
+    x = np.sign(r.standard_normal((n, c))) * r.uniform(0.5, 1.0, (n, c))
+    x[1] *= 2.0 ** 3
+    one = np.ones(c)
+    one[c // 2] = 2.0 ** 26
+    q = torch.full((n, c), 77, dtype=torch.uint8, device=dev)
+    scales = torch.full((n, M.row8_scales(1, c, block)), 77.0, device=dev)
+    for size, g in ((2.0 ** -30, one * 2.0 ** -86), (2.0 ** -30, np.full(c, 2.0 ** -92)),
+                    (2.0 ** -23, np.full(c, 0.7 * 2.0 ** -101))):
+        h32, g32 = (x * size).astype(np.float32), g.astype(np.float32)
+        M.rmsnorm_forward_row8(dev_t(h32), dev_t(g32), q, scales, None, None, n, c, 0.0, block, code)
+        h, _, y, _, rel_y = S.rms(h32.astype(np.float64), None, g32.astype(np.float64), 0.0)
+        assert np.abs(h * g32).min() > 2.0 ** -126
+        want, v = S.scales_of(y, block, largest)
+        R.near("scales", host(scales), want, (rel_y + 2 * S.U) * want)
+        R.near("codes", S.code_values(host(q), fmt), v, S.code_bound(v, fmt))
