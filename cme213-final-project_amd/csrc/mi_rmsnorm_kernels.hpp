@@ -562,7 +562,8 @@ __global__ __launch_bounds__(kBwdGroupThreads<GT>) void rms_bwd_kernel(
 
 // Backward, rows of less than a unit or too long for registers: a workgroup walks a row twice
 // and keeps its columns' sums in its partial row, each column with one thread.  A row's products
-// are added in 64 bits, as the forward kernel's squares are.
+// are added in 64 bits, as the forward kernel's squares are.  Rows of less than a unit can be
+// hundreds of millions: their columns' sums stay in a register, in 64 bits too.
 template <int T, bool ADD>
 __global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
     int rows, int cols, const void* dy, const void* __restrict__ x,
@@ -571,6 +572,8 @@ __global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
     __shared__ SumTop red[2][kThreads / kWave];
     GroupRed<kThreads> group{red};
     float* prow = part + static_cast<size_t>(blockIdx.x) * cols;
+    const bool narrow = cols < row_vec<T>();
+    double own = 0.0;  // the thread's column's, where narrow
     for (int c = threadIdx.x; c < cols; c += kThreads) prow[c] = 0.0f;
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const size_t base = static_cast<size_t>(row) * cols;
@@ -580,14 +583,20 @@ __global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
             s += static_cast<double>(row_get<T>(dy, base + c) * (row_get<T>(x, base + c) * r)) *
                  static_cast<double>(gamma[c]);
         const float m = group.sum(static_cast<float>(s)) / static_cast<float>(cols);
-        for (int c = threadIdx.x; c < cols; c += kThreads) {
+        auto put = [&](int c) {  // the row's gradient in column c; gives gamma's
             const float d = row_get<T>(dy, base + c), n = row_get<T>(x, base + c) * r;
             float v = r * (d * gamma[c] - n * m);
             if constexpr (ADD) v += row_get<T>(dx, base + c);
             row_put<T>(dx, base + c, rounded(v));
-            prow[c] += d * n;
+            return d * n;
+        };
+        if (narrow) {
+            if (static_cast<int>(threadIdx.x) < cols) own += static_cast<double>(put(threadIdx.x));
+        } else {
+            for (int c = threadIdx.x; c < cols; c += kThreads) prow[c] += put(c);
         }
     }
+    if (narrow && static_cast<int>(threadIdx.x) < cols) prow[threadIdx.x] = static_cast<float>(own);
 }
 
 // ---------------------------------------------------------------------------

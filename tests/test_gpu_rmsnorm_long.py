@@ -81,3 +81,18 @@ def test_gradient_of_long_rows_of_equal_values(dev, t, c, value, add):
         R.near("dx", _h64(dx[:, part]), w, bound + R.half_step(t, w) * (1 + 2.0 ** -9))
         w = np.full(300, 2 * d * norm)
         R.near("dgamma", _h64(dg[part]), w, 6 * S.U * w)
+
+
+@pytest.mark.parametrize("t,n,c", [("f32", 2 ** 24, 3), ("bf16", 2 ** 23 + 77, 5), ("f16", 2 ** 22, 1)])
+def test_many_rows_of_a_few_columns(dev, t, n, c):
+    """Gamma's gradient over millions of equal rows."""
+    note(f"rmsnorm many rows of a few columns {n}x{c} {t}")
+    x = torch.full((n, c), 0.7, dtype=R.TYPES[t], device=dev)
+    dy = torch.full((n, c), 1.001, dtype=R.TYPES[t], device=dev)
+    r = (1 / torch.sqrt(x[0, 0].double() ** 2 + EPS)).float()
+    inv = torch.full((n,), float(r), device=dev)
+    dx, dg = torch.empty_like(x), torch.full((c,), 5.0, device=dev)
+    M.rmsnorm_backward(dy, x, inv, torch.ones(c, device=dev), dx, dg, n, c)
+    want = n * _h64(dy)[0] * _h64(x)[0] * _h64(r)
+    # n = x r and its product once each, a workgroup's sum once, its 256 partial rows in 16 slices of 16, the old value
+    R.near("dgamma", _h64(dg), want + 5, (3 + 32) * S.U * want + S.U * (want + 5))
