@@ -137,14 +137,22 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 
-// sum c_e P_e over the workgroups that add partial rows, as whole numbers, which come out the same
-// in any order: each adds its share of n k, the largest such sum, in units of 2^-49 of it, to bits 7
-// to 56 of one word, 1 to the bits below, so that the last one knows that it is, and 1 to those
-// above where its share is no number.  The word says all, so nothing has to be ordered by it.
+// sum c_e P_e over the workgroups that add partial rows.  Each adds its share of n k, the largest
+// such sum, in units of 2^-49 of it, to bits 7 to 56 of one word, 1 to the bits below, so that the
+// last one knows that it is, and 1 to those above where its share is no number: as whole numbers
+// they add up the same in any order, and the word says all, so nothing has to be ordered by it.
+// A share loses less than a unit: a sum of less than kEnough of them (the chosen experts have hardly
+// any probability, 1 / E where the router is balanced) is added again from the shares themselves,
+// in 64 bits, which every workgroup writes when it has counted itself.
+constexpr int kMaxFin = kMaxExperts / kFinExperts;
+constexpr double kShare = 0x1p49;
+constexpr unsigned long long kEnough = 1ull << 32;  // 64 units lost are 2^-26 of it
+constexpr unsigned long long kNone = ~0ull;         // a share not written yet: NaN bits that none has
+
 struct Finish {
     unsigned long long word;
+    unsigned long long share[kMaxFin];
 };
-constexpr double kShare = 0x1p49;
 
 // Sums of the probabilities and counts over a workgroup's tokens: a lane adds its experts'
 // over its rows in registers, the waves' sums meet in LDS, in order.  ONE: the only
@@ -210,7 +218,6 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
     Row r0, r1;
     if (tokens > 0) load(base, r0);
     for (int e = threadIdx.x; e <= experts; e += kFwdThreads) count[e] = 0;
-    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) finish->word = 0;
     __syncthreads();
     while (base < tokens) {
         load(base + stride, r1);
@@ -268,6 +275,10 @@ __global__ __launch_bounds__(kFwdThreads) void balance_fwd_kernel(
             counts[experts] = n;
         }
     } else {
+        if (blockIdx.x == 0) {
+            if (threadIdx.x == 0) finish->word = 0;
+            if (threadIdx.x < kMaxFin) finish->share[threadIdx.x] = kNone;
+        }
         for (int e = threadIdx.x; e < experts; e += kFwdThreads) {
             float s = sums[0][e];
 #pragma unroll
@@ -343,20 +354,40 @@ __global__ __launch_bounds__(kFinThreads) void balance_finish_kernel(
         share = static_cast<double>(m) * static_cast<double>(mean);
     }
     share = wave_sum_d(share);
-    if (threadIdx.x != 0) return;
     const double most = static_cast<double>(k) * max(n, 1);
     const bool number = share - share == 0.0;
-    const unsigned long long own =
-        (number ? static_cast<unsigned long long>(share / most * kShare) << 7 : 1ull << 57) + 1;
-    const unsigned long long word =
-        own + __hip_atomic_fetch_add(&finish->word, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    unsigned long long word = 0;
+    if (threadIdx.x == 0) {
+        const unsigned long long own =
+            (number ? static_cast<unsigned long long>(share / most * kShare) << 7 : 1ull << 57) + 1;
+        word = own + __hip_atomic_fetch_add(&finish->word, own, __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+        // behind it, for what comes before it is waited for together with it
+        __hip_atomic_store(&finish->share[blockIdx.x],
+                           static_cast<unsigned long long>(__double_as_longlong(number ? share : 0.0)),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    word = __shfl(word, 0);
     if ((word & 127) != gridDim.x) return;
-    const double all = static_cast<double>(word >> 7 & ((1ull << 50) - 1)) / kShare * most;
+    const unsigned long long units = word >> 7 & ((1ull << 50) - 1);
+    double all = static_cast<double>(units) / kShare * most;
+    if (units < kEnough) {
+        // Every workgroup has counted itself, and its share comes right behind: the wait for it ends.
+        unsigned long long bits = 0;
+        if (threadIdx.x < gridDim.x) {
+            do {
+                bits = __hip_atomic_load(&finish->share[threadIdx.x], __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+            } while (bits == kNone);
+        }
+        all = wave_sum_d(__longlong_as_double(static_cast<long long>(bits)));
+    }
+    if (threadIdx.x != 0) return;
     *loss = word >> 57 ? __builtin_nanf("") : loss_of(all, experts, k, n, coef);
     counts[experts] = n;
 }
-static_assert(kMaxExperts / kFinExperts < 128 && kFwdBlocks <= kFinThreads,
-              "7 bits count the workgroups; a thread for each partial row");
+static_assert(kMaxFin <= kWave && kFwdBlocks <= kFinThreads,
+              "a lane for each workgroup's share, of which 7 bits count; a thread for each partial row");
 
 // The counts enter less a whole number near their mean, which changes nothing (the p of a row
 // add up to 1) and keeps the bits of what is left.

@@ -452,7 +452,8 @@ int mi_moe_gate_backward(const void* logits, const int* ids, const float* weight
  * counts[experts] = n; probs[e] = the mean of their p_te, the softmax of their logits over all
  * experts (0 for a row of -inf alone); *loss = coef experts / (k n) sum_e counts[e] probs[e],
  * 0 where n is 0.  counts is [experts + 1].  All three are overwritten; sums over the tokens
- * are formed in fp32 in a fixed order, through the library workspace. */
+ * are formed in fp32 in a fixed order, through the library workspace, the loss's over the
+ * experts in 64 bits: its relative error does not grow where it is small. */
 int mi_moe_balance_forward(const void* logits, const int* ids, const unsigned char* valid,
                            int* counts, float* probs, float* loss, int tokens, int experts, int k,
                            float coef, int type, void* stream);

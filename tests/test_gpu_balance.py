@@ -249,3 +249,60 @@ def test_past_2_31_elements(dev):
     for part in (slice(0, 50), slice(n - 50, n)):
         g, bound = S.balance_back(_h64(l[part]), None, host(counts), 1e6, k, COEF)
         R.near("dlogits", _h64(d[part]), g, bound + R.half_step("bf16", g) * (1 + 2.0 ** -9))
+
+
+def _unlikely(n, e, k, low, seed):
+    """Logits near 0, near `low` for the first half of the experts, which all ids are of."""
+    r = np.random.default_rng(seed)
+    l = r.standard_normal((n, e))
+    l[:, :(e + 1) // 2] += low
+    return l.astype(np.float32), r.integers(0, (e + 1) // 2, (n, k)).astype(np.int32)
+
+
+@pytest.mark.parametrize("low", [-8, -14, -20, -30, -45, -75])
+@pytest.mark.parametrize("n,e,k", [(200, 64, 2), (300, 64, 2), (9000, 8, 1), (2000, 1000, 4)])
+def test_loss_of_unlikely_experts(dev, n, e, k, low):
+    """Ids that a bias or a group chose, whose experts have hardly any probability: the loss is
+    good to fp32 however small it is, by one workgroup and by many."""
+    note(f"balance {n}x{e} k={k}, chosen experts' logits {low}")
+    l, ids = _unlikely(n, e, k, low, n + e)
+    counts, probs = torch.empty(e + 1, dtype=torch.int32, device=dev), torch.empty(e, device=dev)
+    loss = torch.full((1,), 77.0, device=dev)
+    M.moe_balance_forward(dev_t(l), dev_t(ids), None, counts, probs, loss, n, e, k, COEF)
+    c, p, p_bound, want, bound = S.balance(l.astype(np.float64), ids, None, k, COEF)
+    assert_exact("counts", host(counts), c)
+    R.near("probs", host(probs), p, p_bound + 2.0 ** -140)
+    R.near("loss", host(loss), [want], [bound])
+    # and of the probabilities that the call wrote, to a rounding of the loss and of its last sum
+    own = COEF * e / (k * n) * (c[:e] * host(probs).astype(np.float64)).sum()
+    R.near("loss", host(loss), [own], [4 * S.U * own])
+    before = host(loss).copy()
+    M.moe_balance_forward(dev_t(l), dev_t(ids), None, counts, probs, loss, n, e, k, COEF)
+    assert host(loss)[0] == before[0]
+
+
+def test_loss_of_unlikely_experts_from_a_graph(dev):
+    """Replays with other calls on the workspace between them, likely and unlikely in turn."""
+    n, e, k = 3000, 96, 2
+    counts, probs = torch.empty(e + 1, dtype=torch.int32, device=dev), torch.empty(e, device=dev)
+    losses = torch.empty(2, device=dev)
+    inputs = [tuple(dev_t(x) for x in _unlikely(n, e, k, low, 1)) for low in (-25, 0)]
+
+    def step(which):
+        l, ids = inputs[which]
+        M.moe_balance_forward(l, ids, None, counts, probs, losses[which:which + 1], n, e, k, COEF)
+    step(0), step(1)
+    torch.cuda.synchronize()
+    want = losses.clone()
+    assert 0 < want[0] < 1e-9 < 1e-4 < want[1]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(0), step(1), step(0)
+    for rep in range(4):
+        losses.fill_(77)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(losses, want), rep
+        step(1)
+        torch.cuda.synchronize()
+        assert torch.equal(losses, want), rep
