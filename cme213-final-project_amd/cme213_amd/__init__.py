@@ -263,8 +263,8 @@ class Bound:
     at call time unless one was given.  The tensors, and a TensorList whose
     args() are among the arguments, are kept alive with the binding.  A
     list's own checks are made: that what is written overlaps nothing else of
-    it, once, and the current device, at every call.  Raises MIError on a
-    non-zero status, like the wrappers."""
+    the call, once, and the current device, at every call.  Raises MIError on
+    a non-zero status, like the wrappers."""
 
     def __init__(self, name, *args, stream=None):
         import torch
@@ -286,7 +286,8 @@ class Bound:
         for x in {id(a.tensors): a.tensors for a in args if isinstance(a, _ListAddress)}.values():
             if name in ("mi_tensors_scale", "mi_tensors_clip"):
                 # without its outs a list's tensors are what is written
-                (x if args[1] is not None else TensorList(x.tensors))._written()
+                (x if args[1] is not None else TensorList(x.tensors))._written(
+                    *[c.value for c in conv[5:] if isinstance(c, c_void_p)])
             _same_device(x.device)
             self._device = x.device
 
@@ -723,6 +724,7 @@ class TensorList:
         self._sizes = (c_longlong * n)(*sizes)
         self._types = (c_int * n)(*[codes[t.dtype] for t in self.tensors])
         self._data, self._outs, self._apart = self._addresses(self.tensors), None, None
+        self._beside = ()  # the last call's scalars
         if outs is not None:
             for i, o in enumerate(self.out_tensors):
                 if o.dtype != torch.float32:
@@ -754,8 +756,9 @@ class TensorList:
         _same_device(self.device)
         return self._arrays + (self.count,)
 
-    def _written(self):
-        """args(), where what is written overlaps nothing else of the list."""
+    def _written(self, *scalars):
+        """args(), where what is written overlaps nothing else of the list, and fp32 scalars at
+        these addresses are none of its elements."""
         if self._apart is None:
             def ranges(tensors):
                 return sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
@@ -768,6 +771,13 @@ class TensorList:
                                   for a, b in ranges(self.tensors))
         if not self._apart:
             raise ValueError("tensors that are written overlap others of the list")
+        if scalars != self._beside:
+            for t in self.tensors + (self.out_tensors or []):
+                begin = t.data_ptr()
+                end = begin + t.numel() * t.element_size()
+                if any(begin < p + 4 and p < end for p in scalars if p is not None):
+                    raise ValueError("a scalar of the call lies in a tensor of the list")
+            self._beside = scalars
         return self._here()
 
 
@@ -782,16 +792,17 @@ def tensors_norm_sq_acc(tensors, result, stream=None):
 def tensors_scale(tensors, scale, stream=None):
     """Every tensor of a TensorList times the device scalar, in place or into its outs."""
     import torch
-    _check(lib.mi_tensors_scale(*tensors._written(), _buf(scale, 1, torch.float32),
-                                _stream(stream)))
+    scale = _buf(scale, 1, torch.float32)
+    _check(lib.mi_tensors_scale(*tensors._written(scale), scale, _stream(stream)))
 
 
 def tensors_clip(tensors, max_norm, norm_sq, clip_scale, stream=None):
     """Clips a TensorList by its global norm: norm_sq and clip_scale are overwritten, then every
     tensor is scaled, in place or into its outs."""
     import torch
-    _check(lib.mi_tensors_clip(*tensors._written(), max_norm, _buf(norm_sq, 1, torch.float32),
-                               _buf(clip_scale, 1, torch.float32), _stream(stream)))
+    norm_sq, clip_scale = _buf(norm_sq, 1, torch.float32), _buf(clip_scale, 1, torch.float32)
+    _check(lib.mi_tensors_clip(*tensors._written(norm_sq, clip_scale), max_norm, norm_sq,
+                               clip_scale, _stream(stream)))
 
 
 # ----- mixture of experts ----------------------------------------------------------

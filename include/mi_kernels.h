@@ -365,13 +365,14 @@ int mi_tensors_norm_sq_acc(const void* const* tensors, const long long* sizes, c
 /* Every element times *d_scale: in place, rounded to its type (outs NULL; nothing is read
  * or written where the scale is 1), or as fp32 in outs[i] (e.g. pieces of the flat buffer that
  * mi_adam_clipped takes).  Tensors to be scaled in place must not overlap each other, outs
- * neither each other nor the tensors. */
+ * neither each other nor the tensors; *d_scale lies in none of them. */
 int mi_tensors_scale(const void* const* tensors, void* const* outs, const long long* sizes,
                      const int* types, int count, const float* d_scale, void* stream);
 
 /* Clipping by the global norm: *d_norm_sq = sum of all elements' squares (overwritten),
  * *d_clip_scale as mi_compute_clip_scale's, then mi_tensors_scale with it.  An infinite norm
- * gives the scale 0, a NaN the scale 1, as there. */
+ * gives the scale 0, a NaN the scale 1, as there.  *d_norm_sq and *d_clip_scale lie apart, in
+ * none of the tensors and outs. */
 int mi_tensors_clip(const void* const* tensors, void* const* outs, const long long* sizes,
                     const int* types, int count, float max_norm, float* d_norm_sq,
                     float* d_clip_scale, void* stream);

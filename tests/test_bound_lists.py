@@ -115,3 +115,34 @@ def test_a_bound_call_makes_the_lists_checks(name, monkeypatch):
     assert len(calls) == 1
     _bind(name, elsewhere)()
     assert len(calls) == 2
+
+
+def _calls(x):
+    """The calls that write a list's tensors, as functions of where their scalars are."""
+    return [lambda a: M.tensors_scale(x, a, stream=0), lambda a: M.tensors_clip(x, 1.0, a, P, stream=0),
+            lambda a: M.tensors_clip(x, 1.0, P, a, stream=0),
+            lambda a: M.bind("mi_tensors_scale", *x.args(), a, stream=0)(),
+            lambda a: M.bind("mi_tensors_clip", *x.args(), 1.0, a, P, stream=0)(),
+            lambda a: M.bind("mi_tensors_clip", *x.args(), 1.0, P, a, stream=0)()]
+
+
+@pytest.mark.parametrize("with_outs", [False, True])
+def test_scalars_lie_outside_the_list(monkeypatch, with_outs):
+    """A scale, norm or clip scale among the elements would be written while others read it."""
+    made = []
+    for name in CALLS:
+        monkeypatch.setattr(M.lib, name, lambda *a: made.append(a) or M.MI_OK)
+    outs = [Stand(0x8000, 4), Stand(0x9000, 100)] if with_outs else None
+    x = M.TensorList([Stand(0x1000, 4, torch.float16), Stand(0x2000, 100)], outs)
+    inside = [0x1000, 0x1004, 0xffe, 0x2000, 0x218c, 0x218e] + [0x8000, 0x918c] * with_outs
+    outside = [0xffc, 0x1008, 0x1ffc, 0x2190] + ([0x7ffc, 0x9190] if with_outs else [0x8000])
+    for call in _calls(x):
+        for a in inside:
+            n = len(made)
+            with pytest.raises(ValueError, match="scalar"):
+                call(a)
+            assert len(made) == n
+        for a in outside + outside:
+            n = len(made)
+            call(a)
+            assert len(made) == n + 1
