@@ -705,7 +705,9 @@ class TensorList:
     """A program's gradients (float32, float16 and bfloat16 CUDA tensors, contiguous, on one
     device) as the mi_tensors_* calls take them, and where their clipped values go: `outs`,
     float32 tensors of as many elements each, or None for in place.  The tensors are kept alive
-    with the list; it is made once and used every step, with the memory that they had then."""
+    with the list, which is of the memory that they had when it was made: it is made once for
+    gradients that are cleared in place (zero_grad(set_to_none=False)), and again after every
+    backward pass for gradients that are dropped, or it would clip the dropped ones."""
 
     def __init__(self, tensors, outs=None):
         import torch

@@ -240,3 +240,27 @@ def test_past_2_31_elements(dev):
     for part in (slice(0, 9000), slice(n - 9000, n - 1)):
         assert torch.equal(x[part], (torch.full((1,), 0.5, device=dev) * c).bfloat16().expand(len(x[part])))
     assert x[-1] == (2 * c).bfloat16()
+
+
+@pytest.mark.parametrize("again", [False, True])
+def test_gradients_of_several_steps(dev, again):
+    """A list is of the memory that the gradients had when it was made: made once for gradients
+    that are cleared where they are, or made again each step for gradients that are dropped."""
+    r = np.random.default_rng(8)
+    params = [torch.from_numpy(r.standard_normal(s).astype(np.float32)).to(dev, t).requires_grad_()
+              for s, t in (((30, 7), torch.float32), ((501,), torch.bfloat16), ((3, 3000), torch.float32))]
+    optimizer = torch.optim.SGD(params, lr=0.1)
+    flat = torch.zeros(sum(p.numel() for p in params), device=dev)
+    n2, c = _one(0), _one(0)
+    grads = None
+    for step in range(3):
+        optimizer.zero_grad(set_to_none=again)
+        x = [torch.from_numpy(r.standard_normal(p.shape).astype(np.float32)).to(dev, p.dtype) for p in params]
+        sum((p * y).float().sum() for p, y in zip(params, x)).backward()
+        if again or grads is None:
+            grads = M.TensorList([p.grad for p in params],
+                                 list(flat.split([p.numel() for p in params])))
+        M.tensors_clip(grads, 1.0, n2, c)
+        want = _norm_sq(x)  # the gradients of this step are x
+        assert abs(host(n2)[0] - want) <= (S.norm_chain(flat.numel()) + 4) * S.U * want
+        assert torch.equal(flat, torch.cat([y.float().reshape(-1) for y in x]) * c)
