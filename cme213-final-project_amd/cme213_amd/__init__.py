@@ -286,7 +286,8 @@ class Bound:
         for x in {id(a.tensors): a.tensors for a in args if isinstance(a, _ListAddress)}.values():
             if name in ("mi_tensors_scale", "mi_tensors_clip"):
                 # without its outs a list's tensors are what is written
-                (x if args[1] is not None else TensorList(x.tensors))._written(
+                own = (args[1] is None) == (x.out_tensors is None)
+                (x if own else TensorList(x.tensors))._written(
                     *[c.value for c in conv[5:] if isinstance(c, c_void_p)])
             _same_device(x.device)
             self._device = x.device

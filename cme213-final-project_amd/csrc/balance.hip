@@ -9,9 +9,11 @@
 //
 // A row's logits lie in the registers of L lanes as in the router's kernels, and are read once.
 // Backward: bound by memory, [65536, 256] fp32 added to what is there 37.3 us, 5.4 TB/s, [32768,
-// 256] bf16 7.7 us, 4.4 TB/s.  Forward: [32768, 256] bf16, 8 slots, 10.8 us for 18 MB: its first
-// launch (8) is bound by instructions (exp2 at a quarter rate, the row's sums and maxima) and a
-// workgroup's start and end, its second (3) by the round trips to the partial rows and to the word.
+// 256] bf16 7.7 us, 4.4 TB/s.  Forward: [32768, 256] bf16, 8 slots, 10.7 us for 18 MB.  Its first
+// launch (7.6) takes 5.0 for 300 tokens and 5.3 for 4096: a workgroup's start, the exchange of its
+// waves' sums and its end.  What more tokens add is bound by memory (131072 17.5 us, 262144 29.3: 90
+// ps and 544 bytes each, 6.0 TB/s).  The second (3) is bound by the round trips to the partial rows
+// and to the word.
 #include <algorithm>
 #include <climits>
 #include <type_traits>

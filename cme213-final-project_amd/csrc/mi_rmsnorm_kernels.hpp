@@ -2,7 +2,8 @@
 // addition and with an output in 8 bits.  Beside the LayerNorm of
 // FINAL_CLEAN_CODE/src/kernels/layernorm.cu:10-308 (its fused residual form and
 // its backward into the residual stream's gradient); the reference has no RMS
-// norm.  Rows are fp32, fp16 or bf16; gamma, statistics and sums fp32.
+// norm.  Rows are fp32, fp16 or bf16; gamma, statistics and sums fp32 (64 bits where a thread adds
+// thousands of numbers one after another).
 //
 //   h = a + b (or x);  r = 1 / sqrt(mean(h^2) + eps);  y = h r gamma
 //   dx = r (g - n mean(g n)),  n = h r,  g = dy gamma;  dgamma += sum_rows dy n
@@ -359,7 +360,9 @@ __global__ __launch_bounds__(kGroupThreads<GT>) void rms_fwd_kernel(
 // Forward, rows of less than a unit or more than the registers hold: a workgroup a row,
 // which it walks twice.  A wave takes 128 columns at a time, the columns of a scale.  A thread adds
 // up to 65536 columns one after another, in 64 bits: in 32 the roundings of equal values go the
-// same way, and the sum is off by 9e-4.
+// same way, and the sum is off by 9e-4.  Bound by single-element loads and, where rows are few, by
+// one workgroup's walk: [2048, 16384] fp32 with the residual 160 us (537 MB, 3.4 TB/s), [64, 131072]
+// bf16 328 us (67 MB).
 template <int T, bool RESID, Out OUT>
 __global__ __launch_bounds__(kThreads) void rms_fwd_walk_kernel(
     int rows, int cols, const void* a, const void* b, const float* __restrict__ gamma,
@@ -563,7 +566,9 @@ __global__ __launch_bounds__(kBwdGroupThreads<GT>) void rms_bwd_kernel(
 // Backward, rows of less than a unit or too long for registers: a workgroup walks a row twice
 // and keeps its columns' sums in its partial row, each column with one thread.  A row's products
 // are added in 64 bits, as the forward kernel's squares are.  Rows of less than a unit can be
-// hundreds of millions: their columns' sums stay in a register, in 64 bits too.
+// hundreds of millions: their columns' sums stay in a register, in 64 bits too.  Bound as the
+// forward kernel, and by the partial row's read and write beside each element: [2048, 16384] fp32
+// onto the residual stream's gradient 491 us (537 MB), [64, 131072] bf16 353 us.
 template <int T, bool ADD>
 __global__ __launch_bounds__(kThreads) void rms_bwd_walk_kernel(
     int rows, int cols, const void* dy, const void* __restrict__ x,
