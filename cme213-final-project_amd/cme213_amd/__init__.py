@@ -287,9 +287,8 @@ class Bound:
             if name in ("mi_tensors_scale", "mi_tensors_clip"):
                 # without its outs a list's tensors are what is written
                 own = (args[1] is None) == (x.out_tensors is None)
-                (x if own else TensorList(x.tensors))._written(
-                    *[c.value for c in conv[5:] if isinstance(c, c_void_p)])
-            _same_device(x.device)
+                (x if own else TensorList(x.tensors))._check_apart(
+                    [c.value for c in conv[5:] if isinstance(c, c_void_p)])
             self._device = x.device
 
     def __call__(self):
@@ -727,7 +726,6 @@ class TensorList:
         self._sizes = (c_longlong * n)(*sizes)
         self._types = (c_int * n)(*[codes[t.dtype] for t in self.tensors])
         self._data, self._outs, self._apart = self._addresses(self.tensors), None, None
-        self._beside = ()  # the last call's scalars
         if outs is not None:
             for i, o in enumerate(self.out_tensors):
                 if o.dtype != torch.float32:
@@ -762,26 +760,36 @@ class TensorList:
     def _written(self, *scalars):
         """args(), where what is written overlaps nothing else of the list, and fp32 scalars at
         these addresses are none of its elements."""
+        self._check_apart(scalars)
+        return self._here()
+
+    def _check_apart(self, scalars):
         if self._apart is None:
             def ranges(tensors):
                 return sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
                               for t in tensors if t.numel())
-            outs = ranges(self.tensors if self._outs is None else self.out_tensors)
+            read = ranges(self.tensors)
+            outs = read if self._outs is None else ranges(self.out_tensors)
             self._apart = all(a[1] <= b[0] for a, b in zip(outs, outs[1:]))
+            self._starts, self._ends = [a for a, _ in outs], [b for _, b in outs]
             if self._apart and self._outs is not None:
-                starts, ends = [a for a, _ in outs], [b for _, b in outs]
-                self._apart = all(bisect.bisect_right(ends, a) == bisect.bisect_left(starts, b)
-                                  for a, b in ranges(self.tensors))
+                self._apart = all(bisect.bisect_right(self._ends, a) ==
+                                  bisect.bisect_left(self._starts, b) for a, b in read)
+                # all that the list has, tensors that overlap each other as one
+                self._starts, self._ends = [], []
+                for a, b in sorted(read + outs):
+                    if self._ends and a <= self._ends[-1]:
+                        self._ends[-1] = max(self._ends[-1], b)
+                    else:
+                        self._starts.append(a)
+                        self._ends.append(b)
         if not self._apart:
             raise ValueError("tensors that are written overlap others of the list")
-        if scalars != self._beside:
-            for t in self.tensors + (self.out_tensors or []):
-                begin = t.data_ptr()
-                end = begin + t.numel() * t.element_size()
-                if any(begin < p + 4 and p < end for p in scalars if p is not None):
+        for p in scalars:
+            if p is not None:
+                i = bisect.bisect_left(self._starts, p + 4) - 1  # the last that begins before its end
+                if i >= 0 and self._ends[i] > p:
                     raise ValueError("a scalar of the call lies in a tensor of the list")
-            self._beside = scalars
-        return self._here()
 
 
 def tensors_norm_sq_acc(tensors, result, stream=None):

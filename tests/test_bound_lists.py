@@ -1,5 +1,6 @@
-"""CPU checks of lists of tensors in bound calls: what a bound call will read stays alive with it.
-The tensors are stand-ins, and no bound call is made."""
+"""CPU checks of lists of tensors in calls: what a bound call will read stays alive with it, and
+what is written overlaps nothing else of the call.  The tensors are stand-ins; the library's
+functions are not called, or replaced."""
 import gc
 import weakref
 
@@ -80,8 +81,8 @@ def test_the_arguments_alone_keep_the_list():
 
 @pytest.mark.parametrize("name", CALLS)
 def test_a_bound_call_makes_the_lists_checks(name, monkeypatch):
-    """What is written overlaps nothing else of the list; the current device is the tensors', when
-    the call is bound and when it is made."""
+    """What is written overlaps nothing else of the list, when the call is bound; the current
+    device is the tensors', when it is made."""
     def args(tensors, outs=None):
         return M.TensorList([Stand(*t) for t in tensors],
                             outs and [Stand(*t) for t in outs]).args()
@@ -101,19 +102,19 @@ def test_a_bound_call_makes_the_lists_checks(name, monkeypatch):
         _bind(name, both)
         with pytest.raises(ValueError, match="overlap"):
             _bind(name, (both[0], None) + both[2:])
-    elsewhere = args([(0x1000, 4, torch.float32, 1)])
-    with pytest.raises(ValueError, match="current device"):
-        _bind(name, elsewhere)
     calls = []
     monkeypatch.setattr(M.lib, name, lambda *a: calls.append(a) or M.MI_OK)
     monkeypatch.setattr(M, "_current_stream", lambda: None)
     bound = _bind(name, apart)
+    elsewhere = _bind(name, args([(0x1000, 4, torch.float32, 1)]))
     bound()
+    with pytest.raises(ValueError, match="current device"):
+        elsewhere()
     monkeypatch.setattr(M, "_current_device", lambda: 1)
     with pytest.raises(ValueError, match="current device"):
         bound()
     assert len(calls) == 1
-    _bind(name, elsewhere)()
+    elsewhere()
     assert len(calls) == 2
 
 
